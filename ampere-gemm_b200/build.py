@@ -1,4 +1,4 @@
-"""Ahead-of-time build of the native GEMM library for sm_100a.
+"""Ahead-of-time build of the native library for sm_100a.
 
 Produces ``tensorcore_gemm/_lib/libb200gemm.so`` next to the Python package,
 in-tree, so a snapshot of the repository carries the built library with it.
@@ -12,10 +12,12 @@ Usage:  python ampere-gemm_b200/build.py [--force] [--verbose]
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -29,7 +31,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xptxas", "-v",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden",
 ]
 
@@ -53,18 +55,28 @@ def needs_build() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile csrc/b200_gemm.cu into the in-tree shared library."""
+    """Compile every csrc/*.cu (in parallel) and link the in-tree shared library."""
     if not force and not needs_build():
         return LIB_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(CSRC / "b200_gemm.cu")]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    log = proc.stdout + proc.stderr
-    (LIB_DIR / "build.log").write_text(" ".join(cmd) + "\n" + log)
-    if proc.returncode != 0:
+    nvcc = _nvcc()
+    with tempfile.TemporaryDirectory(prefix="b200_build_") as tmp_dir:
+        units = sorted(CSRC.glob("*.cu"))
+        objects = [Path(tmp_dir) / (u.stem + ".o") for u in units]
+        cmds = [[nvcc, *NVCC_FLAGS, "-c", "-o", str(o), str(u)] for u, o in zip(units, objects)]
+        tmp = LIB_PATH.with_suffix(".so.tmp")
+        link = [nvcc, *NVCC_FLAGS[:2], "-shared", "-o", str(tmp), *map(str, objects)]
+        with concurrent.futures.ThreadPoolExecutor(len(cmds)) as pool:
+            procs = list(pool.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds))
+        if all(p.returncode == 0 for p in procs):
+            cmds.append(link)
+            procs.append(subprocess.run(link, capture_output=True, text=True))
+    log = "".join(" ".join(c) + "\n" + p.stdout + p.stderr for c, p in zip(cmds, procs))
+    (LIB_DIR / "build.log").write_text(log)
+    failed = [p.returncode for p in procs if p.returncode != 0]
+    if failed:
         sys.stderr.write(log)
-        raise RuntimeError(f"nvcc failed building {LIB_PATH.name} (exit {proc.returncode})")
+        raise RuntimeError(f"nvcc failed building {LIB_PATH.name} (exit {failed[0]})")
     if verbose:
         sys.stdout.write(log)
     tmp.replace(LIB_PATH)

@@ -35,6 +35,7 @@
 #include "kernel_cta1.cuh"
 #include "kernel_cta2.cuh"
 #include "kernel_skinny.cuh"
+#include "tensor_map.cuh"
 #include "../../include/b200_gemm.h"
 
 namespace b200 {
@@ -58,171 +59,6 @@ __global__ void bounded_wait_selftest_kernel(uint64_t limit_ns) {
 // ===========================================================================
 namespace b200 {
 namespace {
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-constexpr int kMaxDevices = 64;
-
-struct DeviceInfo {
-  bool ready = false;
-  bool sm100 = false;
-  int sm_count = 0;
-  int64_t l2_bytes = 0;
-};
-
-std::mutex g_dev_mu;
-DeviceInfo g_dev[kMaxDevices];
-
-int current_device_info(DeviceInfo& out) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return B200_ERR_CUDA;
-  std::lock_guard<std::mutex> lk(g_dev_mu);
-  DeviceInfo& d = g_dev[dev];
-  if (!d.ready) {
-    int major = 0, sms = 0, l2 = 0;
-    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess)
-      return B200_ERR_CUDA;
-    d.sm100 = (major == 10);
-    d.sm_count = sms;
-    d.l2_bytes = l2;
-    d.ready = true;
-  }
-  out = d;
-  return B200_OK;
-}
-
-// 2-D fp16 tensor map over a row-major matrix of `rows` x `cols` (cols
-// contiguous, `ld` elements between rows), box `box_cols` x `box_rows`,
-// 128-byte swizzle, zero fill out of bounds.
-int encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
-                   uint32_t box_rows, CUtensorMapL2promotion promo) {
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) return B200_ERR_TENSOR_MAP;
-  // A zero-extent dimension is not encodable; callers never pass one.
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld * 2};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  auto encode = [&] {
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = encode();
-  if (r == CUDA_ERROR_INVALID_CONTEXT) {
-    // A thread that has made no runtime call yet (e.g. autograd's device
-    // thread) has no current context for this driver call: cudaSetDevice on
-    // the current device makes the primary context current, then retry.
-    int dev = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
-  }
-  if (r != CUDA_SUCCESS && std::getenv("B200_GEMM_DEBUG"))
-    std::fprintf(stderr, "b200_gemm: tensor map rejected (%d): base %p rows %llu cols %llu ld %llu box %u x %u\n",
-                 (int)r, base, (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld, box_cols,
-                 box_rows);
-  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
-}
-
-// Encoding a tensor map is a driver call of about a microsecond; repeated
-// GEMMs on the same buffers reuse the encoded map from a small per-thread
-// cache keyed by every field that goes into it.
-struct TmapKey {
-  const void* base;
-  uint64_t rows, cols, ld;
-  uint32_t box_cols, box_rows, promo;
-  bool operator==(const TmapKey& o) const {
-    return base == o.base && rows == o.rows && cols == o.cols && ld == o.ld && box_cols == o.box_cols &&
-           box_rows == o.box_rows && promo == o.promo;
-  }
-};
-
-struct TmapCache {
-  static constexpr int kEntries = 24;
-  TmapKey key[kEntries];
-  CUtensorMap map[kEntries];
-  bool used[kEntries] = {};
-  int next = 0;
-};
-
-int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
-                 uint32_t box_rows, CUtensorMapL2promotion promo) {
-  static thread_local TmapCache cache;
-  const TmapKey k{base, rows, cols, ld, box_cols, box_rows, static_cast<uint32_t>(promo)};
-  for (int i = 0; i < TmapCache::kEntries; ++i) {
-    if (cache.used[i] && cache.key[i] == k) {
-      *map = cache.map[i];
-      return B200_OK;
-    }
-  }
-  const int rc = encode_tmap_2d(map, base, rows, cols, ld, box_cols, box_rows, promo);
-  if (rc != B200_OK) return rc;
-  const int slot = cache.next;
-  cache.next = (cache.next + 1) % TmapCache::kEntries;
-  cache.key[slot] = k;
-  cache.map[slot] = *map;
-  cache.used[slot] = true;
-  return B200_OK;
-}
-
-// cudaFuncSetAttribute once per (kernel instantiation, device); `done` is
-// the calling launch template's own flag array (all kernels share one
-// function-pointer type, so the flags cannot live here).
-template <typename Kern>
-int ensure_smem_attr(Kern kern, int smem_bytes, std::atomic<uint8_t>* done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return B200_ERR_CUDA;
-  if (dev >= 0 && dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return B200_OK;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess)
-    return B200_ERR_CUDA;
-  if (dev >= 0 && dev < kMaxDevices) done[dev].store(1, std::memory_order_release);
-  return B200_OK;
-}
-
-// GEMM kernels go out with programmatic stream serialisation (PDL): a kernel
-// may be scheduled while the previous one on the stream drains, runs its
-// setup (barriers, TMEM, tensor-map prefetch), and waits in griddep_wait()
-// before its first global access.  B200_GEMM_PDL=0 turns it off.
-bool pdl_enabled() {
-  static const bool on = [] {
-    const char* e = std::getenv("B200_GEMM_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_gemm(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                        Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-  if (e != cudaSuccess) (void)cudaGetLastError();
-  return e;
-}
 
 // One GEMM call as the launchers see it (operands already TMA-compatible).
 struct GemmArgs {
@@ -278,29 +114,6 @@ int launch_tcgen05(const GemmArgs& g, int group_m) {
   const cudaError_t le = launch_gemm(kern, dim3(grid), dim3(kThreads), Cfg::kSmemBytes, stream, ta, tb, tc, M, N, K,
                                      group_m, g.scale);
   return le == cudaSuccess ? B200_OK : B200_ERR_CUDA;
-}
-
-// Largest number of 2-CTA clusters of `kern` that can be resident at once
-// (clusters need both SMs in one GPC, so this can be below sm_count / 2).
-template <typename Kern>
-int max_active_pairs(Kern kern, int smem_bytes, int sm_count) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (sm_count / 2), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = sm_count / 2;
-  }
-  return n;
 }
 
 // ---- split of the last wave along K (pair kernel, MSUB = 1) ----
@@ -661,8 +474,6 @@ bool dyn_tiles() {
   return on;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace b200
 
@@ -694,8 +505,6 @@ int validate_args(const void* C, int64_t M, int64_t N, int64_t K, int64_t lda, i
   }
   return B200_OK;
 }
-
-bool pitch_ok(const void* p, int64_t ld) { return aligned16(p) && (ld % 8) == 0; }
 
 // C <- fp16_rn(beta * C) for an empty reduction (K == 0) with beta != 0.
 __global__ void scale_c_kernel(uint16_t* C, int64_t ldc, int64_t rows, int64_t cols, float beta) {
@@ -809,8 +618,6 @@ struct RepackPlan {
   int64_t lda2 = 0, ldb2 = 0, ldc2 = 0;
   int64_t off_a = 0, off_b = 0, off_c = 0, bytes = 0;
 };
-
-int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 RepackPlan plan_repack(const void* A, const void* B, const void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
                        int64_t ldb, int64_t ldc, int b_layout, int a_layout = B200_A_ROW_MAJOR) {

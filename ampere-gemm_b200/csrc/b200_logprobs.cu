@@ -1,0 +1,506 @@
+// Log probabilities of given tokens, the entropy of their distributions and
+// the top alternatives, with the gradient of the logits.
+//
+// For one row x of V logits with target t:
+//   m = max x, z = sum exp(x - m), lse = m + ln z
+//   logprob = x_t - lse
+//   entropy = -sum p ln p = ln z - sum exp(x - m) (x - m) / z,   p = exp(x - lse)
+//   d logprob / d x_j = [j == t] - p_j
+//   d entropy / d x_j = -p_j (x_j - lse + entropy)
+// Terms with p = 0 (a logit of -inf) are 0.  A row whose logits are all -inf
+// has logprob -inf, entropy 0 and gradient 0; a NaN or +inf in a row makes its
+// logprob, entropy and gradient NaN.  m and ln z are kept apart for the
+// backward pass: (x - m) - ln z does not round away what x - lse would.
+//
+// Bound by memory: the forward reads the logits once (running maximum and
+// sums), the backward reads them and writes their gradient once.  Sums are in
+// fp32 in a fixed order.
+#include <algorithm>
+#include <cstdint>
+
+#include "elem_types.cuh"
+#include "host_common.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = B200_LOGPROBS_MAX_TOP;
+// Logits of a group: the maximum of each group of the row is kept in shared
+// memory while the row streams by.  The top k elements of a row lie in its top
+// k groups (groups ordered by maximum, then lower index: an element outside
+// them has k elements before it, one in each), so the row is not read again.
+constexpr int kGroup = 8;
+// Longest slice of a row that one block takes when alternatives are wanted:
+// 4096 groups, 16 KB of maxima, 16 groups a thread.
+constexpr int kTopSlice = 32768;
+constexpr int kTopGroups = kTopSlice / kGroup;
+// Candidate groups after the threshold: those of the k threads whose best
+// group reaches it, kTopGroups / kThreads each at most.
+constexpr int kMaxCand = kMaxTop * (kTopGroups / kThreads);
+
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// max that yields NaN when an operand is NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Running maximum m, z = sum exp(x - m) and w = sum exp(x - m) (x - m).
+struct Sums {
+  float m, z, w;
+};
+
+// Moves sums to a maximum `m` >= s.m.  x - m = (x - s.m) + (s.m - m); a sum
+// over nothing (s.m = -inf, z = 0) stays empty.
+__device__ __forceinline__ void rebase(Sums& s, float m) {
+  if (s.m == m) return;
+  const float d = s.m - m;
+  const float f = exp2_approx(d * kLog2e);
+  s.w = s.z > 0.0f ? f * fmaf(s.z, d, s.w) : (s.z == 0.0f ? 0.0f : s.z);
+  s.z = s.z * f;
+  s.m = m;
+}
+
+__device__ __forceinline__ Sums merge(Sums a, Sums b) {
+  const float m = max_nan(a.m, b.m);
+  rebase(a, m);
+  rebase(b, m);
+  return Sums{m, a.z + b.z, a.w + b.w};
+}
+
+__device__ __forceinline__ Sums warp_merge(Sums s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums t;
+    t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    t.z = __shfl_xor_sync(0xffffffffu, s.z, o);
+    t.w = __shfl_xor_sync(0xffffffffu, s.w, o);
+    s = merge(s, t);
+  }
+  return s;
+}
+
+// Adds N logits (fp32) whose maximum is `mx`.
+template <int N>
+__device__ __forceinline__ void add_logits(Sums& s, const float (&v)[N], float mx) {
+  if (!(mx <= s.m)) rebase(s, max_nan(s.m, mx));
+  const float m = s.m == kNegInf ? 0.0f : s.m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float d = v[e] - m;
+    const float x = exp2_approx(d * kLog2e);
+    s.z += x;
+    // exp underflows to 0 long before -1e4: the clamp only keeps 0 * -inf out.
+    s.w = fmaf(x, fmaxf(d, -1.0e4f), s.w);
+  }
+}
+
+// Sorts after every key with a smaller value, or with the same value and a
+// higher index.  NaN is above +inf, and -0 equals +0.
+__device__ __forceinline__ unsigned long long make_key(float v, uint32_t index) {
+  uint32_t u = __float_as_uint(v + 0.0f);
+  u = v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_index(unsigned long long k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  if (u == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+// Calls one(index, value) or pack(first index, packs) over the logits
+// [lo, hi) of a row so that every 16-byte aligned pack is read whole: the
+// elements before the first aligned one and after the last go one by one.
+template <typename T>
+struct Span {
+  int64_t head_end, body_end;  // [lo, head_end) single, [head_end, body_end) packs, [body_end, hi) single
+  __device__ __forceinline__ Span(const T* row, int64_t lo, int64_t hi) {
+    constexpr int kV = kVec16<T>;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + lo) & 15u) / sizeof(T);
+    head_end = lo + (off ? kV - static_cast<int>(off) : 0);
+    if (head_end > hi) head_end = hi;
+    body_end = head_end + (hi - head_end) / kV * kV;
+  }
+};
+
+// Block-wide merge; every thread gets the result.
+__device__ __forceinline__ Sums block_merge(Sums s, Sums* buf) {
+  s = warp_merge(s);
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = s;
+  __syncthreads();
+  Sums r = buf[0];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) r = merge(r, buf[i]);
+  return r;
+}
+
+struct Outputs {
+  float* logprob;
+  float* entropy;
+  float2* stats;       // m, ln z
+  float* top_logprob;  // rows x top
+  int64_t* top_index;
+};
+
+template <typename T>
+__device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const T* x, int64_t vocab, int64_t target,
+                                          int64_t ignore, Sums s) {
+  const bool empty = s.m == kNegInf;
+  const float ln_z = logf(s.z);
+  out.stats[row] = make_float2(s.m, ln_z);
+  out.entropy[row] = empty ? 0.0f : ln_z - s.w / s.z;
+  float lp = 0.0f;
+  if (target != ignore) {
+    // A target outside the vocabulary has no probability to give.
+    if (target < 0 || target >= vocab) {
+      lp = __uint_as_float(0x7fffffffu);
+    } else {
+      lp = empty ? kNegInf : (to_f32(x[target]) - s.m) - ln_z;
+    }
+  }
+  out.logprob[row] = lp;
+}
+
+// One slice (blockIdx.x) of one row (blockIdx.y + i * gridDim.y).  With one
+// slice a row, the row's outputs are written here; otherwise the slice's sums
+// and its top keys go to `part_sums` / `part_keys` and logprobs_join_kernel
+// finishes the row.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kThreads)
+    logprobs_fwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows, int64_t vocab,
+                        int64_t ld, int64_t slice, int top, int64_t ignore, Outputs out, Sums* __restrict__ part_sums,
+                        unsigned long long* __restrict__ part_keys) {
+  constexpr int kV = kVec16<T>;
+  __shared__ Sums warp_sums[kWarps];
+  // Group maxima while streaming; then the candidates of the selection.
+  __shared__ float group_max[kTop ? kTopGroups : 1];
+  __shared__ unsigned long long best[kTop ? kThreads : 1];
+  __shared__ unsigned long long cand[kTop ? kMaxCand : 1];
+  __shared__ unsigned long long elems[kTop ? kMaxTop * kGroup : 1];
+  __shared__ unsigned long long threshold;
+  __shared__ int count;
+  pdl_wait();
+  const int slices = gridDim.x;
+  const int64_t lo = blockIdx.x * slice;
+  const int64_t hi = min(lo + slice, vocab);
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const T* x = logits + row * ld;
+    Sums s{kNegInf, 0.0f, 0.0f};
+    const Span<T> span(x, lo, hi);
+    // Group g of the slice is [lo + 8 g, lo + 8 g + 8) counted from the first
+    // aligned element less one group: group 0 is the head (fewer than kV
+    // elements), the last group the tail.
+    constexpr int kPacks = kGroup / kV;  // packs of a group
+    const int64_t body_groups = (span.body_end - span.head_end) / kGroup;
+    if (span.head_end > lo && tid < span.head_end - lo) {
+      const float v[1] = {to_f32(x[lo + tid])};
+      add_logits(s, v, v[0]);
+    }
+    for (int64_t g = tid; g < body_groups; g += kThreads) {
+      float v[kGroup];
+#pragma unroll
+      for (int p = 0; p < kPacks; ++p) {
+        const Pack<T, kV> q = load_pack<T, kV>(x + span.head_end + g * kGroup + p * kV);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) v[p * kV + e] = to_f32(q.v[e]);
+      }
+      float mx = v[0];
+#pragma unroll
+      for (int e = 1; e < kGroup; ++e) mx = max_nan(mx, v[e]);
+      if (kTop) group_max[g] = mx;
+      add_logits(s, v, mx);
+    }
+    const int64_t tail = span.head_end + body_groups * kGroup;  // up to kGroup + kV - 1 elements are left
+    if (tail + tid < hi) {
+      const float v[1] = {to_f32(x[tail + tid])};
+      add_logits(s, v, v[0]);
+    }
+    s = block_merge(s, warp_sums);
+    if constexpr (kTop) {
+      // Threshold: the top-th largest of the threads' best groups.  Keys are
+      // unique, so exactly `top` threads reach it (or all groups qualify).
+      unsigned long long mine = 0;
+      for (int g = tid; g < body_groups; g += kThreads) {
+        const unsigned long long k = make_key(group_max[g], g);
+        mine = k > mine ? k : mine;
+      }
+      best[tid] = mine;
+      if (tid == 0) {
+        threshold = 0;
+        count = 0;
+      }
+      __syncthreads();
+      int rank = 0;
+      for (int i = 0; i < kThreads; ++i) rank += best[i] > mine;
+      if (mine != 0 && rank == top - 1) threshold = mine;
+      __syncthreads();
+      const unsigned long long thr = threshold;
+      for (int g = tid; g < body_groups; g += kThreads) {
+        const unsigned long long k = make_key(group_max[g], g);
+        if (k >= thr) {
+          const int i = atomicAdd(&count, 1);
+          if (i < kMaxCand) cand[i] = k;
+        }
+      }
+      __syncthreads();
+      // With fewer than `top` threads holding a group, every group qualifies:
+      // those are fewer than kThreads <= kMaxCand.
+      const int n_cand = min(count, kMaxCand);
+      __syncthreads();
+      if (tid == 0) count = 0;
+      __syncthreads();
+      // The best `top` groups' elements, and the head's and tail's.
+      for (int i = tid; i < n_cand; i += kThreads) {
+        const unsigned long long k = cand[i];
+        int r = 0;
+        for (int j = 0; j < n_cand; ++j) r += cand[j] > k;
+        if (r < top) {
+          const int64_t first = span.head_end + static_cast<int64_t>(key_index(k)) * kGroup;
+          for (int e = 0; e < kGroup; ++e)
+            elems[r * kGroup + e] = make_key(to_f32(x[first + e]), static_cast<uint32_t>(first + e));
+        }
+      }
+      const int n_body = min(n_cand, top) * kGroup;
+      __syncthreads();
+      // `cand` now takes head and tail (fewer than 4 groups).
+      const int n_head = static_cast<int>(span.head_end - lo), n_tail = static_cast<int>(hi - tail);
+      if (tid < n_head) cand[tid] = make_key(to_f32(x[lo + tid]), static_cast<uint32_t>(lo + tid));
+      if (tid < n_tail) cand[n_head + tid] = make_key(to_f32(x[tail + tid]), static_cast<uint32_t>(tail + tid));
+      __syncthreads();
+      const int n_edge = n_head + n_tail, n_all = n_body + n_edge;
+      const float ln_z = logf(s.z);
+      for (int i = tid; i < n_all; i += kThreads) {
+        const unsigned long long k = i < n_body ? elems[i] : cand[i - n_body];
+        int r = 0;
+        for (int j = 0; j < n_body; ++j) r += elems[j] > k;
+        for (int j = 0; j < n_edge; ++j) r += cand[j] > k;
+        if (r < top) {
+          if (slices == 1) {
+            out.top_index[row * top + r] = key_index(k);
+            out.top_logprob[row * top + r] = s.m == kNegInf ? kNegInf : (key_value(k) - s.m) - ln_z;
+          } else {
+            part_keys[(row * slices + blockIdx.x) * top + r] = k;
+          }
+        }
+      }
+      // A slice shorter than `top` leaves keys over: 0 sorts after every logit.
+      if (slices > 1 && tid >= n_all && tid < top) part_keys[(row * slices + blockIdx.x) * top + tid] = 0;
+    }
+    if (tid == 0) {
+      if (slices == 1)
+        write_row<T>(out, row, x, vocab, targets[row], ignore, s);
+      else
+        part_sums[row * slices + blockIdx.x] = s;
+    }
+    __syncthreads();  // the next row reuses the shared arrays
+  }
+}
+
+// Joins the slices of a row; one block a row.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kThreads)
+    logprobs_join_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows,
+                         int64_t vocab, int64_t ld, int slices, int top, int64_t ignore, Outputs out,
+                         const Sums* __restrict__ part_sums, const unsigned long long* __restrict__ part_keys) {
+  __shared__ Sums warp_sums[kWarps];
+  pdl_wait();
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    Sums s{kNegInf, 0.0f, 0.0f};
+    for (int i = tid; i < slices; i += kThreads) s = merge(s, part_sums[row * slices + i]);
+    s = block_merge(s, warp_sums);
+    if constexpr (kTop) {
+      const unsigned long long* keys = part_keys + row * slices * top;
+      const float ln_z = logf(s.z);
+      for (int i = tid; i < slices * top; i += kThreads) {
+        const unsigned long long k = keys[i];
+        if (k == 0) continue;
+        int r = 0;
+        for (int j = 0; j < slices * top && r < top; ++j) r += keys[j] > k;
+        if (r < top) {
+          out.top_index[row * top + r] = key_index(k);
+          out.top_logprob[row * top + r] = s.m == kNegInf ? kNegInf : (key_value(k) - s.m) - ln_z;
+        }
+      }
+    }
+    if (tid == 0) write_row<T>(out, row, logits + row * ld, vocab, targets[row], ignore, s);
+    __syncthreads();
+  }
+}
+
+// gl ([j == t] - p) - gh p (ln p + entropy)
+template <typename T>
+__device__ __forceinline__ T grad_of(float x, float2 st, float ent, float gl, float gh, bool is_target) {
+  const float d = (x - st.x) - st.y;
+  const float p = exp2_approx(d * kLog2e);
+  const float g = -p * fmaf(gh, fmaxf(d, -1.0e4f) + ent, gl);
+  return from_f32<T>(is_target ? g + gl : g);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    logprobs_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
+                        const float2* __restrict__ stats, const float* __restrict__ entropy,
+                        const float* __restrict__ g_logprob, const float* __restrict__ g_entropy,
+                        T* __restrict__ dlogits, int64_t rows, int64_t vocab, int64_t ld, int64_t ldd, int64_t slice,
+                        int64_t ignore) {
+  constexpr int kV = kVec16<T>;
+  pdl_wait();
+  const int64_t lo = blockIdx.x * slice;
+  const int64_t hi = min(lo + slice, vocab);
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const T* x = logits + row * ld;
+    T* d = dlogits + row * ldd;
+    const int64_t target = targets[row];
+    const float2 lse = stats[row];
+    const float ent = entropy[row];
+    const float gl = g_logprob && target != ignore ? g_logprob[row] : 0.0f;
+    const float gh = g_entropy ? g_entropy[row] : 0.0f;
+    if (lse.x == kNegInf) {
+      // No probability anywhere: nothing depends on the logits.
+      for (int64_t j = lo + tid; j < hi; j += kThreads) d[j] = from_f32<T>(0.0f);
+      continue;
+    }
+    const Span<T> span(x, lo, hi);
+    const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
+    if (!same) {
+      for (int64_t j = lo + tid; j < hi; j += kThreads)
+        d[j] = grad_of<T>(to_f32(x[j]), lse, ent, gl, gh, j == target);
+      continue;
+    }
+    if (lo + tid < span.head_end)
+      d[lo + tid] = grad_of<T>(to_f32(x[lo + tid]), lse, ent, gl, gh, lo + tid == target);
+    for (int64_t j = span.head_end + tid * kV; j < span.body_end; j += kThreads * kV) {
+      const Pack<T, kV> q = load_pack<T, kV>(x + j);
+      Pack<T, kV> o;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) o.v[e] = grad_of<T>(to_f32(q.v[e]), lse, ent, gl, gh, j + e == target);
+      store_pack<T, kV>(d + j, o);
+    }
+    if (span.body_end + tid < hi)
+      d[span.body_end + tid] =
+          grad_of<T>(to_f32(x[span.body_end + tid]), lse, ent, gl, gh, span.body_end + tid == target);
+  }
+}
+
+int cuda_code(cudaError_t e) { return e == cudaSuccess ? B200_OK : B200_ERR_CUDA; }
+
+bool dtype_ok(int d) { return d == B200_DTYPE_F16 || d == B200_DTYPE_BF16 || d == B200_DTYPE_F32; }
+
+template <typename Fn>
+int with_dtype(int dtype, Fn&& fn) {
+  if (dtype == B200_DTYPE_F16) return fn(__half{});
+  if (dtype == B200_DTYPE_BF16) return fn(__nv_bfloat16{});
+  return fn(float{});
+}
+
+// Slices a row is cut into: enough blocks for the device when rows are few
+// (4096 logits each at least), and none longer than the selection can hold.
+int64_t row_slices(int64_t rows, int64_t vocab, int top) {
+  constexpr int64_t kBlocks = 4 * 148, kLeast = 4096;
+  int64_t s = std::max<int64_t>(1, std::min(kBlocks / std::max<int64_t>(rows, 1), vocab / kLeast));
+  if (top > 0) s = std::max(s, (vocab + kTopSlice - 1) / kTopSlice);
+  return s;
+}
+
+// Slice length (a multiple of kGroup) for about `slices` slices, none empty.
+int64_t slice_length(int64_t vocab, int64_t slices) { return round_up((vocab + slices - 1) / slices, kGroup); }
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int64_t b200_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top) {
+  using namespace b200;
+  if (rows < 0 || vocab < 0 || top < 0 || top > kMaxTop) return -B200_ERR_INVALID_ARGUMENT;
+  if (vocab > 0x7fffffff) return -B200_ERR_TOO_LARGE;
+  const int64_t s = row_slices(rows, vocab, top);
+  if (s <= 1) return 0;
+  return round_up(rows * s * (int64_t)sizeof(Sums), 256) + rows * s * top * 8;
+}
+
+extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* targets, float* logprob, float* entropy,
+                                       float* stats, float* top_logprob, int64_t* top_index, int64_t rows, int64_t vocab,
+                                       int64_t ld, int top, int64_t ignore_index, int dtype, void* workspace,
+                                       int64_t workspace_bytes, void* stream_ptr) {
+  using namespace b200;
+  if (rows < 0 || vocab < 0 || top < 0 || top > kMaxTop || top > vocab || !dtype_ok(dtype))
+    return B200_ERR_INVALID_ARGUMENT;
+  if (vocab > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (rows == 0) return B200_OK;
+  if (vocab == 0 || !logits || !targets || !logprob || !entropy || !stats || ld < vocab ||
+      (top > 0 && (!top_logprob || !top_index)))
+    return B200_ERR_INVALID_ARGUMENT;
+  const int64_t need = b200_token_logprobs_workspace_size(rows, vocab, top);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return B200_ERR_WORKSPACE;
+  DeviceInfo dev;
+  if (int rc = current_device_info(dev)) return rc;
+  if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const int64_t slice = slice_length(vocab, row_slices(rows, vocab, top));
+  const int64_t slices = (vocab + slice - 1) / slice;
+  const Outputs out{logprob, entropy, reinterpret_cast<float2*>(stats), top_logprob, top_index};
+  Sums* sums = static_cast<Sums*>(workspace);
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(
+      static_cast<uint8_t*>(workspace) + round_up(rows * slices * (int64_t)sizeof(Sums), 256));
+  const dim3 grid((unsigned)slices, (unsigned)std::min<int64_t>(rows, 65535));
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const T* x = static_cast<const T*>(logits);
+    int rc = cuda_code(top > 0 ? launch_gemm(logprobs_fwd_kernel<T, true>, grid, dim3(kThreads), 0, stream, x, targets,
+                                             rows, vocab, ld, slice, top, ignore_index, out, sums, keys)
+                               : launch_gemm(logprobs_fwd_kernel<T, false>, grid, dim3(kThreads), 0, stream, x,
+                                             targets, rows, vocab, ld, slice, top, ignore_index, out, sums, keys));
+    if (rc || slices == 1) return rc;
+    const dim3 jgrid((unsigned)std::min<int64_t>(rows, 0x7fffffff));
+    return cuda_code(top > 0 ? launch_gemm(logprobs_join_kernel<T, true>, jgrid, dim3(kThreads), 0, stream, x, targets,
+                                           rows, vocab, ld, (int)slices, top, ignore_index, out, sums, keys)
+                             : launch_gemm(logprobs_join_kernel<T, false>, jgrid, dim3(kThreads), 0, stream, x,
+                                           targets, rows, vocab, ld, (int)slices, top, ignore_index, out, sums, keys));
+  });
+}
+
+extern "C" int b200_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
+                                       const float* entropy, const float* g_logprob, const float* g_entropy,
+                                       void* dlogits, int64_t rows, int64_t vocab, int64_t ld, int64_t ldd,
+                                       int64_t ignore_index, int dtype, void* stream_ptr) {
+  using namespace b200;
+  if (rows < 0 || vocab < 0 || !dtype_ok(dtype)) return B200_ERR_INVALID_ARGUMENT;
+  if (vocab > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (rows == 0 || vocab == 0) return B200_OK;
+  if (!logits || !targets || !stats || !entropy || !dlogits || ld < vocab || ldd < vocab)
+    return B200_ERR_INVALID_ARGUMENT;
+  DeviceInfo dev;
+  if (int rc = current_device_info(dev)) return rc;
+  if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  constexpr int64_t kSlice = 16384;
+  const int64_t slice = std::min(kSlice, round_up(vocab, kGroup));
+  const int64_t slices = (vocab + slice - 1) / slice;
+  const dim3 grid((unsigned)slices, (unsigned)std::min<int64_t>(rows, 65535));
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return cuda_code(launch_gemm(logprobs_bwd_kernel<T>, grid, dim3(kThreads), 0, stream,
+                                 static_cast<const T*>(logits), targets, reinterpret_cast<const float2*>(stats), entropy, g_logprob, g_entropy,
+                                 static_cast<T*>(dlogits), rows, vocab, ld, ldd, slice, ignore_index));
+  });
+}

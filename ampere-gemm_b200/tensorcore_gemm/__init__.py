@@ -2,8 +2,12 @@
 
 Public surface identical to the reference (tensorcore_gemm/__init__.py:1-3).
 Importing the package also registers ``torch.ops.tensorcore_gemm.mm`` (the
-same GEMM as a dispatcher operator with autograd, see ``ops``).
+same GEMM as a dispatcher operator with autograd, see ``ops``) and the
+operators of the modules ``norm`` (layer norm) and ``logprobs`` (token log
+probabilities).
 """
+from . import logprobs as _logprobs  # noqa: F401  (registers torch.ops.tensorcore_gemm.token_logprobs)
+from . import norm as _norm  # noqa: F401  (registers torch.ops.tensorcore_gemm.layer_norm)
 from . import ops as _ops  # noqa: F401  (registers torch.ops.tensorcore_gemm.mm)
 from .gemm import KERNEL_MODES, gemm, gemm_pretransposed, is_supported
 

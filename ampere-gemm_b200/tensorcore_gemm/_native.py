@@ -42,6 +42,11 @@ B200_B_COL_MAJOR = 1
 B200_A_ROW_MAJOR = 0
 B200_A_COL_MAJOR = 1
 
+B200_DTYPE_F16 = 0
+B200_DTYPE_BF16 = 1
+B200_DTYPE_F32 = 2
+B200_LOGPROBS_MAX_TOP = 64
+
 # Every symbol the header declares, with its ctypes signature.
 _SIGNATURES = {
     "b200_gemm_f16": (
@@ -91,6 +96,26 @@ _SIGNATURES = {
          ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
          ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
          ctypes.c_int, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_void_p],
+    ),
+    "b200_layer_norm_fwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 6 + [ctypes.c_int64] * 4 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_void_p],
+    ),
+    "b200_layer_norm_bwd_workspace_size": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
+    "b200_layer_norm_bwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 8 + [ctypes.c_int64] * 5 +
+        [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "b200_token_logprobs_workspace_size": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "b200_token_logprobs_fwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 7 + [ctypes.c_int64] * 3 +
+        [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "b200_token_logprobs_bwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 7 + [ctypes.c_int64] * 5 + [ctypes.c_int, ctypes.c_void_p],
     ),
     "b200_ipc_handle_size": (ctypes.c_int, []),
     "b200_ipc_alloc": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p]),

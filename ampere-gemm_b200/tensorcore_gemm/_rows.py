@@ -1,0 +1,76 @@
+"""Helpers of the operators that work on the rows of a tensor (norm, ffn,
+logprobs): argument checks, the 2-D view the C ABI takes, workspaces and the
+launch on torch's current stream."""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from .gemm import _GET_DEVICE, _current_stream
+
+DTYPE_CODES = {
+    torch.float16: _native.B200_DTYPE_F16,
+    torch.bfloat16: _native.B200_DTYPE_BF16,
+    torch.float32: _native.B200_DTYPE_F32,
+}
+
+
+def check_cuda(name: str, t, dtypes=tuple(DTYPE_CODES)) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
+
+
+def as_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`t` as a matrix of its last dimension's rows, and its row pitch.
+
+    A row-strided view (a column slice) is used in place; anything else, an
+    expanded tensor among them, is made contiguous."""
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(0, 0)
+    if t.stride(1) == 1 or cols <= 1:
+        if t.shape[0] <= 1:
+            return t, max(1, cols)
+        if t.stride(0) >= max(1, cols):
+            return t, t.stride(0)
+    return t.contiguous(), max(1, cols)
+
+
+def workspace(nbytes: int, device: torch.device, what: str) -> torch.Tensor | None:
+    """Device memory for a call (None when it needs none); freed to torch's
+    allocator, which reuses it in stream order."""
+    if nbytes < 0:
+        _native.check(-nbytes, what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def launch(name: str, dev: int, *args) -> None:
+    """Calls C entry point `name` with `args` and the current stream of device `dev`; raises on an error code."""
+    fn = getattr(_native.load(), name)
+    if dev != _GET_DEVICE():
+        with torch.cuda.device(dev):
+            code = fn(*args, _current_stream(dev))
+    else:
+        code = fn(*args, _current_stream(dev))
+    if code != _native.B200_OK:
+        _native.check(code, name)
+
+
+def plain_eager(*tensors) -> bool:
+    """True when the call can go straight to the kernels: real tensors, not being traced."""
+    if torch.compiler.is_compiling():
+        return False
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and type(t) not in (torch.Tensor, torch.nn.Parameter):
+            return False
+    return True
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

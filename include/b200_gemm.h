@@ -182,6 +182,67 @@ B200_API int b200_ipc_free(void* ptr);
 B200_API int b200_ipc_open(const void* handle, void** ptr);
 B200_API int b200_ipc_close(void* ptr);
 
+/* Element types of the operators below. */
+#define B200_DTYPE_F16 0
+#define B200_DTYPE_BF16 1
+#define B200_DTYPE_F32 2
+
+/*
+ * Layer norm over the last dimension: y = (x - mean) * rstd * w + b with
+ * rstd = 1 / sqrt(variance + eps), x and y rows x cols with row pitches in
+ * elements.  x and y are of `dtype`; w and b (cols each, either may be NULL)
+ * of `wdtype`: the same type, or B200_DTYPE_F32.  mean and rstd (rows floats
+ * each, either may be NULL) receive the statistics the backward call reads.
+ * Any alignment and pitch is taken; rows that start on 16 bytes run fastest.
+ * No counterpart in the reference.
+ */
+B200_API int b200_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
+                                 int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, int dtype, int wdtype,
+                                 float eps, void* stream);
+
+/*
+ * Its gradients: dx (of `dtype`), and dw and db (of `wdtype`, cols each;
+ * either may be NULL), summed over the rows in fp32 in a fixed order.  With dw
+ * or db, the workspace (b200_layer_norm_bwd_workspace_size bytes, 256-byte
+ * aligned) holds the partial sums; it must not be reused until the call's
+ * work on `stream` has finished.
+ */
+B200_API int64_t b200_layer_norm_bwd_workspace_size(int64_t rows, int64_t cols);
+B200_API int b200_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
+                                 void* dx, void* dw, void* db, int64_t rows, int64_t cols, int64_t lddy, int64_t ldx,
+                                 int64_t lddx, int dtype, int wdtype, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
+/*
+ * Log probabilities of given tokens: for each row of logits (rows x vocab, row
+ * pitch ld, of `dtype`) the log softmax at targets[row], the entropy of the
+ * softmax, and the `top` (<= B200_LOGPROBS_MAX_TOP) largest log probabilities
+ * with their indices, largest first, equal logits by lower index (NaN first of
+ * all).  A target equal to ignore_index gives logprob 0; any other target
+ * outside [0, vocab) gives NaN.  A row of -inf throughout gives logprob -inf
+ * and entropy 0.  stats (rows x 2 floats) receives the row's maximum and
+ * ln(sum exp(x - max)), which the backward call reads.  The workspace
+ * (b200_token_logprobs_workspace_size bytes, may be 0; 256-byte aligned)
+ * holds the parts of rows that several blocks share.  No counterpart in the
+ * reference.
+ */
+#define B200_LOGPROBS_MAX_TOP 64
+B200_API int64_t b200_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
+B200_API int b200_token_logprobs_fwd(const void* logits, const int64_t* targets, float* logprob, float* entropy,
+                                     float* stats, float* top_logprob, int64_t* top_index, int64_t rows, int64_t vocab,
+                                     int64_t ld, int top, int64_t ignore_index, int dtype, void* workspace,
+                                     int64_t workspace_bytes, void* stream);
+
+/*
+ * The gradient of the logits (pitch ldd, of `dtype`) from those of the log
+ * probabilities and of the entropies (rows floats each, either may be NULL).
+ * Rows whose target is ignore_index get the entropy's part only.
+ */
+B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
+                                     const float* entropy, const float* g_logprob, const float* g_entropy,
+                                     void* dlogits, int64_t rows, int64_t vocab, int64_t ld, int64_t ldd,
+                                     int64_t ignore_index, int dtype, void* stream);
+
 /* Human-readable text of a return code (static storage). Counterpart of the
  * TORCH_CHECK messages of the reference launcher (gemm.py:33-47, 150-152). */
 B200_API const char* b200_gemm_strerror(int code);
