@@ -18,6 +18,9 @@
 namespace b200 {
 namespace {
 
+constexpr int kMaxRowThreads = 512;  // threads of a row that stays in registers: 128 registers each
+constexpr int kLongThreads = 1024;   // threads of a longer row
+
 __device__ __forceinline__ void pdl_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -44,7 +47,8 @@ __device__ __forceinline__ float row_sum(float v, bool one_warp, float* red) {
 // Forward.  blockDim = (threads of a row, rows of a block); a thread holds NV
 // packs of VEC elements, pack j at (j * blockDim.x + threadIdx.x) * VEC.
 template <typename T, typename W, int VEC, int NV>
-__global__ void layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
+__global__ void __launch_bounds__(kMaxRowThreads)
+    layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
                                       T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                       int64_t rows, int cols, int64_t ldx, int64_t ldy, float eps) {
   __shared__ float red[2][32];
@@ -112,7 +116,7 @@ __global__ void layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restri
 // Forward for rows longer than the registers of a block hold: one block a
 // row, which is read three times (the second and third from L2).
 template <typename T, typename W>
-__global__ void layer_norm_fwd_long_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
+__global__ void __launch_bounds__(kLongThreads) layer_norm_fwd_long_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
                                            T* __restrict__ y, float* __restrict__ mean_out,
                                            float* __restrict__ rstd_out, int64_t rows, int cols, int64_t ldx,
                                            int64_t ldy, float eps) {
@@ -145,7 +149,8 @@ __global__ void layer_norm_fwd_long_kernel(const T* __restrict__ x, const W* __r
 // writes its sums once, as row blockIdx.x of `part` (gridDim.x x 2 x cols:
 // dw, then db), and layer_norm_bwd_reduce_kernel adds those rows up.
 template <typename T, typename W, int VEC, int NV>
-__global__ void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
+__global__ void __launch_bounds__(kMaxRowThreads)
+    layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
                                       const float* __restrict__ mean, const float* __restrict__ rstd_in,
                                       T* __restrict__ dx, float* __restrict__ part, int64_t rows, int cols,
                                       int64_t lddy, int64_t ldx, int64_t lddx) {
@@ -265,7 +270,7 @@ __global__ void layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restr
 
 // dx for rows longer than a block's registers hold: one block a row.
 template <typename T, typename W>
-__global__ void layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
+__global__ void __launch_bounds__(kLongThreads) layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
                                            const float* __restrict__ mean, const float* __restrict__ rstd_in,
                                            T* __restrict__ dx, int64_t rows, int cols, int64_t lddy, int64_t ldx,
                                            int64_t lddx) {
@@ -347,13 +352,16 @@ int round32(int v) { return (v + 31) / 32 * 32; }
 RowPlan plan_rows(int packs, int max_nv, int threads_wanted) {
   for (int nv = 1; nv <= max_nv; nv *= 2) {
     const int t = round32((packs + nv - 1) / nv);
-    if (t <= threads_wanted || (nv == max_nv && t <= 1024)) return RowPlan{nv, t, t == 32 ? 4 : 1};
+    if (t <= threads_wanted || (nv == max_nv && t <= kMaxRowThreads)) return RowPlan{nv, t, t == 32 ? 4 : 1};
   }
   return RowPlan{0, 0, 1};
 }
 
 constexpr int kFwdMaxNv = 8;
-constexpr int kBwdMaxElems = 16;  // columns a thread sums dw and db of: 32 registers
+// Columns a thread sums dw and db of, in packs: two registers each, beside the
+// packs of x, dy and w.
+template <int VEC>
+constexpr int kBwdMaxNv = VEC == 1 ? 16 : 4;
 
 template <int V>
 using IntC = std::integral_constant<int, V>;
@@ -436,7 +444,7 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
   return with_types(dtype, wdtype, [&](auto t, auto wt) {
     using T = decltype(t);
     using W = decltype(wt);
-    const RowPlan p = plan_rows(vec ? n / vec16 : n, kFwdMaxNv, rows >= 4 * dev.sm_count ? 128 : 1024);
+    const RowPlan p = plan_rows(vec ? n / vec16 : n, kFwdMaxNv, rows >= 4 * dev.sm_count ? 128 : kMaxRowThreads);
     auto go = [&](auto vc, auto nvc) {
       auto kern = layer_norm_fwd_kernel<T, W, decltype(vc)::value, decltype(nvc)::value>;
       const int64_t blocks = (rows + p.rows - 1) / p.rows;
@@ -447,7 +455,7 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
     };
     if (p.nv == 0) {
       const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
-      return cuda_code(launch_gemm(layer_norm_fwd_long_kernel<T, W>, dim3(grid), dim3(1024), 0, stream,
+      return cuda_code(launch_gemm(layer_norm_fwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream,
                                    static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b),
                                    static_cast<T*>(y), mean, rstd, rows, n, ldx, ldy, eps));
     }
@@ -502,10 +510,11 @@ extern "C" int b200_layer_norm_bwd(const void* dy, const void* x, const void* w,
     T* dxp = static_cast<T*>(dx);
     int parts = 0;
     int rc;
-    const RowPlan p = vec ? plan_rows(n / vec16, kBwdMaxElems / vec16, 512) : plan_rows(n, kBwdMaxElems, 512);
+    const RowPlan p = vec ? plan_rows(n / vec16, kBwdMaxNv<kVec16<T>>, kMaxRowThreads)
+                          : plan_rows(n, kBwdMaxNv<1>, kMaxRowThreads);
     if (p.nv == 0) {
       const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
-      rc = cuda_code(launch_gemm(layer_norm_bwd_long_kernel<T, W>, dim3(grid), dim3(1024), 0, stream, dyp, xp, wp,
+      rc = cuda_code(launch_gemm(layer_norm_bwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream, dyp, xp, wp,
                                  mean, rstd, dxp, rows, n, lddy, ldx, lddx));
       if (rc || !sums) return rc;
       parts = (int)std::min<int64_t>(rows, 32);
@@ -524,7 +533,7 @@ extern "C" int b200_layer_norm_bwd(const void* dy, const void* x, const void* w,
       rc = with_nv(p.nv, [&](auto nvc) {
         constexpr int kNv = decltype(nvc)::value;
         if (vec) {
-          if constexpr (kNv * kVec16<T> <= kBwdMaxElems) return go(IntC<kVec16<T>>{}, nvc);
+          if constexpr (kNv <= kBwdMaxNv<kVec16<T>>) return go(IntC<kVec16<T>>{}, nvc);
           return (int)B200_ERR_INVALID_ARGUMENT;
         }
         return go(IntC<1>{}, nvc);
