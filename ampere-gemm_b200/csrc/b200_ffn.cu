@@ -1,0 +1,223 @@
+// Gated feed-forward block, forward and backward:
+//
+//   g = x Wg^T, u = x Wu^T, a = act(g) u, y = a Wo^T          (w_in = [Wg; Wu])
+//   da = dy Wo, dg = da u act'(g), du = da act(g)
+//   dWo = dy^T a, dx = [dg du] w_in, dw_in = [dg du]^T x
+//
+// Both input projections, the activation and the product are one GEMM launch
+// whose epilogue sees g and u of the same elements (kernel_cta2.cuh,
+// epilogue_gate.cuh); da is never written either: its epilogue turns it into
+// dg, du and a.  The other products are plain GEMMs on the library's kernels.
+// g, u, a, dg and du are kept in the operands' 16-bit type between launches:
+// the tensor cores take 16-bit operands, and each such rounding adds about as
+// much error as the one rounding of the result.
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "gemm_internal.h"
+#include "kernel_cta2.cuh"
+#include "tensor_map.cuh"
+
+namespace b200 {
+namespace {
+
+struct GateShape {
+  int rows, hidden, depth;  // of the fused GEMM: M, N (columns of a), K
+};
+
+// Launches the pair kernel with a fused epilogue: 256 x 256 accumulator tiles,
+// one cluster per tile, tiles taken dynamically.  A is rows x depth (K-major);
+// B is 2 hidden x depth (gate and up) or depth x hidden row-major (backward).
+template <bool kBf16, int kEpi>
+int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, const GateShape& s,
+                const FusedArgs<kEpi>& fx, cudaStream_t stream) {
+  constexpr bool kUp = kEpi == kEpiGateUp;
+  constexpr int kOutN = kUp ? 128 : 256;
+  using Cfg = PairConfig<3, 2, 1>;
+  CUtensorMap ta, tb, tc;
+  int rc = make_tmap_2d(&ta, A, s.rows, s.depth, lda, kBK, kBM, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (rc) return rc;
+  rc = kUp ? make_tmap_2d(&tb, B, 2 * (uint64_t)s.hidden, s.depth, ldb, kBK, Cfg::kHalfN,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B)
+           : make_tmap_2d(&tb, B, s.depth, s.hidden, ldb, 64, Cfg::kStageK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tc, C, s.rows, s.hidden, ldc, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+  if (rc) return rc;
+  auto kern = gemm_f16_tcgen05_pair_kernel<3, 2, 1, !kUp, false, 256, true, kBf16, kEpi>;
+  static std::atomic<uint8_t> attr_done[kMaxDevices];
+  if (int e = ensure_smem_attr(kern, Cfg::kSmemBytes, attr_done)) return e;
+  const long long tiles =
+      (long long)((s.rows + Cfg::kTileM - 1) / Cfg::kTileM) * ((s.hidden + kOutN - 1) / kOutN);
+  if (tiles > 0x3fffffffLL) return B200_ERR_TOO_LARGE;
+  EpiParams ep;
+  ep.m = s.rows;
+  ep.n = s.hidden;
+  ep.n_tma = s.hidden;
+  ep.ldc = ldc;
+  ep.c = static_cast<uint16_t*>(C);
+  const cudaError_t le = launch_gemm(kern, dim3(2 * (unsigned)tiles), dim3(kThreads), Cfg::kSmemBytes, stream, ta, tb,
+                                     tc, s.rows, s.hidden, s.depth, 8, ep, SplitTail{}, fx);
+  return le == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
+// Map of a rows x hidden output block that the epilogue warps store.
+int store_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+  return make_tmap_2d(map, base, rows, cols, ld, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+}
+
+template <bool kBf16>
+int gate_up(const void* x, int64_t ldx, const void* w_in, int64_t ldw, uint16_t* a, uint16_t* gate_up, int act,
+            const GateShape& s, cudaStream_t stream) {
+  FusedArgs<kEpiGateUp> fx;
+  fx.activation = act;
+  fx.save = gate_up != nullptr;
+  // Unused maps point at `a`, so that every launch has valid ones.
+  const int64_t ld = gate_up ? 2 * (int64_t)s.hidden : s.hidden;
+  if (int rc = store_map(&fx.tmap_g, gate_up ? gate_up : a, s.rows, s.hidden, ld)) return rc;
+  if (int rc = store_map(&fx.tmap_u, gate_up ? gate_up + s.hidden : a, s.rows, s.hidden, ld)) return rc;
+  return launch_gate<kBf16, kEpiGateUp>(x, ldx, w_in, ldw, a, s.hidden, s, fx, stream);
+}
+
+template <bool kBf16>
+int gate_bwd(const void* dy, int64_t lddy, const void* w_out, int64_t ldw, const uint16_t* gate_up, uint16_t* dgu,
+             uint16_t* a, int act, const GateShape& s, cudaStream_t stream) {
+  FusedArgs<kEpiGateBwd> fx;
+  fx.activation = act;
+  fx.g = gate_up;
+  fx.u = gate_up + s.hidden;
+  fx.ld = 2 * (int64_t)s.hidden;
+  if (int rc = store_map(&fx.tmap_dg, dgu, s.rows, s.hidden, fx.ld)) return rc;
+  if (int rc = store_map(&fx.tmap_du, dgu + s.hidden, s.rows, s.hidden, fx.ld)) return rc;
+  if (int rc = store_map(&fx.tmap_a, a, s.rows, s.hidden, s.hidden)) return rc;
+  return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s.hidden, s, fx, stream);
+}
+
+int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
+               int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* stream) {
+  return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, stream);
+}
+
+// Checks shared by the two directions; *empty: some dimension is 0.
+int check_ffn(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int activation, int dtype, bool* empty) {
+  if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return B200_ERR_INVALID_ARGUMENT;
+  if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) return B200_ERR_INVALID_ARGUMENT;
+  if (dtype != B200_DTYPE_F16 && dtype != B200_DTYPE_BF16) return B200_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7fffffff || dim > 0x7fffffff || hidden > 0x3fffffff || out_dim > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (hidden % 8 != 0) return B200_ERR_MISALIGNED;
+  *empty = rows == 0 || dim == 0 || hidden == 0 || out_dim == 0;
+  return B200_OK;
+}
+
+int zero_rows(void* p, int64_t ld, int64_t rows, int64_t cols, cudaStream_t stream) {
+  if (!p || rows == 0 || cols == 0) return B200_OK;
+  return cudaMemset2DAsync(p, ld * 2, 0, cols * 2, rows, stream) == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
+// Bytes of a rows x cols 16-bit matrix in a workspace.
+int64_t part_bytes(int64_t rows, int64_t cols) { return round_up(rows * cols * 2, 256); }
+
+bool workspace_ok(const void* ws, int64_t bytes, int64_t need) {
+  return need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255u) == 0);
+}
+
+}  // namespace
+
+int take_error_word_ffn() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int)) != cudaSuccess) return -1;
+  const int zero = 0;
+  if (v != 0 && cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+
+}  // namespace b200
+
+extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int backward) {
+  if (rows < 0 || hidden < 0) return -B200_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7fffffff || hidden > 0x3fffffff) return -B200_ERR_TOO_LARGE;
+  return b200::part_bytes(rows, hidden) + (backward ? b200::part_bytes(rows, 2 * hidden) : 0);
+}
+
+extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w_out, void* y, void* gate_up,
+                                  int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int64_t ldx,
+                                  int64_t ldw_in, int64_t ldw_out, int64_t ldy, int activation, int dtype,
+                                  void* workspace, int64_t workspace_bytes, void* stream_ptr) {
+  using namespace b200;
+  bool empty = false;
+  if (int rc = check_ffn(rows, dim, hidden, out_dim, activation, dtype, &empty)) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (empty) {
+    if (rows > 0 && out_dim > 0 && (!y || ldy < out_dim)) return B200_ERR_INVALID_ARGUMENT;
+    if (int rc = zero_rows(gate_up, 2 * hidden, rows, 2 * hidden, stream)) return rc;
+    return zero_rows(y, ldy, rows, out_dim, stream);
+  }
+  if (!x || !w_in || !w_out || !y || ldx < dim || ldw_in < dim || ldw_out < hidden || ldy < out_dim)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (!pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) || !pitch_ok(y, ldy) ||
+      (gate_up && !aligned16(gate_up)))
+    return B200_ERR_MISALIGNED;
+  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, hidden, 0)))
+    return B200_ERR_WORKSPACE;
+  DeviceInfo dev;
+  if (int rc = current_device_info(dev)) return rc;
+  if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
+  const bool bf16 = dtype == B200_DTYPE_BF16;
+  uint16_t* a = static_cast<uint16_t*>(workspace);
+  const GateShape s{(int)rows, (int)hidden, (int)dim};
+  const int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(x, ldx, w_in, ldw_in, a,
+                                                                     static_cast<uint16_t*>(gate_up), activation, s,
+                                                                     stream);
+  if (rc) return rc;
+  return plain_gemm(bf16, a, w_out, y, rows, out_dim, hidden, hidden, ldw_out, ldy, B200_A_ROW_MAJOR, B200_B_COL_MAJOR,
+                    stream_ptr);
+}
+
+extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_in, const void* w_out,
+                                  const void* gate_up, void* dx, void* dw_in, void* dw_out, int64_t rows, int64_t dim,
+                                  int64_t hidden, int64_t out_dim, int64_t lddy, int64_t ldx, int64_t ldw_in,
+                                  int64_t ldw_out, int64_t lddx, int64_t lddw_in, int64_t lddw_out, int activation,
+                                  int dtype, void* workspace, int64_t workspace_bytes, void* stream_ptr) {
+  using namespace b200;
+  bool empty = false;
+  if (int rc = check_ffn(rows, dim, hidden, out_dim, activation, dtype, &empty)) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if ((dx && lddx < dim) || (dw_in && lddw_in < dim) || (dw_out && lddw_out < hidden)) return B200_ERR_INVALID_ARGUMENT;
+  if (empty) {
+    if (int rc = zero_rows(dx, lddx, rows, dim, stream)) return rc;
+    if (int rc = zero_rows(dw_in, lddw_in, 2 * hidden, dim, stream)) return rc;
+    return zero_rows(dw_out, lddw_out, out_dim, hidden, stream);
+  }
+  if (!dy || !x || !w_in || !w_out || !gate_up || lddy < out_dim || ldx < dim || ldw_in < dim || ldw_out < hidden)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (!pitch_ok(dy, lddy) || !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) ||
+      !aligned16(gate_up) || (dx && !pitch_ok(dx, lddx)) || (dw_in && !pitch_ok(dw_in, lddw_in)) ||
+      (dw_out && !pitch_ok(dw_out, lddw_out)))
+    return B200_ERR_MISALIGNED;
+  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, hidden, 1)))
+    return B200_ERR_WORKSPACE;
+  DeviceInfo dev;
+  if (int rc = current_device_info(dev)) return rc;
+  if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
+  const bool bf16 = dtype == B200_DTYPE_BF16;
+  uint16_t* dgu = static_cast<uint16_t*>(workspace);
+  uint16_t* a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + part_bytes(rows, 2 * hidden));
+  const GateShape s{(int)rows, (int)hidden, (int)out_dim};
+  int rc = (bf16 ? gate_bwd<true> : gate_bwd<false>)(dy, lddy, w_out, ldw_out, static_cast<const uint16_t*>(gate_up),
+                                                     dgu, a, activation, s, stream);
+  if (rc) return rc;
+  if (dx) {
+    rc = plain_gemm(bf16, dgu, w_in, dx, rows, dim, 2 * hidden, 2 * hidden, ldw_in, lddx, B200_A_ROW_MAJOR,
+                    B200_B_ROW_MAJOR, stream_ptr);
+    if (rc) return rc;
+  }
+  if (dw_in) {
+    rc = plain_gemm(bf16, dgu, x, dw_in, 2 * hidden, dim, rows, 2 * hidden, ldx, lddw_in, B200_A_COL_MAJOR,
+                    B200_B_ROW_MAJOR, stream_ptr);
+    if (rc) return rc;
+  }
+  if (dw_out)
+    rc = plain_gemm(bf16, dy, a, dw_out, out_dim, hidden, rows, lddy, hidden, lddw_out, B200_A_COL_MAJOR,
+                    B200_B_ROW_MAJOR, stream_ptr);
+  return rc;
+}

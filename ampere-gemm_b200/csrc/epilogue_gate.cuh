@@ -1,0 +1,227 @@
+// Epilogues of the gated feed-forward block for the 2-CTA GEMM kernel:
+//
+//   gate and up   g = x Wg^T, u = x Wu^T in one tile;  a = act(g) u
+//   backward      da = dy Wo in the accumulator;       a, dg = da u act'(g), du = da act(g)
+//
+// Activations are computed in fp32 from the fp32 accumulators (forward) or
+// from the saved 16-bit g and u (backward).
+#pragma once
+
+#include "gemm_common.cuh"
+
+namespace b200 {
+
+// Epilogues of the pair kernel.
+constexpr int kEpiPlain = 0;    // C = alpha * acc + beta * C
+constexpr int kEpiGateUp = 1;   // C = act(g) u, optionally g and u too
+constexpr int kEpiGateBwd = 2;  // dg, du and a from da and the saved g, u
+
+template <int kEpi>
+struct FusedArgs {};
+
+template <>
+struct FusedArgs<kEpiGateUp> {
+  CUtensorMap tmap_g, tmap_u;  // where g and u are kept for the backward pass
+  int activation = 0;          // B200_ACT_*
+  int save = 0;                // 0: g and u are not stored
+};
+
+template <>
+struct FusedArgs<kEpiGateBwd> {
+  CUtensorMap tmap_dg, tmap_du, tmap_a;
+  const uint16_t* g = nullptr;  // the saved g and u, row pitch ld (elements)
+  const uint16_t* u = nullptr;
+  int64_t ld = 0;
+  int activation = 0;
+};
+
+// act(g) and act'(g).  The exponentials and quotients are the approximate
+// ones: their relative error, a few 2^-22, is far below the 16-bit rounding of
+// what they end up in.
+struct ActValue {
+  float f, slope;
+};
+
+__device__ __forceinline__ float sigmoid_approx(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+template <int kAct, bool kSlope>
+__device__ __forceinline__ ActValue activate(float g) {
+  ActValue r;
+  r.slope = 0.0f;
+  if constexpr (kAct == 0) {  // silu: g s(g)
+    const float s = sigmoid_approx(g);
+    r.f = g * s;
+    if (kSlope) r.slope = s * (1.0f + g * (1.0f - s));
+  } else if constexpr (kAct == 1) {  // gelu: g Phi(g)
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    r.f = g * cdf;
+    if (kSlope) r.slope = cdf + g * (0.39894228040143268f * __expf(-0.5f * g * g));
+  } else {  // gelu with tanh: g (1 + tanh z) / 2 = g s(2z), z = sqrt(2/pi) (g + 0.044715 g^3)
+    constexpr float kC = 0.79788456080286536f, kA = 0.044715f;
+    const float s = sigmoid_approx(2.0f * kC * g * (1.0f + kA * g * g));
+    r.f = g * s;
+    if (kSlope) r.slope = s + g * (2.0f * s * (1.0f - s)) * (kC * (1.0f + 3.0f * kA * g * g));
+  }
+  return r;
+}
+
+// Gate and up: the accumulator row holds g in columns [0, 128) and u in
+// [128, 256).  Stores a at columns [n0, n0 + 128) of C and, when kept, g and u
+// through their own maps.  `release` hands the accumulator back once it is in
+// registers.
+template <bool kBf16, int kAct, typename Release>
+__device__ __forceinline__ void gate_up_chunks(const FusedArgs<kEpiGateUp>& fx, const CUtensorMap& tmap_c,
+                                               const EpiParams& sc, uint32_t t_row, uint8_t* epi_buf,
+                                               uint32_t epi_addr, int& sbuf, int lane, int n0, int y,
+                                               Release&& release) {
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    uint32_t pa[32], pg[32], pu[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t g[32], u[32];
+      tmem_ld_32x32b_x32(t_row + c * kEpiCols + h * 32, g);
+      tmem_ld_32x32b_x32(t_row + 128 + c * kEpiCols + h * 32, u);
+      tmem_ld_wait_regs(g);
+      tmem_ld_wait_regs(u);
+      if (c == 1 && h == 1) release();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float a[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          a[i] = activate<kAct, false>(__uint_as_float(g[2 * e + i])).f * __uint_as_float(u[2 * e + i]);
+        pa[16 * h + e] = pack_16bit_rn<kBf16>(__float_as_uint(a[0]), __float_as_uint(a[1]));
+        pg[16 * h + e] = pack_16bit_rn<kBf16>(g[2 * e], g[2 * e + 1]);
+        pu[16 * h + e] = pack_16bit_rn<kBf16>(u[2 * e], u[2 * e + 1]);
+      }
+    }
+    const int x = n0 + c * kEpiCols;
+    epi_store_block_packed<2>(&tmap_c, epi_buf, epi_addr, sbuf, lane, pa, x, y, sc);
+    if (fx.save) {
+      epi_store_block_packed<2>(&fx.tmap_g, epi_buf, epi_addr, sbuf, lane, pg, x, y, sc);
+      epi_store_block_packed<2>(&fx.tmap_u, epi_buf, epi_addr, sbuf, lane, pu, x, y, sc);
+    }
+  }
+}
+
+template <bool kBf16, typename Release>
+__device__ __forceinline__ void gate_up_epilogue(const FusedArgs<kEpiGateUp>& fx, const CUtensorMap& tmap_c,
+                                                 const EpiParams& sc, uint32_t t_row, uint8_t* epi_buf,
+                                                 uint32_t epi_addr, int& sbuf, int lane, int n0, int y,
+                                                 Release&& release) {
+  if (fx.activation == 0)
+    gate_up_chunks<kBf16, 0>(fx, tmap_c, sc, t_row, epi_buf, epi_addr, sbuf, lane, n0, y, release);
+  else if (fx.activation == 1)
+    gate_up_chunks<kBf16, 1>(fx, tmap_c, sc, t_row, epi_buf, epi_addr, sbuf, lane, n0, y, release);
+  else
+    gate_up_chunks<kBf16, 2>(fx, tmap_c, sc, t_row, epi_buf, epi_addr, sbuf, lane, n0, y, release);
+}
+
+// Reads the 32 x 64 blocks of the saved g and u at column x, row y: lane l
+// takes 16-byte piece l % 8 of rows l / 8, l / 8 + 4, ... (whole 128-byte row
+// pieces per instruction).  N is a multiple of 8, so a piece is in or out as a
+// whole; pieces out of range read as 0.
+__device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx, uint4 (&g)[8], uint4 (&u)[8],
+                                               int lane, int x, int y, int M, int N) {
+  const int col = x + (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = y + i * 4 + (lane >> 3);
+    g[i] = u[i] = make_uint4(0, 0, 0, 0);
+    if (row < M && col < N) {
+      const int64_t off = static_cast<int64_t>(row) * fx.ld + col;
+      g[i] = *reinterpret_cast<const uint4*>(fx.g + off);
+      u[i] = *reinterpret_cast<const uint4*>(fx.u + off);
+    }
+  }
+}
+
+// Backward: the accumulator row holds da at columns [n0, n0 + 256).  Per 64
+// columns, g and u go through the warp's two staging buffers into the layout
+// of the accumulator (lane = row), dg and du replace them there and leave by
+// TMA, then a takes the first buffer.  The next block's g and u are fetched
+// meanwhile.
+template <bool kBf16, int kAct, typename Release>
+__device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[8], uint4 (&uv)[8],
+                                                uint32_t t_row, uint8_t* epi_buf, int lane, int n0, int y, int M,
+                                                int N, Release&& release) {
+  uint8_t* buf0 = epi_buf;
+  uint8_t* buf1 = epi_buf + kEpiBufBytes;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const int x = n0 + c * kEpiCols;
+    uint32_t lo[32], hi[32];
+    tmem_ld_32x32b_x32(t_row + c * kEpiCols, lo);
+    tmem_ld_32x32b_x32(t_row + c * kEpiCols + 32, hi);
+    tmem_ld_wait_regs(lo);
+    tmem_ld_wait_regs(hi);
+    if (c == 3) release();
+    if (x >= N) continue;
+    if (lane == 0) bulk_wait_group_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      const int at = r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+      *reinterpret_cast<uint4*>(buf0 + at) = gv[i];
+      *reinterpret_cast<uint4*>(buf1 + at) = uv[i];
+    }
+    __syncwarp();
+    if (c < 3) gate_bwd_fetch(fx, gv, uv, lane, x + kEpiCols, y, M, N);
+    uint32_t pa[32];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = lane * 128 + ((j ^ (lane & 7)) << 4);
+      const uint4 gq = *reinterpret_cast<const uint4*>(buf0 + at);
+      const uint4 uq = *reinterpret_cast<const uint4*>(buf1 + at);
+      const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w}, uw[4] = {uq.x, uq.y, uq.z, uq.w};
+      const uint32_t* d = (j < 4) ? (lo + 8 * j) : (hi + 8 * (j - 4));
+      uint32_t dg[4], du[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 g = unpack_16bit<kBf16>(gw[e]), u = unpack_16bit<kBf16>(uw[e]);
+        const ActValue v0 = activate<kAct, true>(g.x), v1 = activate<kAct, true>(g.y);
+        const float d0 = __uint_as_float(d[2 * e]), d1 = __uint_as_float(d[2 * e + 1]);
+        pa[4 * j + e] = pack_16bit_rn<kBf16>(__float_as_uint(v0.f * u.x), __float_as_uint(v1.f * u.y));
+        dg[e] = pack_16bit_rn<kBf16>(__float_as_uint(d0 * u.x * v0.slope), __float_as_uint(d1 * u.y * v1.slope));
+        du[e] = pack_16bit_rn<kBf16>(__float_as_uint(d0 * v0.f), __float_as_uint(d1 * v1.f));
+      }
+      *reinterpret_cast<uint4*>(buf0 + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+      *reinterpret_cast<uint4*>(buf1 + at) = make_uint4(du[0], du[1], du[2], du[3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(&fx.tmap_dg, buf0, x, y);
+      tma_store_2d(&fx.tmap_du, buf1, x, y);
+      bulk_commit_group();
+      bulk_wait_group_read<0>();
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint4*>(buf0 + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+          make_uint4(pa[4 * j], pa[4 * j + 1], pa[4 * j + 2], pa[4 * j + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(&fx.tmap_a, buf0, x, y);
+      bulk_commit_group();
+    }
+  }
+}
+
+template <bool kBf16, typename Release>
+__device__ __forceinline__ void gate_bwd_epilogue(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[8], uint4 (&uv)[8],
+                                                  uint32_t t_row, uint8_t* epi_buf, int lane, int n0, int y, int M,
+                                                  int N, Release&& release) {
+  if (fx.activation == 0)
+    gate_bwd_chunks<kBf16, 0>(fx, gv, uv, t_row, epi_buf, lane, n0, y, M, N, release);
+  else if (fx.activation == 1)
+    gate_bwd_chunks<kBf16, 1>(fx, gv, uv, t_row, epi_buf, lane, n0, y, M, N, release);
+  else
+    gate_bwd_chunks<kBf16, 2>(fx, gv, uv, t_row, epi_buf, lane, n0, y, M, N, release);
+}
+
+}  // namespace b200

@@ -219,7 +219,7 @@ __device__ __forceinline__ void epi_issue_store(const CUtensorMap* tmap_c, uint8
 // block may write: a tile whose width is not a multiple of 64 ends in a block
 // of which only the columns before x_end are its own; that block leaves by
 // plain stores (the next tile owns the rest of the 64).
-template <int NBUF>
+template <int NBUF, bool kBf16 = false>
 __device__ __forceinline__ void epi_store_block(const CUtensorMap* tmap_c, uint8_t* epi_buf, uint32_t epi_addr,
                                                 int& sbuf, int lane, const uint32_t (&lo)[32],
                                                 const uint32_t (&hi)[32], int x, int y, const EpiParams& sc,
@@ -235,8 +235,9 @@ __device__ __forceinline__ void epi_store_block(const CUtensorMap* tmap_c, uint8
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t* v = (j < 4) ? (lo + 8 * j) : (hi + 8 * (j - 4));
-      st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pack_half2_rn(v[0], v[1]), pack_half2_rn(v[2], v[3]),
-                   pack_half2_rn(v[4], v[5]), pack_half2_rn(v[6], v[7]));
+      st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pack_16bit_rn<kBf16>(v[0], v[1]),
+                   pack_16bit_rn<kBf16>(v[2], v[3]), pack_16bit_rn<kBf16>(v[4], v[5]),
+                   pack_16bit_rn<kBf16>(v[6], v[7]));
     }
   } else {
     bool have_old = false;
@@ -278,15 +279,15 @@ __device__ __forceinline__ void epi_store_block(const CUtensorMap* tmap_c, uint8
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 old = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+          const float2 old = unpack_16bit<kBf16>(o[e]);
           f[2 * e] = fmaf(sc.beta, old.x, f[2 * e]);
           f[2 * e + 1] = fmaf(sc.beta, old.y, f[2 * e + 1]);
         }
       }
-      st_shared_v4(addr, pack_half2_rn(__float_as_uint(f[0]), __float_as_uint(f[1])),
-                   pack_half2_rn(__float_as_uint(f[2]), __float_as_uint(f[3])),
-                   pack_half2_rn(__float_as_uint(f[4]), __float_as_uint(f[5])),
-                   pack_half2_rn(__float_as_uint(f[6]), __float_as_uint(f[7])));
+      st_shared_v4(addr, pack_16bit_rn<kBf16>(__float_as_uint(f[0]), __float_as_uint(f[1])),
+                   pack_16bit_rn<kBf16>(__float_as_uint(f[2]), __float_as_uint(f[3])),
+                   pack_16bit_rn<kBf16>(__float_as_uint(f[4]), __float_as_uint(f[5])),
+                   pack_16bit_rn<kBf16>(__float_as_uint(f[6]), __float_as_uint(f[7])));
     }
   }
   epi_issue_store<NBUF>(tmap_c, buf, sbuf, lane, x, y, sc, x_end);

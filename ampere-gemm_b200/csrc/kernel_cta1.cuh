@@ -5,7 +5,7 @@
 
 namespace b200 {
 
-template <int BN, int STAGES, bool kBRowMajor, bool kAColMajor>
+template <int BN, int STAGES, bool kBRowMajor, bool kAColMajor, bool kBf16 = false>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_f16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                             const __grid_constant__ CUtensorMap tmap_c, int M, int N, int K, int group_m,
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- MMA issuer (one lane) ----------------
     if (lane == 0) {
       constexpr uint32_t idesc =
-          make_idesc_f16_f32(kBM, BN, kAColMajor ? Major::kMN : Major::kK, kBRowMajor ? Major::kMN : Major::kK);
+          make_idesc_f16_f32(kBM, BN, kAColMajor ? Major::kMN : Major::kK, kBRowMajor ? Major::kMN : Major::kK, kBf16);
       const uint32_t a_base = smem_u32(smem_a);
       const uint32_t b_base = smem_u32(smem_b);
       int stage = 0;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&tmem_empty[acc]);
         }
         // The store that last used this buffer must have finished reading it.
-        epi_store_block<2>(&tmap_c, epi_buf, epi_addr, buf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32, sc,
+        epi_store_block<2, kBf16>(&tmap_c, epi_buf, epi_addr, buf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32, sc,
                            &c_bar[ew], c_phase);
       }
     }

@@ -26,6 +26,7 @@
 // (MSUB * KSUB * 4 >= 8) to keep the tensor pipe fed.
 #pragma once
 
+#include "epilogue_gate.cuh"
 #include "gemm_common.cuh"
 
 namespace b200 {
@@ -75,14 +76,19 @@ struct PairConfig {
 // in raster order.  The leader's producer fetches each next tile while the
 // current one loads and hands it to every role of both CTAs through a
 // two-slot queue in shared memory (tile -1 ends the loop).
-template <int STAGES, int KSUB, int MSUB, bool kBRowMajor, bool kAColMajor, int BN = 256, bool kDyn = false>
+template <int STAGES, int KSUB, int MSUB, bool kBRowMajor, bool kAColMajor, int BN = 256, bool kDyn = false,
+          bool kBf16 = false, int kEpi = kEpiPlain>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_f16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                                  const __grid_constant__ CUtensorMap tmap_b,
                                  const __grid_constant__ CUtensorMap tmap_c, int M, int N, int K, int group_m,
-                                 const __grid_constant__ EpiParams sc, const __grid_constant__ SplitTail st) {
+                                 const __grid_constant__ EpiParams sc, const __grid_constant__ SplitTail st,
+                                 const __grid_constant__ FusedArgs<kEpi> fx) {
   using Cfg = PairConfig<STAGES, KSUB, MSUB, BN>;
   constexpr int kAcc = Cfg::kAccBufs;
+  // Columns of C per tile: the gate-and-up tile pairs 128 columns of each.
+  constexpr int kOutN = kEpi == kEpiGateUp ? Cfg::kTileN / 2 : Cfg::kTileN;
+  static_assert(kEpi == kEpiPlain || (MSUB == 1 && BN == 256), "fused epilogues: 256 x 256 pair tiles");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_a = smem;
@@ -117,7 +123,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   TileScheduler sched;
   sched.num_m = (M + Cfg::kTileM - 1) / Cfg::kTileM;
-  sched.num_n = (N + Cfg::kTileN - 1) / Cfg::kTileN;
+  sched.num_n = (N + kOutN - 1) / kOutN;
   sched.group_m = group_m;
   const int num_tiles = sched.num_m * sched.num_n;
   const int num_kb = (K + Cfg::kStageK - 1) / Cfg::kStageK;
@@ -240,7 +246,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int mb, nb;
         sched.tile_coords(u.t, mb, nb);
         const int m0 = mb * Cfg::kTileM + static_cast<int>(rank) * (kBM * MSUB);
-        const int nh0 = nb * Cfg::kTileN + static_cast<int>(rank) * (Cfg::kTileN / 2);
+        // Gate and up: CTA 0 stages the gate's rows of B, CTA 1 the up
+        // projection's (N rows further down), so that each accumulator row
+        // holds both for the same 128 columns.  Rows staged past the gate's
+        // last are the up projection's first; their columns are not stored.
+        const int nh0 = kEpi == kEpiGateUp ? nb * kOutN + static_cast<int>(rank) * N
+                                           : nb * Cfg::kTileN + static_cast<int>(rank) * (Cfg::kTileN / 2);
         for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!B200_TIMED(0, mbar_wait(&empty_bar[stage], phase ^ 1u, kDevTimeoutProducer))) { ok = false; break; }
 #ifdef B200_GEMM_NOLOAD
@@ -300,7 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ---------------- MMA issuer (leader CTA, one lane) ----------------
     if (leader && lane == 0) {
       constexpr uint32_t idesc = make_idesc_f16_f32(256, Cfg::kTileN, kAColMajor ? Major::kMN : Major::kK,
-                                                    kBRowMajor ? Major::kMN : Major::kK);
+                                                    kBRowMajor ? Major::kMN : Major::kK, kBf16);
       const uint32_t a_base = smem_u32(smem_a);
       const uint32_t b_base = smem_u32(smem_b);
       int stage = 0;
@@ -481,6 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int sbuf = 0;
     uint32_t c_phase = 0;
     int local = 0;
+    [[maybe_unused]] uint4 saved_g[8], saved_u[8];
     WorkUnit u;
     auto next_unit = [&](int it, WorkUnit& w) -> bool {
       if constexpr (!kDyn) {
@@ -502,8 +514,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int it = 0; next_unit(it, u); ++it, ++local) {
       int mb, nb;
       sched.tile_coords(u.t, mb, nb);
-      const int n0 = nb * Cfg::kTileN;
+      const int n0 = nb * kOutN;
       const int buf = local % kAcc;
+      if constexpr (kEpi == kEpiGateBwd) {
+        // The tile's first block of g and u arrives while the MMAs still run.
+        const int y = mb * Cfg::kTileM + static_cast<int>(rank) * kBM + quad * 32;
+        gate_bwd_fetch(fx, saved_g, saved_u, lane, n0, y, M, N);
+      }
       const uint32_t acc_phase = (local / kAcc) & 1;
       bool got = true;
 #pragma unroll 1
@@ -522,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
         continue;
 #endif
-        if (MSUB == 1 && u.s >= 0) {
+        if (kEpi == kEpiPlain && MSUB == 1 && u.s >= 0) {
           // Tail unit of a split tile: publish this K range's part, and if it
           // is the last to arrive, sum all parts and store the tile.  Parts
           // move as 8 KB bulk copies ([quad][chunk] blocks of [q][lane]
@@ -656,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 lo[e] = __float_as_uint(acc[e]);
                 hi[e] = __float_as_uint(acc[32 + e]);
               }
-              epi_store_block<2>(&tmap_c, epi_buf, epi_addr, sbuf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32,
+              epi_store_block<2, kBf16>(&tmap_c, epi_buf, epi_addr, sbuf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32,
                                  sc, &c_bar[ew], c_phase);
             }
             asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
@@ -669,6 +686,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
+          continue;
+        }
+        if constexpr (kEpi == kEpiGateUp) {
+          gate_up_epilogue<kBf16>(fx, tmap_c, sc, t_row, epi_buf, epi_addr, sbuf, lane, n0, m0 + quad * 32, [&] {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
+          });
+          continue;
+        }
+        if constexpr (kEpi == kEpiGateBwd) {
+          gate_bwd_epilogue<kBf16>(fx, saved_g, saved_u, t_row, epi_buf, lane, n0, m0 + quad * 32, M, N, [&] {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
+          });
           continue;
         }
         if (MSUB == 2 && sc.alpha == 1.0f && sc.beta == 0.0f) {
@@ -687,8 +720,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tmem_ld_wait_regs(hi);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              pk[c][e] = pack_half2_rn(lo[2 * e], lo[2 * e + 1]);
-              pk[c][16 + e] = pack_half2_rn(hi[2 * e], hi[2 * e + 1]);
+              pk[c][e] = pack_16bit_rn<kBf16>(lo[2 * e], lo[2 * e + 1]);
+              pk[c][16 + e] = pack_16bit_rn<kBf16>(hi[2 * e], hi[2 * e + 1]);
             }
           }
           tc_fence_before_sync();
@@ -715,7 +748,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
           }
-          epi_store_block<2>(&tmap_c, epi_buf, epi_addr, sbuf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32, sc,
+          epi_store_block<2, kBf16>(&tmap_c, epi_buf, epi_addr, sbuf, lane, lo, hi, n0 + c * kEpiCols, m0 + quad * 32, sc,
                              &c_bar[ew], c_phase, n0 + Cfg::kTileN);
         }
       }

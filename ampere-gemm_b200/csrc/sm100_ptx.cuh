@@ -9,6 +9,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 namespace b200 {
@@ -27,8 +28,8 @@ enum DeviceError : int {
   kDevTimeoutSplitFixup = 6, // a split tile's last unit waited too long for another range's part
 };
 
-// Defined here: the library is one translation unit (csrc/b200_gemm.cu).
-__device__ int g_device_error = 0;
+// Each translation unit has its own word; b200_gemm_last_device_error reads them all.
+static __device__ int g_device_error = 0;
 
 // Wall-clock budget of one bounded wait, in nanoseconds (2 s).  The largest
 // GEMM in scope runs for a few milliseconds, so only a lost arrival reaches it.
@@ -314,6 +315,26 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&r)[32]) {
 __device__ __forceinline__ uint32_t pack_half2_rn(uint32_t lo_bits, uint32_t hi_bits) {
   __half2 h = __floats2half2_rn(__uint_as_float(lo_bits), __uint_as_float(hi_bits));
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// The same for either 16-bit type.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_16bit_rn(uint32_t lo_bits, uint32_t hi_bits) {
+  if constexpr (kBf16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo_bits), __uint_as_float(hi_bits));
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    return pack_half2_rn(lo_bits, hi_bits);
+  }
+}
+
+// A packed pair as two fp32.
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack_16bit(uint32_t v) {
+  if constexpr (kBf16)
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

@@ -40,17 +40,19 @@ B200_HD uint64_t make_smem_desc(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t
 // M (for A) or N (for B) index is contiguous (B stored row-major K x N).
 enum class Major : uint32_t { kK = 0, kMN = 1 };
 
-// Instruction descriptor for tcgen05.mma kind::f16 with fp16 A/B and fp32 D:
+// Instruction descriptor for tcgen05.mma kind::f16 with A and B both fp16 or
+// both bf16, and fp32 D:
 //   bits  4..5   D format (1 = f32)
-//   bits  7..9   A format (0 = f16)
-//   bits 10..12  B format (0 = f16)
+//   bits  7..9   A format (0 = f16, 1 = bf16)
+//   bits 10..12  B format (the same as A's)
 //   bit  15      A major (0 = K, 1 = MN)
 //   bit  16      B major
 //   bits 17..22  N >> 3
 //   bits 24..28  M >> 4
-B200_HD uint32_t make_idesc_f16_f32(uint32_t m, uint32_t n, Major a_major, Major b_major) {
+B200_HD uint32_t make_idesc_f16_f32(uint32_t m, uint32_t n, Major a_major, Major b_major, bool bf16 = false) {
   uint32_t d = 0;
   d |= 1u << 4;
+  if (bf16) d |= (1u << 7) | (1u << 10);
   d |= (static_cast<uint32_t>(a_major) & 1u) << 15;
   d |= (static_cast<uint32_t>(b_major) & 1u) << 16;
   d |= ((n >> 3) & 0x3Fu) << 17;

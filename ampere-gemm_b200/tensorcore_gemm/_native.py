@@ -46,6 +46,9 @@ B200_DTYPE_F16 = 0
 B200_DTYPE_BF16 = 1
 B200_DTYPE_F32 = 2
 B200_LOGPROBS_MAX_TOP = 64
+B200_ACT_SILU = 0
+B200_ACT_GELU = 1
+B200_ACT_GELU_TANH = 2
 
 # Every symbol the header declares, with its ctypes signature.
 _SIGNATURES = {
@@ -116,6 +119,17 @@ _SIGNATURES = {
     "b200_token_logprobs_bwd": (
         ctypes.c_int,
         [ctypes.c_void_p] * 7 + [ctypes.c_int64] * 5 + [ctypes.c_int, ctypes.c_void_p],
+    ),
+    "b200_gated_ffn_workspace_size": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "b200_gated_ffn_fwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 8 +
+        [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "b200_gated_ffn_bwd": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 8 + [ctypes.c_int64] * 11 +
+        [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
     ),
     "b200_ipc_handle_size": (ctypes.c_int, []),
     "b200_ipc_alloc": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p]),

@@ -1,0 +1,207 @@
+"""Gated feed-forward block, forward and backward, on B200 kernels.
+
+    g = x Wg^T, u = x Wu^T, a = act(g) u, y = a w_out^T        w_in = [Wg; Wu]
+    da = dy w_out, dg = da u act'(g), du = da act(g)
+    dx = [dg du] w_in, dw_in = [dg du]^T x, dw_out = dy^T a
+
+Both input projections, the activation and the product are one launch, the
+output projection a second one; so is da with dg, du and a in the backward
+pass.  `gated_ffn` is the entry point; `torch.ops.tensorcore_gemm.gated_ffn`
+is the same operator for tracers (it also returns [g u]).  fp16 or bf16
+operands, fp32 accumulation and activation; CUDA tensors only, nothing falls
+back to another implementation.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from ._rows import DTYPE_CODES, as_rows, check_cuda, launch, plain_eager, ptr, wants_grad, workspace
+
+ACTIVATIONS = {"silu": _native.B200_ACT_SILU, "gelu": _native.B200_ACT_GELU, "gelu_tanh": _native.B200_ACT_GELU_TANH}
+
+_TYPES = (torch.float16, torch.bfloat16)
+
+
+def _check(x, w_in, w_out, activation) -> None:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"Unsupported activation {activation!r}. Expected one of {tuple(ACTIVATIONS)}.")
+    for name, t in (("x", x), ("w_in", w_in), ("w_out", w_out)):
+        check_cuda(name, t, _TYPES)
+        if t.dtype != x.dtype:
+            raise RuntimeError(f"{name} must have x's dtype")
+        if t.device != x.device:
+            raise RuntimeError("x, w_in and w_out must be on the same CUDA device")
+    if x.dim() < 1 or w_in.dim() != 2 or w_out.dim() != 2:
+        raise RuntimeError("x needs at least one dimension, w_in and w_out two")
+    if w_in.shape[1] != x.shape[-1]:
+        raise RuntimeError("Inner dimensions must match: w_in is 2F x D for x of width D")
+    if w_in.shape[0] != 2 * w_out.shape[1]:
+        raise RuntimeError("w_in must have twice as many rows (gate, then up) as w_out has columns")
+
+
+def _pad8(n: int) -> int:
+    return -(-n // 8) * 8
+
+
+def _pitched(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`t` as a matrix that TMA can read (unit column stride, 16-byte aligned
+    base and pitch) and its pitch; copied only when it is not one already."""
+    t, ld = as_rows(t)
+    if ld % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, ld
+    rows, cols = t.shape
+    if rows == 1 and t.data_ptr() % 16 == 0:
+        return t, _pad8(cols)                   # one row: its pitch is never used
+    buf = torch.empty((rows, _pad8(cols)), dtype=t.dtype, device=t.device)
+    buf[:, :cols].copy_(t)
+    return buf, buf.shape[1]
+
+
+def _padded_weights(w_in, w_out):
+    """The weights with a hidden width that is a multiple of 8: zero rows after
+    the gate's and after the up projection's, zero columns in w_out.  The
+    hidden units added are 0 throughout."""
+    f = w_out.shape[1]
+    fp = _pad8(f)
+    if fp == f:
+        return w_in, w_out
+    wi = w_in.new_zeros((2, fp, w_in.shape[1]))
+    wi[:, :f].copy_(w_in.reshape(2, f, w_in.shape[1]))
+    wo = w_out.new_zeros((w_out.shape[0], fp))
+    wo[:, :f].copy_(w_out)
+    return wi.view(2 * fp, -1), wo
+
+
+def _result(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """A matrix for the kernels to write: dense when its rows start on 16 bytes, else with padded rows."""
+    buf = torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device)
+    return buf[:, :cols]
+
+
+def _forward(x, w_in, w_out, activation: str, save: bool):
+    """y, and with `save` [g u] (rows x 2 hidden, hidden rounded up to 8) for the backward pass."""
+    dim, out_dim = x.shape[-1], w_out.shape[0]
+    rows = x.numel() // dim if dim else x.shape[:-1].numel()
+    w_in, w_out = _padded_weights(w_in, w_out)
+    hidden = w_out.shape[1]
+    gate_up = torch.empty((rows, 2 * hidden), dtype=x.dtype, device=x.device) if save else None
+    if rows == 0 or out_dim == 0 or dim == 0 or hidden == 0:
+        return x.new_zeros((*x.shape[:-1], out_dim)), gate_up
+    x2, ldx = _pitched(x)
+    wi, ldi = _pitched(w_in)
+    wo, ldo = _pitched(w_out)
+    y = _result(rows, out_dim, x)
+    ws_bytes = _native.load().b200_gated_ffn_workspace_size(rows, hidden, 0)
+    ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
+    launch("b200_gated_ffn_fwd", x.get_device(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr(),
+           ptr(gate_up), rows, dim, hidden, out_dim, ldx, ldi, ldo, _pad8(out_dim), ACTIVATIONS[activation],
+           DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
+    return y.contiguous().view(*x.shape[:-1], out_dim), gate_up
+
+
+def _backward(dy, x, w_in, w_out, gate_up, activation: str, need_x: bool, need_in: bool, need_out: bool):
+    """dx, dw_in and dw_out (None where not needed)."""
+    dim, (out_dim, f) = x.shape[-1], w_out.shape
+    rows = gate_up.shape[0]
+    if rows == 0 or out_dim == 0 or dim == 0 or f == 0:
+        return (torch.zeros_like(x, memory_format=torch.contiguous_format) if need_x else None,
+                w_in.new_zeros(w_in.shape) if need_in else None, w_out.new_zeros(w_out.shape) if need_out else None)
+    wi, wo = _padded_weights(w_in, w_out)
+    hidden = wo.shape[1]
+    dy2, lddy = _pitched(dy)
+    x2, ldx = _pitched(x)
+    wi, ldi = _pitched(wi)
+    wo, ldo = _pitched(wo)
+    dx = _result(rows, dim, x) if need_x else None
+    dwi = _result(2 * hidden, dim, x) if need_in else None
+    dwo = _result(out_dim, hidden, x) if need_out else None
+    ws_bytes = _native.load().b200_gated_ffn_workspace_size(rows, hidden, 1)
+    ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
+    launch("b200_gated_ffn_bwd", x.get_device(), dy2.data_ptr(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(),
+           gate_up.data_ptr(), ptr(dx), ptr(dwi), ptr(dwo), rows, dim, hidden, out_dim, lddy, ldx, ldi, ldo,
+           _pad8(dim), _pad8(dim), hidden, ACTIVATIONS[activation], DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
+    if need_x:
+        dx = dx.contiguous().view(x.shape)
+    if need_in:
+        dwi = dwi.contiguous() if hidden == f else dwi.unflatten(0, (2, hidden))[:, :f].reshape(2 * f, dim)
+    if need_out:
+        dwo = dwo[:, :f].contiguous()
+    return dx, dwi, dwo
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, activation):
+        y, gate_up = _forward(x, w_in, w_out, activation, True)
+        ctx.save_for_backward(x, w_in, w_out, gate_up)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return *_backward(dy, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:3]), None
+
+
+def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """y = (act(x Wg^T) * (x Wu^T)) w_out^T for x (..., D), w_in = [Wg; Wu] (2F x D) and w_out (N x F).
+
+    All float16 or all bfloat16.  activation: "silu", "gelu" or "gelu_tanh".
+    Any sizes and strides; operands whose rows do not start on 16 bytes, and
+    weights whose F is not a multiple of 8, are copied first.  Differentiable
+    in x, w_in and w_out (once).  a = act(g) u (and, for the backward pass, g
+    and u) are rounded to x's type.
+    """
+    if not plain_eager(x, w_in, w_out):
+        return torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, activation)[0]
+    _check(x, w_in, w_out, activation)
+    if wants_grad(x, w_in, w_out):
+        return _GatedFfn.apply(x, w_in, w_out, activation)
+    return _forward(x, w_in, w_out, activation, False)[0]
+
+
+# ---------------------------------------------------------------------------
+# The dispatcher operators
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("tensorcore_gemm::gated_ffn", mutates_args=())
+def _gated_ffn_op(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
+                  activation: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """y and [g u] of `gated_ffn` (the latter is not differentiable)."""
+    _check(x, w_in, w_out, activation)
+    return _forward(x, w_in, w_out, activation, True)
+
+
+@_gated_ffn_op.register_fake
+def _(x, w_in, w_out, activation):
+    _check(x, w_in, w_out, activation)
+    rows = x.shape[:-1].numel()
+    return (torch.empty((*x.shape[:-1], w_out.shape[0]), dtype=x.dtype, device=x.device),
+            torch.empty((rows, 2 * _pad8(w_out.shape[1])), dtype=x.dtype, device=x.device))
+
+
+@torch.library.custom_op("tensorcore_gemm::gated_ffn_backward", mutates_args=())
+def _gated_ffn_backward_op(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
+                           gate_up: torch.Tensor,
+                           activation: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _backward(dy, x, w_in, w_out, gate_up, activation, True, True, True)
+
+
+@_gated_ffn_backward_op.register_fake
+def _(dy, x, w_in, w_out, gate_up, activation):
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, w_in, w_out))
+
+
+def _setup_context(ctx, inputs, output) -> None:
+    x, w_in, w_out, activation = inputs
+    ctx.save_for_backward(x, w_in, w_out, output[1])
+    ctx.activation = activation
+    ctx.mark_non_differentiable(output[1])
+
+
+def _op_backward(ctx, dy, _dgate_up):
+    return *torch.ops.tensorcore_gemm.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation), None
+
+
+_gated_ffn_op.register_autograd(_op_backward, setup_context=_setup_context)

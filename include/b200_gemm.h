@@ -243,6 +243,40 @@ B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets,
                                      void* dlogits, int64_t rows, int64_t vocab, int64_t ld, int64_t ldd,
                                      int64_t ignore_index, int dtype, void* stream);
 
+/*
+ * Gated feed-forward block: with w_in = [Wg; Wu] (2 hidden x dim) and w_out
+ * (out_dim x hidden),
+ *   g = x Wg^T, u = x Wu^T, a = act(g) u, y = a w_out^T
+ * for `rows` rows of x, all of `dtype` (B200_DTYPE_F16 or B200_DTYPE_BF16) with
+ * fp32 accumulation and activation; a is rounded to `dtype` between the two
+ * launches.  gate_up (rows x 2 hidden, dense; may be NULL) receives [g u] for
+ * the backward call.  Operands as for b200_gemm_f16 (16-byte bases, pitches a
+ * multiple of 8 elements), and hidden a multiple of 8: B200_ERR_MISALIGNED
+ * otherwise.  The workspace (b200_gated_ffn_workspace_size bytes, 256-byte
+ * aligned) holds a, in the backward also dg and du; it must not be reused
+ * until the call's work on `stream` has finished.  No counterpart in the
+ * reference.
+ */
+#define B200_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define B200_ACT_GELU 1      /* g Phi(g), Phi the normal distribution function */
+#define B200_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+B200_API int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int backward);
+B200_API int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w_out, void* y, void* gate_up,
+                                int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int64_t ldx,
+                                int64_t ldw_in, int64_t ldw_out, int64_t ldy, int activation, int dtype,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients: da = dy w_out, dg = da u act'(g), du = da act(g),
+ *   dx = [dg du] w_in, dw_in = [dg du]^T x, dw_out = dy^T a
+ * (each may be NULL when it is not wanted).
+ */
+B200_API int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_in, const void* w_out,
+                                const void* gate_up, void* dx, void* dw_in, void* dw_out, int64_t rows, int64_t dim,
+                                int64_t hidden, int64_t out_dim, int64_t lddy, int64_t ldx, int64_t ldw_in,
+                                int64_t ldw_out, int64_t lddx, int64_t lddw_in, int64_t lddw_out, int activation,
+                                int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Human-readable text of a return code (static storage). Counterpart of the
  * TORCH_CHECK messages of the reference launcher (gemm.py:33-47, 150-152). */
 B200_API const char* b200_gemm_strerror(int code);

@@ -1,0 +1,329 @@
+"""The gated feed-forward block, forward and backward, against the formulas in 64 bits.
+
+Tolerances.  Every product sums n 16-bit products in fp32: off by at most
+n * 2^-24 of the sum of their magnitudes.  Results, and a, g, u, dg and du
+between the launches, are rounded to the operands' type (u = 2^-11 for fp16,
+2^-8 for bf16, and half a subnormal step of fp16).  `Exact` carries a bound
+beside each value: for a product A B^T with elementwise bounds eA, eB it is
+|A| eB + eA |B| + eA eB + n 2^-24 |A||B|, for a function of g the derivative's
+maximum times g's bound; approximate exponentials add a relative 2^-19.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tensorcore_gemm import ffn
+
+F16, BF16 = torch.float16, torch.bfloat16
+UNIT = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TINY = {F16: 2.0 ** -25, BF16: 1e-37}
+E19 = 2.0 ** -19
+
+
+def make(rows, dim, hidden, out_dim, dtype, dev, seed=0):
+    gen = torch.Generator().manual_seed(rows + 10 * dim + 100 * hidden + seed)
+    t = lambda r, c, s: (s * torch.randn((r, c), generator=gen)).to(dtype).to(dev)
+    return (t(rows, dim, 1.0), t(2 * hidden, dim, dim ** -0.5), t(out_dim, hidden, hidden ** -0.5), t(rows, out_dim, 1.0))
+
+
+def act64(kind, g):
+    """act(g), act'(g), and bounds of |act'| and |act''|."""
+    if kind == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s + g * s * torch.sigmoid(-g), 1.1, 0.5
+    if kind == "gelu":
+        c = torch.special.ndtr(g)
+        return g * c, c + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi), 1.13, 0.8
+    k = math.sqrt(2 / math.pi)
+    s = torch.sigmoid(2 * k * (g + 0.044715 * g ** 3))
+    return g * s, s + 2 * g * s * (1 - s) * k * (1 + 3 * 0.044715 * g * g), 1.13, 0.85
+
+
+class Val:
+    """A value with an elementwise bound of how far the kernels' may be off."""
+
+    def __init__(self, v, e=None):
+        self.v, self.e = v.double(), torch.zeros_like(v, dtype=torch.float64) if e is None else e
+
+    def t(self):
+        return Val(self.v.t(), self.e.t())
+
+    def dot(self, b):
+        """self @ b^T"""
+        a, n = self, self.v.shape[1]
+        aa, bb = a.v.abs(), b.v.abs()
+        e = aa @ b.e.t() + a.e @ bb.t() + a.e @ b.e.t() + n * 2.0 ** -24 * (aa @ bb.t())
+        return Val(a.v @ b.v.t(), e)
+
+    def times(self, b):
+        e = self.v.abs() * b.e + self.e * b.v.abs() + self.e * b.e
+        v = self.v * b.v
+        return Val(v, e + 2.0 ** -23 * v.abs())
+
+    def rounded(self, dtype):
+        return Val(self.v, self.e + UNIT[dtype] * (self.v.abs() + self.e) + TINY[dtype])
+
+    def check(self, got):
+        assert ((got.double() - self.v).abs() <= self.e).all(), ((got.double() - self.v).abs() / self.e).max()
+
+
+class Exact:
+    def __init__(self, x, w_in, w_out, kind, dy=None):
+        dt = x.dtype
+        hidden = w_out.shape[1]
+        X, Wi, Wo = Val(x), Val(w_in), Val(w_out)
+        gu = X.dot(Wi)
+        g, u = Val(gu.v[:, :hidden], gu.e[:, :hidden]), Val(gu.v[:, hidden:], gu.e[:, hidden:])
+
+        def apply(g):
+            f, s, l1, l2 = act64(kind, g.v)
+            fe = l1 * g.e + E19 * (f.abs() + 2.0 ** -4 * g.v.abs())
+            return Val(f, fe), Val(s, l2 * g.e + E19 * (1 + g.v.abs()))
+
+        self.y = apply(g)[0].times(u).rounded(dt).dot(Wo).rounded(dt)
+        if dy is None:
+            return
+        DY = Val(dy)
+        g, u = g.rounded(dt), u.rounded(dt)
+        f, s = apply(g)
+        a = f.times(u).rounded(dt)
+        da = DY.dot(Wo.t())
+        dg, du = da.times(u).times(s).rounded(dt), da.times(f).rounded(dt)
+        dgu = Val(torch.cat([dg.v, du.v], 1), torch.cat([dg.e, du.e], 1))
+        self.dx = dgu.dot(Wi.t()).rounded(dt)
+        self.dw_in = dgu.t().dot(X.t()).rounded(dt)
+        self.dw_out = DY.t().dot(a.t()).rounded(dt)
+
+
+def run(x, w_in, w_out, kind, dy):
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w_in, w_out)]
+    y = ffn.gated_ffn(*leaves, activation=kind)
+    return y, *torch.autograd.grad(y, leaves, dy)
+
+
+def check_all(x, w_in, w_out, kind, dy):
+    ex = Exact(x, w_in, w_out, kind, dy)
+    y, dx, dwi, dwo = run(x, w_in, w_out, kind, dy)
+    ex.y.check(ffn.gated_ffn(x, w_in, w_out, activation=kind))
+    for want, got, like in ((ex.y, y, dy), (ex.dx, dx, x), (ex.dw_in, dwi, w_in), (ex.dw_out, dwo, w_out)):
+        assert got.shape == like.shape and got.dtype == like.dtype
+        want.check(got)
+
+
+# rows, dim, hidden, out_dim: one row, few, odd ones, sizes around the tiles (256 rows, 128 hidden units, 64 deep)
+SIZES = [(1, 8, 8, 8), (1, 256, 512, 256), (3, 64, 128, 64), (17, 100, 60, 100), (33, 129, 131, 65), (128, 128, 128, 128),
+         (130, 200, 264, 200), (256, 512, 1000, 512), (257, 511, 1001, 510), (700, 96, 384, 104), (1500, 320, 72, 320),
+         (64, 1024, 2816, 1024), (2, 2000, 33, 7)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(ffn.ACTIVATIONS))
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size", SIZES)
+def test_forward_and_gradients(cuda_device, native_lib, size, dtype, kind):
+    x, w_in, w_out, dy = make(*size, dtype, cuda_device)
+    check_all(x, w_in, w_out, kind, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [2, 5, 8, 9, 15, 16, 24, 31, 32, 48, 63, 65, 100, 127, 129, 200, 255, 300])
+def test_row_counts(cuda_device, native_lib, rows, dtype):
+    """Every row count near where the kernels change."""
+    x, w_in, w_out, _ = make(rows, 384, 776, 392, dtype, cuda_device)
+    Exact(x, w_in, w_out, "silu").y.check(ffn.gated_ffn(x, w_in, w_out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_large_gates(cuda_device, native_lib, rows):
+    """Gates far into both tails: no overflow on the way."""
+    x, w_in, w_out, dy = make(rows, 64, 136, 64, BF16, cuda_device)
+    w_in = w_in.clone()
+    w_in[:136] *= 100
+    for kind in ffn.ACTIVATIONS:
+        y, dx, dwi, dwo = run(x, w_in, w_out, kind, dy)
+        ex = Exact(x, w_in, w_out, kind)
+        ex.y.check(y)
+        assert all(t.isfinite().all() for t in (y, dx, dwi, dwo))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_strided_operands(cuda_device, native_lib, rows):
+    x, w_in, w_out, dy = make(rows, 200, 160, 120, F16, cuda_device)
+    want = Exact(x[:, 8:136], w_in[:, 16:144], w_out[:, :160], "silu", dy[:, :120])
+    y, dx, dwi, dwo = run(x[:, 8:136], w_in[:, 16:144], w_out[:, :160], "silu", dy[:, :120])
+    want.y.check(y)
+    leaf = [t.clone().requires_grad_() for t in (x, w_in, w_out)]
+    y = ffn.gated_ffn(leaf[0][:, 8:136], leaf[1][:, 16:144], leaf[2])
+    want.y.check(y)
+    g = torch.autograd.grad(y, leaf, dy)
+    want.dx.check(g[0][:, 8:136])
+    want.dw_in.check(g[1][:, 16:144])
+    want.dw_out.check(g[2])
+    # misaligned columns, transposed storage, expanded rows, more dimensions
+    Exact(x[:, 3:131], w_in[:, 1:129], w_out, "gelu").y.check(
+        ffn.gated_ffn(x[:, 3:131], w_in[:, 1:129], w_out, activation="gelu"))
+    xt, wit, wot = (t.t().contiguous().t() for t in (x, w_in, w_out))
+    Exact(x, w_in, w_out, "silu").y.check(ffn.gated_ffn(xt, wit, wot))
+    e = x[:1].expand(rows, 200)
+    Exact(e, w_in, w_out, "silu").y.check(ffn.gated_ffn(e, w_in, w_out))
+    assert torch.equal(ffn.gated_ffn(x.view(rows, 1, 200), w_in, w_out).view(rows, 120), ffn.gated_ffn(x, w_in, w_out))
+
+
+@pytest.mark.gpu
+def test_only_some_gradients(cuda_device, native_lib):
+    x, w_in, w_out, dy = make(70, 64, 96, 80, BF16, cuda_device)
+    full = run(x, w_in, w_out, "silu", dy)[1:]
+    for i in range(3):
+        args = [x, w_in, w_out]
+        args[i] = args[i].clone().requires_grad_()
+        g, = torch.autograd.grad(ffn.gated_ffn(*args), (args[i],), dy)
+        assert torch.equal(g, full[i])
+
+
+@pytest.mark.gpu
+def test_nan_stays_in_its_row(cuda_device, native_lib):
+    for rows in (6, 300):
+        x, w_in, w_out, _ = make(rows, 128, 256, 128, F16, cuda_device)
+        x = x.clone()
+        x[2, 5] = float("nan")
+        y = ffn.gated_ffn(x, w_in, w_out)
+        assert y[2].isnan().all()
+        good = [i for i in range(rows) if i != 2]
+        Exact(x[good], w_in, w_out, "silu").y.check(y[good])
+
+
+@pytest.mark.gpu
+def test_results_do_not_change_from_run_to_run(cuda_device, native_lib):
+    for rows in (4, 40, 900):
+        x, w_in, w_out, dy = make(rows, 512, 1400, 512, BF16, cuda_device)
+        first = run(x, w_in, w_out, "silu", dy)
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(first, run(x, w_in, w_out, "silu", dy)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(ffn.ACTIVATIONS))
+def test_gradient_against_differences(cuda_device, native_lib, kind):
+    """The gradient along v against the central difference of the 64-bit function (step 1e-4, error about 1e-7).
+
+    The kernels' gradient of 64 x 48 elements carries roundings of 2^-11 that are independent of v, each
+    weighted with at most its value; four standard deviations of their sum are allowed."""
+    x, w_in, w_out, dy = make(64, 48, 56, 48, F16, cuda_device)
+    grads = run(x, w_in, w_out, kind, dy)[1:]
+    gen = torch.Generator().manual_seed(2)
+    for i, g in enumerate(grads):
+        v = torch.randn(g.shape, generator=gen).to(cuda_device).double()
+
+        def f(s):
+            args = [t.double() for t in (x, w_in, w_out)]
+            args[i] = args[i] + s * v
+            gate, up = (args[0] @ args[1].t()).chunk(2, 1)
+            return (dy.double() * ((act64(kind, gate)[0] * up) @ args[2].t())).sum()
+
+        diff = (f(1e-4) - f(-1e-4)) / 2e-4
+        got = (g.double() * v).sum()
+        # roundings on the way: of g, u (through a smooth function), a or dg and du, and the result
+        assert abs(got - diff) <= 4 * 4 * 2.0 ** -11 * (g.double() * v).square().sum().sqrt() + 1e-4
+
+
+@pytest.mark.gpu
+def test_empty(cuda_device, native_lib):
+    for rows, dim, hidden, out_dim in [(0, 16, 8, 16), (5, 0, 8, 16), (5, 16, 0, 16), (5, 16, 8, 0)]:
+        x, w_in, w_out, dy = (torch.ones(s, device=cuda_device, dtype=F16) for s in
+                              ((rows, dim), (2 * hidden, dim), (out_dim, hidden), (rows, out_dim)))
+        for t in run(x, w_in, w_out, "silu", dy):
+            assert not t.any()
+        assert not ffn.gated_ffn(x, w_in, w_out).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 30, 400])
+def test_stream_and_graph(cuda_device, native_lib, rows):
+    x, w_in, w_out, _ = make(rows, 512, 1024, 512, F16, cuda_device)
+    ex = Exact(x, w_in, w_out, "silu")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(20):                              # back to back, weights written just before their use
+            wi, wo = w_in * 1.0, w_out * 1.0
+            y = ffn.gated_ffn(x, wi, wo)
+    s.synchronize()
+    ex.y.check(y)
+    buf = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ffn.gated_ffn(buf, w_in, w_out)
+    buf.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    ex.y.check(out)
+
+
+@pytest.mark.gpu
+def test_dispatcher_operator(cuda_device, native_lib):
+    x, w_in, w_out, dy = make(40, 64, 72, 64, F16, cuda_device)
+    leaves = [t.clone().requires_grad_() for t in (x, w_in, w_out)]
+    y, gate_up = torch.ops.tensorcore_gemm.gated_ffn(*leaves, "silu")
+    assert gate_up.shape == (40, 144)
+    for p, q in zip((y, *torch.autograd.grad(y, leaves, dy)), run(x, w_in, w_out, "silu", dy)):
+        assert torch.equal(p, q)
+    torch.library.opcheck(torch.ops.tensorcore_gemm.gated_ffn, (*leaves, "silu"),
+                          test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.gpu
+def test_refusals(cuda_device, native_lib):
+    x, w_in, w_out, _ = make(4, 16, 8, 16, F16, cuda_device)
+    for args, match in [((x.float(), w_in, w_out), "float16 or bfloat16"), ((x, w_in.bfloat16(), w_out), "dtype"),
+                        ((x, w_in[:, :8], w_out), "Inner"), ((x, w_in[:15], w_out), "twice"),
+                        ((x, w_in, w_out.cpu()), "CUDA"), ((x, w_in[0], w_out), "two")]:
+        with pytest.raises(RuntimeError, match=match):
+            ffn.gated_ffn(*args)
+    with pytest.raises(ValueError, match="Unsupported activation"):
+        ffn.gated_ffn(x, w_in, w_out, activation="relu")
+    a = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(ffn.gated_ffn(a, w_in, w_out).sum(), (a,), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+def test_cpu_tensors_raise():
+    t = torch.zeros((8, 8), dtype=F16)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        ffn.gated_ffn(t, torch.zeros((16, 8), dtype=F16), t)
+
+
+def test_fake_shapes_without_gpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(allow_non_fake_inputs=False):
+        x = torch.empty((3, 5, 16), dtype=BF16, device="cuda")
+        w_in, w_out = (torch.empty(s, dtype=BF16, device="cuda") for s in ((22, 16), (24, 11)))
+        y = ffn.gated_ffn(x, w_in, w_out)
+        assert y.shape == (3, 5, 24) and y.dtype == BF16
+        with pytest.raises(RuntimeError, match="twice"):
+            ffn.gated_ffn(x, w_in[:20], w_out)
+
+
+def test_c_argument_checks_without_gpu(native_lib):
+    size, fwd, bwd = (native_lib.b200_gated_ffn_workspace_size, native_lib.b200_gated_ffn_fwd,
+                      native_lib.b200_gated_ffn_bwd)
+    p = 4096
+    assert size(-1, 8, 0) == -1 and size(4, 64, 0) == 512 and size(4, 64, 1) == 512 + 1024
+    args = [p] * 5 + [4, 64, 64, 64, 64, 64, 64, 64, 0, 1, p, 1 << 20, None]
+    def with_(a, i, v):
+        return [v if j == i else q for j, q in enumerate(a)]
+    for i, v, code in [(0, None, 1), (1, None, 1), (2, None, 1), (3, None, 1), (5, -1, 1), (5, 1 << 31, 3), (7, 63, 2),
+                       (9, 63, 1), (9, 68, 2), (12, 60, 1), (13, 3, 1), (14, 2, 1), (15, None, 8), (15, p + 8, 8),
+                       (16, 511, 8), (0, p + 2, 2), (4, p + 2, 2)]:
+        assert fwd(*with_(args, i, v)) == code, (i, v)
+    args = [p] * 8 + [4, 64, 64, 64] + [64] * 7 + [0, 1, p, 1 << 20, None]
+    for i, v, code in [(0, None, 1), (4, None, 1), (4, p + 2, 2), (5, p + 2, 2), (16, 63, 1), (16, 68, 2), (18, 60, 1),
+                       (21, p + 8, 8), (22, 1535, 8)]:
+        assert bwd(*with_(args, i, v)) == code, (i, v)
