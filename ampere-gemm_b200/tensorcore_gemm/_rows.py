@@ -3,6 +3,8 @@ logprobs): argument checks, the 2-D view the C ABI takes, workspaces and the
 launch on torch's current stream."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native
@@ -74,3 +76,38 @@ def plain_eager(*tensors) -> bool:
 
 def wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _Refuse(torch.autograd.Function):
+    """Identity whose differentiation raises."""
+
+    @staticmethod
+    def forward(ctx, *tensors):
+        return tuple(t.view_as(t) for t in tensors)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this gradient cannot be differentiated again: the operator is once_differentiable")
+
+
+def once_differentiable(backward):
+    """A Function's backward whose results refuse to be differentiated.
+
+    torch's decorator of that name lets a second differentiation through,
+    as a constant, when the incoming gradient needs none itself."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        again = torch.is_grad_enabled()          # create_graph=True
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not again:
+            return out
+        at = [i for i, t in enumerate(out) if t is not None]
+        refused = _Refuse.apply(*(out[i].detach().requires_grad_() for i in at)) if at else ()
+        out = list(out)
+        for i, t in zip(at, refused):
+            out[i] = t
+        return tuple(out)
+
+    return wrapper

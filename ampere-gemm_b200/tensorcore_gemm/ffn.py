@@ -14,10 +14,10 @@ back to another implementation.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._rows import DTYPE_CODES, as_rows, check_cuda, launch, plain_eager, ptr, wants_grad, workspace
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+                    workspace)
 
 ACTIVATIONS = {"silu": _native.B200_ACT_SILU, "gelu": _native.B200_ACT_GELU, "gelu_tanh": _native.B200_ACT_GELU_TANH}
 

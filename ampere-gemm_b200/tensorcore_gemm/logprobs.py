@@ -17,10 +17,10 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._rows import DTYPE_CODES, as_rows, check_cuda, launch, plain_eager, ptr, wants_grad, workspace
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+                    workspace)
 
 #: Most alternatives a call can ask for.
 MAX_TOP = _native.B200_LOGPROBS_MAX_TOP

@@ -15,10 +15,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._rows import DTYPE_CODES, as_rows, check_cuda, launch, plain_eager, ptr, wants_grad, workspace
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+                    workspace)
 
 
 def _check(x, weight, bias) -> None:
