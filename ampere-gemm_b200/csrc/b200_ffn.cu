@@ -17,6 +17,7 @@
 
 #include "gemm_internal.h"
 #include "kernel_cta2.cuh"
+#include "kernel_rows.cuh"
 #include "tensor_map.cuh"
 
 namespace b200 {
@@ -98,6 +99,122 @@ int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int6
   return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, stream);
 }
 
+// ---- few rows of x (kernel_rows.cuh) ----
+
+constexpr int kRowsMaxSmem = 220 * 1024;
+
+// Largest number of S-CTA clusters of the rows kernel resident at once, one
+// CTA an SM.
+template <typename Kern>
+int rows_clusters(Kern kern, int parts, int sm_count) {
+  if (parts == 1) return sm_count;
+  static int cache[kMaxDevices][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sm_count / parts;
+  int& n = cache[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3];
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count / parts * parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kRowsMaxSmem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int got = 0;
+  if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess || got <= 0) {
+    (void)cudaGetLastError();
+    got = sm_count / parts;
+  }
+  return n = std::min(got, sm_count / parts);
+}
+
+// Stages fit beside another CTA of the kind (the next launch's, which starts
+// to read its weights early) when they take this much; a stage too large for
+// two in that space takes what one CTA may have.
+int rows_limit() {
+  static const int v = [] {
+    const char* e = std::getenv("B200_FFN_ROWS");
+    return e ? std::atoi(e) : kRowsMaxTokens;
+  }();
+  return v;
+}
+
+constexpr int kRowsPairRing = 94 * 1024;
+constexpr int kRowsSoloRing = 200 * 1024;
+
+template <bool kBf16, bool kGate>
+int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ld_out, int tokens, int n,
+                int k, int act, bool w_early, const DeviceInfo& dev, cudaStream_t stream) {
+  auto kern = gemm_rows_kernel<kBf16, kGate>;
+  static std::atomic<uint8_t> attr_done[kMaxDevices];
+  if (int e = ensure_smem_attr(kern, kRowsMaxSmem, attr_done)) return e;
+  constexpr int kAccs = kGate ? 2 : 1;
+  RowsShape sh;
+  sh.tokens = tokens;
+  sh.tokens_pad = (tokens + 15) / 16 * 16;
+  sh.n = n;
+  sh.k_blocks = (k + kBK - 1) / kBK;
+  sh.activation = act;
+  sh.w_early = w_early ? 1 : 0;
+  // CTAs of a cluster: the number that makes a CTA's loads (its rows of w and
+  // all of x, over its share of K) fewest; a cluster's reduction costs about
+  // as much as 48 KB of loads.
+  int parts = 1;
+  long long best = -1;
+  for (int s = 1; s <= 8 && s <= sh.k_blocks; s *= 2) {
+    const int slots = rows_clusters(kern, s, dev.sm_count);
+    const int waves = (n + slots * 128 - 1) / (slots * 128);
+    const int block = (n + slots * waves - 1) / (slots * waves);
+    const long long bytes = (long long)waves * (kAccs * block + sh.tokens_pad) * 128 * ((sh.k_blocks + s - 1) / s) +
+                            (s > 1 ? 48 * 1024 : 0);
+    if (best < 0 || bytes < best) {
+      best = bytes;
+      parts = s;
+      sh.block = block;
+    }
+  }
+  sh.block_pad = (sh.block + 7) / 8 * 8;
+  const int sub = rows_sub_bytes(sh, kGate);
+  const int share = (sh.k_blocks + parts - 1) / parts;
+  sh.k_sub = std::max(1, std::min({16 * 1024 / sub, 8, share}));
+  const int stage = sub * sh.k_sub;
+  const int ring = 3 * stage <= kRowsPairRing ? kRowsPairRing : kRowsSoloRing;
+  sh.stages = std::min({ring / stage, kRowsMaxStages, (share + sh.k_sub - 1) / sh.k_sub});
+  sh.tail = (int)round_up(std::max(0, (128 - sh.block_pad - sh.tokens_pad) * 128), 1024);
+  // Tokens of a reduction round: what the stages hold in fp32.
+  sh.chunk = std::min(sh.tokens_pad, (sh.stages * stage + sh.tail) / (kAccs * 512) / 16 * 16);
+  if (parts > 1 && sh.chunk < 16) {
+    sh.tail += 16 * kAccs * 512;
+    sh.chunk = 16;
+  }
+  const int smem = sh.stages * stage + sh.tail + kRowsBarBytes + 1024;
+  if (smem > kRowsMaxSmem) return B200_ERR_CUDA;
+  CUtensorMap tw, tx;
+  int rc = make_tmap_2d(&tw, w, (uint64_t)kAccs * n, k, ldw, kBK, sh.block, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tx, x, tokens, k, ldx, kBK, sh.tokens_pad, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((n + sh.block - 1) / sh.block * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, static_cast<uint16_t*>(out), ld_out, sh);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
 // Checks shared by the two directions; *empty: some dimension is 0.
 int check_ffn(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int activation, int dtype, bool* empty) {
   if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return B200_ERR_INVALID_ARGUMENT;
@@ -165,6 +282,14 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   const bool bf16 = dtype == B200_DTYPE_BF16;
   uint16_t* a = static_cast<uint16_t*>(workspace);
   const GateShape s{(int)rows, (int)hidden, (int)dim};
+  const bool few = rows <= rows_limit();
+  if (few && !gate_up) {
+    const int rc = (bf16 ? launch_rows<true, true> : launch_rows<false, true>)(
+        x, ldx, w_in, ldw_in, a, hidden, (int)rows, (int)hidden, (int)dim, activation, false, dev, stream);
+    if (rc) return rc;
+    return (bf16 ? launch_rows<true, false> : launch_rows<false, false>)(
+        a, hidden, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim, (int)hidden, 0, true, dev, stream);
+  }
   const int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(x, ldx, w_in, ldw_in, a,
                                                                      static_cast<uint16_t*>(gate_up), activation, s,
                                                                      stream);
