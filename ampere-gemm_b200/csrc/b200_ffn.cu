@@ -131,19 +131,15 @@ int rows_clusters(Kern kern, int parts, int sm_count) {
   return n = std::min(got, sm_count / parts);
 }
 
-// Stages fit beside another CTA of the kind (the next launch's, which starts
-// to read its weights early) when they take this much; a stage too large for
-// two in that space takes what one CTA may have.
-int rows_limit() {
-  static const int v = [] {
-    const char* e = std::getenv("B200_FFN_ROWS");
-    return e ? std::atoi(e) : kRowsMaxTokens;
-  }();
-  return v;
+// Few enough rows of x for the rows kernel.  It reads the weights once, evenly
+// over the SMs (4096 x 12288: 54 us for 1 token, 69 for 128, 119 for 256,
+// against 294, 131 and 133 with the pair kernel, whose loads of a mostly empty
+// tile of x collide); its epilogue grows with the tokens, which small weights
+// do not hide (512 x 1408: 18 us for 128 tokens, 22 for 160, pair 22; 128 x
+// 400: 10 for 32, 13.5 for 64, pair 13).
+bool few_rows(int64_t rows, int64_t dim, int64_t hidden) {
+  return rows <= kRowsMaxTokens && 25 * rows * rows <= dim * hidden;
 }
-
-constexpr int kRowsPairRing = 94 * 1024;
-constexpr int kRowsSoloRing = 200 * 1024;
 
 template <bool kBf16, bool kGate>
 int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ld_out, int tokens, int n,
@@ -159,19 +155,25 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* ou
   sh.k_blocks = (k + kBK - 1) / kBK;
   sh.activation = act;
   sh.w_early = w_early ? 1 : 0;
-  // CTAs of a cluster: the number that makes a CTA's loads (its rows of w and
-  // all of x, over its share of K) fewest; a cluster's reduction costs about
-  // as much as 48 KB of loads.
+  // CTAs of a cluster: the least estimated time of a CTA, in cycles.  A 64-deep
+  // block of K costs 5.1 a row of w (128 bytes at the 25 bytes a cycle that an
+  // SM gets of the memory's rate), 2 a token (from L2), and 0.4 of its MMAs'
+  // time (4 an accumulator, 42 each or N / 2), which the loads hide in part; a
+  // cluster's reduction costs 700, another wave 3000.  Fitted to sweeps over
+  // 512 x 1408 to 4096 x 12288 and 1 to 128 tokens (a row block per SM, no
+  // clusters, was 1.3-2.3x slower for w_out).
   int parts = 1;
-  long long best = -1;
-  for (int s = 1; s <= 8 && s <= sh.k_blocks; s *= 2) {
+  double best = -1.0;
+  for (int s = 1; s <= kRowsMaxParts && s <= sh.k_blocks; s *= 2) {
     const int slots = rows_clusters(kern, s, dev.sm_count);
     const int waves = (n + slots * 128 - 1) / (slots * 128);
     const int block = (n + slots * waves - 1) / (slots * waves);
-    const long long bytes = (long long)waves * (kAccs * block + sh.tokens_pad) * 128 * ((sh.k_blocks + s - 1) / s) +
-                            (s > 1 ? 48 * 1024 : 0);
-    if (best < 0 || bytes < best) {
-      best = bytes;
+    const int share = (sh.k_blocks + s - 1) / s;
+    const double mma = 0.4 * kAccs * 4 * std::max(42, sh.tokens_pad / 2);
+    const double cycles = waves * share * (5.1 * kAccs * block + 2.0 * sh.tokens_pad + mma) + (s > 1 ? 700.0 : 0.0) +
+                          3000.0 * (waves - 1);
+    if (best < 0.0 || cycles < best) {
+      best = cycles;
       parts = s;
       sh.block = block;
     }
@@ -179,17 +181,17 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* ou
   sh.block_pad = (sh.block + 7) / 8 * 8;
   const int sub = rows_sub_bytes(sh, kGate);
   const int share = (sh.k_blocks + parts - 1) / parts;
-  sh.k_sub = std::max(1, std::min({16 * 1024 / sub, 8, share}));
+  // 48 KB a stage (16 KB: 10-30 % slower, each stage costs its commit) in a
+  // ring of 200 KB (94 KB, beside the next launch's: 4-8 % slower).
+  constexpr int kStageTarget = 48 * 1024, kRing = 200 * 1024;
+  sh.k_sub = std::min(share, std::max(1, kStageTarget / sub));
   const int stage = sub * sh.k_sub;
-  const int ring = 3 * stage <= kRowsPairRing ? kRowsPairRing : kRowsSoloRing;
-  sh.stages = std::min({ring / stage, kRowsMaxStages, (share + sh.k_sub - 1) / sh.k_sub});
+  sh.stages = std::min({kRing / stage, kRowsMaxStages, (share + sh.k_sub - 1) / sh.k_sub});
   sh.tail = (int)round_up(std::max(0, (128 - sh.block_pad - sh.tokens_pad) * 128), 1024);
   // Tokens of a reduction round: what the stages hold in fp32.
-  sh.chunk = std::min(sh.tokens_pad, (sh.stages * stage + sh.tail) / (kAccs * 512) / 16 * 16);
-  if (parts > 1 && sh.chunk < 16) {
-    sh.tail += 16 * kAccs * 512;
-    sh.chunk = 16;
-  }
+  constexpr int kTokenBytes = kAccs * 128 * 4;
+  if (sh.stages * stage + sh.tail < 16 * kTokenBytes) sh.tail = 16 * kTokenBytes;
+  sh.chunk = std::min(sh.tokens_pad, (sh.stages * stage + sh.tail) / kTokenBytes / 16 * 16);
   const int smem = sh.stages * stage + sh.tail + kRowsBarBytes + 1024;
   if (smem > kRowsMaxSmem) return B200_ERR_CUDA;
   CUtensorMap tw, tx;
@@ -282,8 +284,7 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   const bool bf16 = dtype == B200_DTYPE_BF16;
   uint16_t* a = static_cast<uint16_t*>(workspace);
   const GateShape s{(int)rows, (int)hidden, (int)dim};
-  const bool few = rows <= rows_limit();
-  if (few && !gate_up) {
+  if (few_rows(rows, dim, hidden) && !gate_up) {
     const int rc = (bf16 ? launch_rows<true, true> : launch_rows<false, true>)(
         x, ldx, w_in, ldw_in, a, hidden, (int)rows, (int)hidden, (int)dim, activation, false, dev, stream);
     if (rc) return rc;

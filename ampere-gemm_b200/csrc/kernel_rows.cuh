@@ -11,8 +11,7 @@
 // of it, by every cluster) by S; the S parts are added up through distributed
 // shared memory in a fixed order.
 //
-//   warp 0      TMA producer; warp 1 MMA issuer; warps 2..5 epilogue, thread =
-//               row of w, so a store instruction writes 32 neighbours of one t.
+//   warp 0      TMA producer; warp 1 MMA issuer; warps 2..5 epilogue.
 //
 // Launched with programmatic stream serialisation.  With `w_early`, w was not
 // written by the kernel before this one on the stream: the first stages of w
@@ -26,6 +25,7 @@ namespace b200 {
 
 constexpr int kRowsMaxTokens = 256;  // N of one MMA
 constexpr int kRowsMaxStages = 16;
+constexpr int kRowsMaxParts = 8;     // CTAs of a cluster
 
 struct RowsShape {
   int tokens;      // rows of x
@@ -66,15 +66,65 @@ __device__ __forceinline__ void tmem_ld_wait_regs16(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// One lane of a converged warp, as a predicate word for the forms below.  The
+// whole warp runs the producer's and the issuer's loops and only the elected
+// lane's instruction takes effect: with warp-uniform operands a
+// tcgen05.mma.cta_group::1 of N = 16 is issued every 42 cycles, its commit
+// costs 150; from a branch that one lane takes they are 71 and 210 (measured).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p;
+}
+
+__device__ __forceinline__ void umma_f16_cta1_if(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_commit_cta1_if(uint32_t elected, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(elected)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d_if(uint32_t elected, uint32_t dst, const void* tmap, uint32_t bar,
+                                               int32_t x, int32_t y, uint64_t cache_hint) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;\n\t}" ::"r"(dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y), "l"(cache_hint), "r"(elected)
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx_if(uint32_t elected, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b64 st;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(elected)
+      : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_nctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
 
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
   return v;
 }
 
@@ -108,6 +158,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * sh.k_blocks / parts);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * sh.k_blocks / parts);
   const int num_stages = (kb1 - kb0 + sh.k_sub - 1) / sh.k_sub;
+  // Every cluster reads all of x.  Clusters start at different places of K and
+  // wrap around: in step, they would all ask one L2 slice for the same line.
+  const int start = static_cast<int>(static_cast<int64_t>(blockIdx.x) / parts * num_stages / (gridDim.x / parts));
+  auto k_stage = [&](int it) { return it + start < num_stages ? it + start : it + start - num_stages; };
+  auto subs = [&](int it) { return min(sh.k_sub, kb1 - kb0 - k_stage(it) * sh.k_sub); };
   uint32_t tmem_cols = 32;
   while (tmem_cols < static_cast<uint32_t>(kAccs * sh.tokens_pad)) tmem_cols *= 2;
 
@@ -132,95 +187,100 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem_base = *tmem_base_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      const uint64_t pol_w = policy_evict_first();   // read once
-      const uint64_t pol_x = policy_evict_last();    // read by every cluster
-      auto subs = [&](int it) { return min(sh.k_sub, kb1 - kb0 - it * sh.k_sub); };
-      auto load_w = [&](int it, int stage) {
-        const int n_sub = subs(it);
-        mbar_arrive_expect_tx(&full_bar[stage],
-                              static_cast<uint32_t>(n_sub * (kAccs * sh.block + sh.tokens_pad) * 128));
-        for (int j = 0; j < n_sub; ++j) {
-          uint8_t* dst = smem + stage * stage_bytes + j * sub_bytes;
-          const int k = (kb0 + it * sh.k_sub + j) * kBK;
-          tma_load_2d(dst, &tmap_w, &full_bar[stage], k, n0, pol_w);
-          if (kGate) tma_load_2d(dst + sh.block_pad * 128, &tmap_w, &full_bar[stage], k, sh.n + n0, pol_w);
-        }
-      };
-      auto load_x = [&](int it, int stage) {
-        const int n_sub = subs(it);
-        for (int j = 0; j < n_sub; ++j)
-          tma_load_2d(smem + stage * stage_bytes + j * sub_bytes + kAccs * sh.block_pad * 128, &tmap_x,
-                      &full_bar[stage], (kb0 + it * sh.k_sub + j) * kBK, 0, pol_x);
-      };
-      const int first = min(num_stages, sh.stages);
-      if (sh.w_early)
-        for (int it = 0; it < first; ++it) load_w(it, it);
-      griddep_wait();
-      griddep_launch_dependents();
-      for (int it = 0; it < first; ++it) {
-        if (!sh.w_early) load_w(it, it);
-        load_x(it, it);
+    const uint32_t el = elect_lane();
+    const uint64_t pol_w = policy_evict_first();  // read once
+    const uint64_t pol_x = policy_evict_last();   // read by every cluster
+    const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full_bar);
+    const uint32_t sub_tx = static_cast<uint32_t>((kAccs * sh.block + sh.tokens_pad) * 128);
+    auto load_w = [&](int it, int stage) {
+      const int n_sub = subs(it);
+      const uint32_t bar = full0 + stage * 8;
+      uint32_t dst = smem0 + stage * stage_bytes;
+      int k = (kb0 + k_stage(it) * sh.k_sub) * kBK;
+      mbar_expect_tx_if(el, bar, static_cast<uint32_t>(n_sub) * sub_tx);
+      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) {
+        tma_load_2d_if(el, dst, &tmap_w, bar, k, n0, pol_w);
+        if (kGate) tma_load_2d_if(el, dst + sh.block_pad * 128, &tmap_w, bar, k, sh.n + n0, pol_w);
       }
-      int issued = first;
-      for (int it = first; it < num_stages; ++it) {
-        const int stage = it % sh.stages;
-        if (!mbar_wait(&empty_bar[stage], static_cast<uint32_t>(it / sh.stages - 1) & 1u, kDevTimeoutProducer)) {
-          ok = false;
-          break;
-        }
-        load_w(it, stage);
-        load_x(it, stage);
-        ++issued;
-      }
-      if (!ok) {
-        // Let every load still in flight land before the CTA leaves.
-        for (int it = max(0, issued - sh.stages); it < issued; ++it)
-          mbar_wait_drain(&full_bar[it % sh.stages], static_cast<uint32_t>(it / sh.stages) & 1u);
-      }
+    };
+    auto load_x = [&](int it, int stage) {
+      const int n_sub = subs(it);
+      const uint32_t bar = full0 + stage * 8;
+      uint32_t dst = smem0 + stage * stage_bytes + kAccs * sh.block_pad * 128;
+      int k = (kb0 + k_stage(it) * sh.k_sub) * kBK;
+      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) tma_load_2d_if(el, dst, &tmap_x, bar, k, 0, pol_x);
+    };
+    const int first = min(num_stages, sh.stages);
+    if (sh.w_early)
+      for (int it = 0; it < first; ++it) load_w(it, it);
+    griddep_wait();
+    griddep_launch_dependents();
+    for (int it = 0; it < first; ++it) {
+      if (!sh.w_early) load_w(it, it);
+      load_x(it, it);
+    }
+    int issued = first, stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int it = first; it < num_stages; ++it) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase, kDevTimeoutProducer));
+      if (!ok) break;
+      load_w(it, stage);
+      load_x(it, stage);
+      ++issued;
+      if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
+    }
+    if (!ok && lane == 0) {
+      // Let every load still in flight land before the CTA leaves.
+      for (int it = max(0, issued - sh.stages); it < issued; ++it)
+        mbar_wait_drain(&full_bar[it % sh.stages], static_cast<uint32_t>(it / sh.stages) & 1u);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc =
-          make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad), Major::kK, Major::kK, kBf16);
-      const uint32_t base = smem_u32(smem);
-      bool ok = true;
-      for (int it = 0; it < num_stages; ++it) {
-        const int stage = it % sh.stages;
-        ok = mbar_wait(&full_bar[stage], static_cast<uint32_t>(it / sh.stages) & 1u, kDevTimeoutMma);
-        if (!ok) break;
-        tc_fence_after_sync();
-        const int n_sub = min(sh.k_sub, kb1 - kb0 - it * sh.k_sub);
-        for (int j = 0; j < n_sub; ++j) {
-          const uint32_t w_addr = base + stage * stage_bytes + j * sub_bytes;
-          const uint32_t x_addr = w_addr + kAccs * sh.block_pad * 128;
+    const uint32_t el = elect_lane();
+    const uint32_t idesc = make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad), Major::kK, Major::kK, kBf16);
+    // Descriptors advance by adding to their address field (units of 16 bytes;
+    // addresses stay below 2^18).
+    const uint64_t w_desc0 = make_desc_kmajor_sw128(smem_u32(smem));
+    const uint64_t up_off = static_cast<uint64_t>(sh.block_pad * 128) >> 4;
+    const uint64_t x_off = static_cast<uint64_t>(kAccs * sh.block_pad * 128) >> 4;
+    const uint64_t sub_off = static_cast<uint64_t>(sub_bytes) >> 4;
+    const uint32_t d_up = tmem_base + sh.tokens_pad;
+    uint32_t acc = 0;
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int it = 0; it < num_stages; ++it) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, kDevTimeoutMma));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const int n_sub = subs(it);
+      uint64_t wd = w_desc0 + (static_cast<uint64_t>(stage * stage_bytes) >> 4);
+      for (int j = 0; j < n_sub; ++j, wd += sub_off) {
 #pragma unroll
-          for (int k = 0; k < kBK / kUmmaK; ++k) {
-            const uint64_t xd = make_desc_kmajor_sw128(x_addr + k * (kUmmaK * 2));
-            const uint32_t acc = (it | j | k) != 0 ? 1u : 0u;
-            umma_f16_cta1(tmem_base, make_desc_kmajor_sw128(w_addr + k * (kUmmaK * 2)), xd, idesc, acc);
-            if (kGate)
-              umma_f16_cta1(tmem_base + sh.tokens_pad,
-                            make_desc_kmajor_sw128(w_addr + sh.block_pad * 128 + k * (kUmmaK * 2)), xd, idesc, acc);
-          }
+        for (int k = 0; k < kBK / kUmmaK; ++k) {
+          const uint64_t step = static_cast<uint64_t>(k * (kUmmaK * 2)) >> 4;
+          umma_f16_cta1_if(el, tmem_base, wd + step, wd + (x_off + step), idesc, acc);
+          if (kGate) umma_f16_cta1_if(el, d_up, wd + (up_off + step), wd + (x_off + step), idesc, acc);
+          acc = 1;
         }
-        umma_commit_cta1(&empty_bar[stage]);
       }
-      if (ok) {
-        umma_commit_cta1(done_bar);
-      } else {
-        umma_commit_cta1(drain_bar);
-        mbar_wait_drain(drain_bar, 0);
-      }
+      umma_commit_cta1_if(el, &empty_bar[stage]);
+      if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
+    }
+    if (ok) {
+      umma_commit_cta1_if(el, done_bar);
+    } else {
+      umma_commit_cta1_if(el, drain_bar);
+      if (lane == 0) mbar_wait_drain(drain_bar, 0);
     }
   }
   __syncwarp();
 
-  // ---- epilogue: warps 2..5, thread = lane `row` of the accumulators ----
-  const int row = (warp & 3) * 32 + lane;
-  const int n = n0 + row;
-  const bool mine = warp >= 2 && row < sh.block && n < sh.n;
+  // ---- epilogue: warps 2..5 ----
+  // Rounds of `chunk` tokens: each CTA stages its accumulators in the idle
+  // pipeline stages ([accumulator][token][row of w], fp32), then takes every
+  // S-th token, adds up the S parts and stores.  An item is one token's next
+  // four rows of w; items are dealt to all 128 threads, whatever `block` is.
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
   bool got = true;
   if (warp >= 2) {
@@ -228,60 +288,60 @@ __global__ void __launch_bounds__(kThreads, 2)
     got = __shfl_sync(0xffffffffu, got, 0);
     tc_fence_after_sync();
   }
-  if (parts == 1) {
+  float* part = reinterpret_cast<float*>(smem);
+  const int quads = (min(sh.block, sh.n - n0) + 3) >> 2;
+  for (int c0 = 0; c0 < sh.tokens; c0 += sh.chunk) {
+    const int c1 = min(sh.tokens_pad, c0 + sh.chunk);
+    const int row = (warp & 3) * 32 + lane;
+    if (warp >= 2 && (warp & 3) * 32 < sh.block) {
+      for (int t0 = c0; t0 < c1; t0 += 16) {
+#pragma unroll
+        for (int a = 0; a < kAccs; ++a) {
+          uint32_t g[16];
+          tmem_ld_32x32b_x16(t_row + a * sh.tokens_pad + t0, g);
+          tmem_ld_wait_regs16(g);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) part[(a * sh.chunk + t0 - c0 + e) * 128 + row] = __uint_as_float(g[e]);
+        }
+      }
+    }
+    cluster_sync();
     if (warp >= 2 && got) {
-      for (int t0 = 0; t0 < sh.tokens; t0 += 16) {
-        uint32_t g[16], u[16];
-        tmem_ld_32x32b_x16(t_row + t0, g);
-        if (kGate) tmem_ld_32x32b_x16(t_row + sh.tokens_pad + t0, u);
-        tmem_ld_wait_regs16(g);
-        if (kGate) tmem_ld_wait_regs16(u);
+      const int tokens = (min(c1, sh.tokens) - c0 - rank + parts - 1) / parts;  // of this CTA (0 or less: none)
+      for (int i = threadIdx.x - 64; i < tokens * quads; i += kEpiWarps * 32) {
+        const int q = i % quads, t = c0 + rank + parts * (i / quads);
+        float4 v[kAccs][kRowsMaxParts];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float v = __uint_as_float(g[e]);
-          if (kGate) v = gate_value(sh.activation, v, __uint_as_float(u[e]));
-          if (mine && t0 + e < sh.tokens)
-            out[static_cast<int64_t>(t0 + e) * ld_out + n] =
-                static_cast<uint16_t>(pack_16bit_rn<kBf16>(__float_as_uint(v), 0u));
+        for (int a = 0; a < kAccs; ++a) {
+          const uint32_t at = smem_u32(part + (a * sh.chunk + t - c0) * 128 + 4 * q);
+#pragma unroll
+          for (int p = 0; p < kRowsMaxParts; ++p)
+            v[a][p] = p < parts ? ld_shared_cluster_v4(mapa_shared(at, p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float4 r[kAccs];
+#pragma unroll
+        for (int a = 0; a < kAccs; ++a) {
+          r[a] = v[a][0];
+#pragma unroll
+          for (int p = 1; p < kRowsMaxParts; ++p) {
+            r[a].x += v[a][p].x;
+            r[a].y += v[a][p].y;
+            r[a].z += v[a][p].z;
+            r[a].w += v[a][p].w;
+          }
+        }
+        const float g[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+        const float u[4] = {r[kAccs - 1].x, r[kAccs - 1].y, r[kAccs - 1].z, r[kAccs - 1].w};
+        uint16_t* o = out + static_cast<int64_t>(t) * ld_out + n0 + 4 * q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = kGate ? gate_value(sh.activation, g[e], u[e]) : g[e];
+          if (4 * q + e < sh.block && n0 + 4 * q + e < sh.n)
+            o[e] = static_cast<uint16_t>(pack_16bit_rn<kBf16>(__float_as_uint(y), 0u));
         }
       }
     }
-  } else {
-    // Each round stages `chunk` tokens of the parts in the idle pipeline
-    // stages ([accumulator][token][row]) and adds up every S-th of them.
-    float* part = reinterpret_cast<float*>(smem);
-    for (int c0 = 0; c0 < sh.tokens; c0 += sh.chunk) {
-      const int c1 = min(sh.tokens_pad, c0 + sh.chunk);
-      if (warp >= 2) {
-        for (int t0 = c0; t0 < c1; t0 += 16) {
-#pragma unroll
-          for (int a = 0; a < kAccs; ++a) {
-            uint32_t g[16];
-            tmem_ld_32x32b_x16(t_row + a * sh.tokens_pad + t0, g);
-            tmem_ld_wait_regs16(g);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              part[(a * sh.chunk + t0 - c0 + e) * 128 + row] = __uint_as_float(g[e]);
-          }
-        }
-      }
-      cluster_sync();
-      if (mine && got) {
-        for (int t = c0 + rank; t < min(c1, sh.tokens); t += parts) {
-          float v[kAccs];
-#pragma unroll
-          for (int a = 0; a < kAccs; ++a) {
-            const uint32_t at = smem_u32(part + (a * sh.chunk + t - c0) * 128 + row);
-            v[a] = 0.0f;
-            for (int p = 0; p < parts; ++p) v[a] += ld_shared_cluster_f32(mapa_shared(at, p));
-          }
-          const float r = kGate ? gate_value(sh.activation, v[0], v[kAccs - 1]) : v[0];
-          out[static_cast<int64_t>(t) * ld_out + n] =
-              static_cast<uint16_t>(pack_16bit_rn<kBf16>(__float_as_uint(r), 0u));
-        }
-      }
-      cluster_sync();
-    }
+    cluster_sync();
   }
 
   tc_fence_before_sync();
