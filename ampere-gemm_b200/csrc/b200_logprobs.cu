@@ -220,7 +220,11 @@ __global__ void __launch_bounds__(kThreads)
       for (int p = 0; p < kPacks; ++p) {
         const Pack<T, kV> q = load_pack<T, kV>(x + span.head_end + g * kGroup + p * kV);
 #pragma unroll
-        for (int e = 0; e < kV; ++e) v[p * kV + e] = to_f32(q.v[e]);
+        for (int e = 0; e < kV / 2; ++e) {
+          const float2 f = q.pair(e);
+          v[p * kV + 2 * e] = f.x;
+          v[p * kV + 2 * e + 1] = f.y;
+        }
       }
       float mx = v[0];
 #pragma unroll
@@ -347,12 +351,11 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // gl ([j == t] - p) - gh p (ln p + entropy)
-template <typename T>
-__device__ __forceinline__ T grad_of(float x, float2 st, float ent, float gl, float gh, bool is_target) {
+__device__ __forceinline__ float grad_of(float x, float2 st, float ent, float gl, float gh, bool is_target) {
   const float d = (x - st.x) - st.y;
   const float p = exp2_approx(d * kLog2e);
   const float g = -p * fmaf(gh, fmaxf(d, -1.0e4f) + ent, gl);
-  return from_f32<T>(is_target ? g + gl : g);
+  return is_target ? g + gl : g;
 }
 
 template <typename T>
@@ -384,21 +387,26 @@ __global__ void __launch_bounds__(kThreads)
     const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
     if (!same) {
       for (int64_t j = lo + tid; j < hi; j += kThreads)
-        d[j] = grad_of<T>(to_f32(x[j]), lse, ent, gl, gh, j == target);
+        d[j] = from_f32<T>(grad_of(to_f32(x[j]), lse, ent, gl, gh, j == target));
       continue;
     }
     if (lo + tid < span.head_end)
-      d[lo + tid] = grad_of<T>(to_f32(x[lo + tid]), lse, ent, gl, gh, lo + tid == target);
+      d[lo + tid] = from_f32<T>(grad_of(to_f32(x[lo + tid]), lse, ent, gl, gh, lo + tid == target));
     for (int64_t j = span.head_end + tid * kV; j < span.body_end; j += kThreads * kV) {
       const Pack<T, kV> q = load_pack<T, kV>(x + j);
       Pack<T, kV> o;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) o.v[e] = grad_of<T>(to_f32(q.v[e]), lse, ent, gl, gh, j + e == target);
+      for (int e = 0; e < kV / 2; ++e) {
+        const float2 f = q.pair(e);
+        o.set_pair(e, make_float2(grad_of(f.x, lse, ent, gl, gh, j + 2 * e == target),
+                                  grad_of(f.y, lse, ent, gl, gh, j + 2 * e + 1 == target)));
+      }
       store_pack<T, kV>(d + j, o);
     }
     if (span.body_end + tid < hi)
       d[span.body_end + tid] =
-          grad_of<T>(to_f32(x[span.body_end + tid]), lse, ent, gl, gh, span.body_end + tid == target);
+          from_f32<T>(
+          grad_of(to_f32(x[span.body_end + tid]), lse, ent, gl, gh, span.body_end + tid == target));
   }
 }
 

@@ -32,81 +32,172 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sum over the threads of one row.  A row is one warp (each warp of the block
-// has its own), or the whole block; `red` is then 32 floats that no thread
-// still reads from the sum before the last.
-__device__ __forceinline__ float row_sum(float v, bool one_warp, float* red) {
-  v = warp_sum(v);
-  if (one_warp) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  return warp_sum(lane < warps ? red[lane] : 0.0f);
+// Sum over the `width` lanes (8, 16 or 32, aligned) that share a row.
+__device__ __forceinline__ float lanes_sum(float v, int width) {
+  if (width == 32) return warp_sum(v);
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 2);
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  if (width == 16) v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v;
 }
 
-// Forward.  blockDim = (threads of a row, rows of a block); a thread holds NV
-// packs of VEC elements, pack j at (j * blockDim.x + threadIdx.x) * VEC.
-template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kMaxRowThreads)
+// red[0] + ... + red[n - 1], n <= 32, read four at a time by every thread.
+__device__ __forceinline__ float sum_of(const float* red, int n) {
+  float s = 0.0f;
+  for (int i = 0; i < n; i += 4) {
+    const float4 r = *reinterpret_cast<const float4*>(red + i);
+    s += r.x;
+    if (i + 1 < n) s += r.y;
+    if (i + 2 < n) s += r.z;
+    if (i + 3 < n) s += r.w;
+  }
+  return s;
+}
+
+// Sum over the `tpr` threads of one row: lanes of a warp, or the whole block;
+// `red` is then 32 floats that no thread still reads from the sum before the
+// last.
+__device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
+  if (tpr <= 32) return lanes_sum(v, tpr);
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return sum_of(red, tpr >> 5);
+}
+
+// Where a thread's packs of a row lie: pack j at (j * threads of the row +
+// threadIdx.x) * VEC.  With TPR != 0 the row has TPR threads and exactly
+// TPR * NV packs, so offsets are constants and nothing is checked.
+template <int VEC, int TPR>
+struct Columns {
+  int cols;
+  __device__ __forceinline__ int at(int j) const {
+    return (j * (TPR ? TPR : static_cast<int>(blockDim.x)) + static_cast<int>(threadIdx.x)) * VEC;
+  }
+  __device__ __forceinline__ bool has(int j) const { return TPR != 0 || at(j) < cols; }
+};
+
+// A thread's packs of a row; those past its end (or of no row) are zero.
+template <typename T, int VEC, int NV, int TPR>
+__device__ __forceinline__ void load_row(Pack<T, VEC> (&v)[NV], const T* row, const Columns<VEC, TPR>& col,
+                                         bool active) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    v[j] = Pack<T, VEC>{};
+    if (active && col.has(j)) v[j] = load_pack<T, VEC>(row + col.at(j));
+  }
+}
+
+template <typename T, int VEC, int NV, int TPR>
+__device__ __forceinline__ void store_row(T* row, const Pack<T, VEC> (&v)[NV], const Columns<VEC, TPR>& col) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (col.has(j)) store_pack<T, VEC>(row + col.at(j), v[j]);
+}
+
+// 1 / sqrt(v) for v >= 0: the approximate one after a Newton step (within
+// 2^-23 of it); 0 and infinity as they are.
+__device__ __forceinline__ float inverse_sqrt(float v) {
+  const float r = rsqrtf(v);
+  const float s = fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r);
+  return v > 0.0f && v < __builtin_huge_valf() ? s : r;
+}
+
+// fn for each pair of a pack's elements (a single one with 0).
+template <typename T, int VEC, typename Fn>
+__device__ __forceinline__ void for_pairs(const Pack<T, VEC>& p, Fn&& fn) {
+  if constexpr (VEC == 1) {
+    fn(make_float2(to_f32(p.v), 0.0f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) fn(p.pair(i));
+  }
+}
+
+// Asynchronous copy of 16 bytes into shared memory; a thread's copies are
+// counted by its own commit groups.
+__device__ __forceinline__ void copy_async_16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Forward.  blockDim = (threads of a row, rows of a block).  The blocks are
+// resident and loop over rows.
+template <typename T, typename W, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads)
     layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
-                                      T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                                      int64_t rows, int cols, int64_t ldx, int64_t ldy, float eps) {
-  __shared__ float red[2][32];
+                          T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows,
+                          int cols, int64_t ldx, int64_t ldy, float eps) {
+  __shared__ __align__(16) float red[2][32];
   pdl_wait();
-  const bool one_warp = blockDim.x == 32;
+  const Columns<VEC, TPR> col{cols};
+  const int tpr = TPR ? TPR : static_cast<int>(blockDim.x);
   const float inv_n = 1.0f / static_cast<float>(cols);
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < rows; row += step) {
-    const T* xr = x + row * ldx;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const T* xr = x + row * ldx;
+  T* yr = y + row * ldy;
+  // The rows of a block take their turns together: row - threadIdx.y is the same for all.
+  for (; row - threadIdx.y < rows; row += step, xr += step * ldx, yr += step * ldy) {
+    const bool active = row < rows;
     Pack<T, VEC> v[NV];
-    float s = 0.0f;
+    load_row<T, VEC, NV>(v, xr, col, active);
+    float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) v[j] = load_pack<T, VEC>(xr + c);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s += to_f32(v[j].v[e]);
-      }
-    }
-    const float mu = row_sum(s, one_warp, red[0]) * inv_n;
+    for (int j = 0; j < NV; ++j)
+      for_pairs<T, VEC>(v[j], [&](float2 f) { s2 = add2(s2, f); });
+    const float mu = row_sum(s2.x + s2.y, tpr, red[0]) * inv_n;
     // The centred squares are summed in a second pass over the registers:
     // sum(x^2) - n mu^2 would lose the variance of a row with a large mean.
-    float q = 0.0f;
+    const float2 minus_mu = pair_of(-mu);
+    float2 q2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
+      if (col.has(j))
+        for_pairs<T, VEC>(v[j], [&](float2 f) {
+          f = add2(f, minus_mu);
+          if (VEC == 1) f.y = 0.0f;
+          q2 = fma2(f, f, q2);
+        });
+    }
+    const float rstd = inverse_sqrt(row_sum(q2.x + q2.y, tpr, red[1]) * inv_n + eps);
+    const float2 r2 = pair_of(rstd);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = to_f32(v[j].v[e]) - mu;
-          q = fmaf(d, d, q);
+    for (int j = 0; j < NV; ++j) {
+      if (active && col.has(j)) {
+        const int c = col.at(j);
+        if constexpr (VEC == 1) {
+          const float h = (to_f32(v[j].v) - mu) * rstd;
+          yr[c] = from_f32<T>(fmaf(h, w ? to_f32(w[c]) : 1.0f, b ? to_f32(b[c]) : 0.0f));
+        } else {
+          float2 f[VEC / 2];
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) f[i] = mul2(add2(v[j].pair(i), minus_mu), r2);
+          if (w) {
+            const Pack<W, VEC> p = load_pack<W, VEC>(w + c);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) f[i] = mul2(f[i], p.pair(i));
+          }
+          if (b) {
+            const Pack<W, VEC> p = load_pack<W, VEC>(b + c);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) f[i] = add2(f[i], p.pair(i));
+          }
+          Pack<T, VEC> o;
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) o.set_pair(i, f[i]);
+          store_pack<T, VEC>(yr + c, o);
         }
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum(q, one_warp, red[1]) * inv_n + eps);
-    T* yr = y + row * ldy;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
-        Pack<T, VEC> o;
-        Pack<W, VEC> wv, bv;
-        if (w) wv = load_pack<W, VEC>(w + c);
-        if (b) bv = load_pack<W, VEC>(b + c);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = (to_f32(v[j].v[e]) - mu) * rstd;
-          o.v[e] = from_f32<T>(fmaf(h, w ? to_f32(wv.v[e]) : 1.0f, b ? to_f32(bv.v[e]) : 0.0f));
-        }
-        store_pack<T, VEC>(yr + c, o);
-      }
-    }
-    if (threadIdx.x == 0) {
+    if (active && threadIdx.x == 0) {
       if (mean_out) mean_out[row] = mu;
       if (rstd_out) rstd_out[row] = rstd;
     }
@@ -120,20 +211,20 @@ __global__ void __launch_bounds__(kLongThreads) layer_norm_fwd_long_kernel(const
                                            T* __restrict__ y, float* __restrict__ mean_out,
                                            float* __restrict__ rstd_out, int64_t rows, int cols, int64_t ldx,
                                            int64_t ldy, float eps) {
-  __shared__ float red[2][32];
+  __shared__ __align__(16) float red[2][32];
   pdl_wait();
   const float inv_n = 1.0f / static_cast<float>(cols);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
     float s = 0.0f;
     for (int c = threadIdx.x; c < cols; c += blockDim.x) s += to_f32(xr[c]);
-    const float mu = row_sum(s, false, red[0]) * inv_n;
+    const float mu = row_sum(s, blockDim.x, red[0]) * inv_n;
     float q = 0.0f;
     for (int c = threadIdx.x; c < cols; c += blockDim.x) {
       const float d = to_f32(xr[c]) - mu;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.0f / sqrtf(row_sum(q, false, red[1]) * inv_n + eps);
+    const float rstd = inverse_sqrt(row_sum(q, blockDim.x, red[1]) * inv_n + eps);
     for (int c = threadIdx.x; c < cols; c += blockDim.x)
       y[row * ldy + c] = from_f32<T>(
           fmaf((to_f32(xr[c]) - mu) * rstd, w ? to_f32(w[c]) : 1.0f, b ? to_f32(b[c]) : 0.0f));
@@ -144,92 +235,147 @@ __global__ void __launch_bounds__(kLongThreads) layer_norm_fwd_long_kernel(const
   }
 }
 
-// Backward.  Same layout as the forward kernel.  A thread keeps the same
-// columns for all its rows, so it sums their dw and db in registers; a block
-// writes its sums once, as row blockIdx.x of `part` (gridDim.x x 2 x cols:
-// dw, then db), and layer_norm_bwd_reduce_kernel adds those rows up.
-template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(kMaxRowThreads)
+template <int N>
+__device__ __forceinline__ float element(const float2 (&f)[N], int e) {
+  return e & 1 ? f[e / 2].y : f[e / 2].x;
+}
+
+constexpr int kBwdThreads = 512;  // of a block, all its rows together
+// Rows on their way while one is worked on, with NV packs a thread.
+template <int NV>
+constexpr int kAhead = NV <= 2 ? 3 : 1;
+
+// Backward.  Threads and packs as in the forward kernel; with several rows in
+// a block, each row's threads are whole warps with their own barrier, or lanes
+// of a warp.  A thread keeps the same columns for all its rows, so it sums
+// their dw and db in registers; a block writes its sums once, as row
+// blockIdx.x of `part` (gridDim.x x 2 x cols: dw, then db), and
+// layer_norm_bwd_reduce_kernel adds those rows up.  With 16-byte packs, rows
+// arrive through a ring in shared memory in which every thread reads only what
+// it requested itself: no barrier, and no registers for rows on their way.
+template <typename T, typename W, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR == 320 ? TPR : kBwdThreads, TPR == 320 ? 2 : 1)
     layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
-                                      const float* __restrict__ mean, const float* __restrict__ rstd_in,
-                                      T* __restrict__ dx, float* __restrict__ part, int64_t rows, int cols,
-                                      int64_t lddy, int64_t ldx, int64_t lddx) {
-  __shared__ float red[2][2][32];
-  extern __shared__ float col_sum[];  // [2][cols], blocks of more than one row
+                          const float* __restrict__ mean, const float* __restrict__ rstd_in, T* __restrict__ dx,
+                          float* __restrict__ part, int64_t rows, int cols, int64_t lddy, int64_t ldx, int64_t lddx) {
+  constexpr bool kAsync = VEC * sizeof(T) == 16;
+  constexpr int kSlots = kAhead<NV> + 1;
+  __shared__ float2 red[2][kBwdThreads / 32];
+  extern __shared__ __align__(16) uint8_t dyn[];  // the ring; after the loop the block's column sums
   pdl_wait();
-  const bool one_warp = blockDim.x == 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const Columns<VEC, TPR> col{cols};
+  const int tpr = TPR ? TPR : static_cast<int>(blockDim.x);
+  const int tid = threadIdx.y * tpr + threadIdx.x;
+  const int threads = tpr * blockDim.y;
+  const int warps = tpr >> 5;  // of a row
   const float inv_n = 1.0f / static_cast<float>(cols);
-  float dw[NV][VEC], db[NV][VEC];
+  constexpr int kPairs = VEC * NV / 2;
+  float2 dw[kPairs], db[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) dw[i] = db[i] = make_float2(0.0f, 0.0f);
   Pack<W, VEC> wv[NV];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * VEC;
-    if (w && c < cols) wv[j] = load_pack<W, VEC>(w + c);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[j][e] = db[j][e] = 0.0f;
-  }
-  int parity = 0;
+  if (w) load_row<W, VEC, NV>(wv, w, col, true);
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < rows; row += step) {
-    const T* xr = x + row * ldx;
-    const T* gr = dy + row * lddy;
-    Pack<T, VEC> xv[NV], gv[NV];
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(dyn) + tid;  // [slot][x, dy][j][thread]
+  int64_t next = row0;  // the row requested next
+  const T* xn = x + next * ldx;
+  const T* gn = dy + next * lddy;
+  auto request = [&](int slot) {
+    if (next < rows) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
-        xv[j] = load_pack<T, VEC>(xr + c);
-        gv[j] = load_pack<T, VEC>(gr + c);
-      }
-    }
-    const float mu = mean[row], rstd = rstd_in[row];
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float g = to_f32(gv[j].v[e]);
-          const float h = (to_f32(xv[j].v[e]) - mu) * rstd;
-          const float q = g * (w ? to_f32(wv[j].v[e]) : 1.0f);
-          s1 += q;
-          s2 = fmaf(q, h, s2);
-          dw[j][e] = fmaf(g, h, dw[j][e]);
-          db[j][e] += g;
+      for (int j = 0; j < NV; ++j) {
+        if (col.has(j)) {
+          copy_async_16(ring + ((slot * 2 + 0) * NV + j) * threads, xn + col.at(j));
+          copy_async_16(ring + ((slot * 2 + 1) * NV + j) * threads, gn + col.at(j));
         }
       }
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (!one_warp) {
-      // Two buffers in turn: one barrier a row is enough.
-      if (lane == 0) {
-        red[parity][0][warp] = s1;
-        red[parity][1][warp] = s2;
+    copy_async_commit();
+    next += step;
+    xn += step * ldx;
+    gn += step * lddy;
+  };
+  if (kAsync) {
+#pragma unroll
+    for (int i = 0; i < kAhead<NV>; ++i) request(i);
+  }
+  int parity = 0, slot = 0;
+  float next_mu = row0 < rows ? mean[row0] : 0.0f, next_rstd = row0 < rows ? rstd_in[row0] : 0.0f;
+  T* dr = dx + row0 * lddx;
+  for (int64_t row = row0; row - threadIdx.y < rows; row += step, dr += step * lddx) {
+    const bool active = row < rows;
+    Pack<T, VEC> xv[NV], gv[NV];
+    if (kAsync) {
+      request(slot == 0 ? kSlots - 1 : slot - 1);
+      copy_async_wait<kAhead<NV>>();
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xv[j] = gv[j] = Pack<T, VEC>{};
+        if (active && col.has(j)) {
+          xv[j] = ring[((slot * 2 + 0) * NV + j) * threads];
+          gv[j] = ring[((slot * 2 + 1) * NV + j) * threads];
+        }
       }
-      __syncthreads();
-      s1 = warp_sum(lane < warps ? red[parity][0][lane] : 0.0f);
-      s2 = warp_sum(lane < warps ? red[parity][1][lane] : 0.0f);
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
+    } else {
+      load_row<T, VEC, NV>(xv, x + row * ldx, col, active);
+      load_row<T, VEC, NV>(gv, dy + row * lddy, col, active);
+    }
+    const float mu = next_mu, rstd = next_rstd;
+    if (row + step < rows) {
+      next_mu = mean[row + step];
+      next_rstd = rstd_in[row + step];
+    }
+    // h and q; elements past the end have x = dy = 0, so all they add is 0.
+    float2 h[kPairs], q[kPairs], acc1 = make_float2(0.0f, 0.0f), acc2 = acc1;
+    unpack<T, VEC, NV>(xv, h);
+    unpack<T, VEC, NV>(gv, q);
+    const float2 minus_mu = pair_of(-mu), r2 = pair_of(rstd);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      h[i] = mul2(add2(h[i], minus_mu), r2);
+      dw[i] = fma2(q[i], h[i], dw[i]);
+      db[i] = add2(db[i], q[i]);
+    }
+    if (w) {
+      float2 c2[kPairs];
+      unpack<W, VEC, NV>(wv, c2);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) q[i] = mul2(q[i], c2[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      acc1 = add2(acc1, q[i]);
+      acc2 = fma2(q[i], h[i], acc2);
+    }
+    float s1 = acc1.x + acc1.y, s2 = acc2.x + acc2.y;
+    if (tpr <= 32) {
+      s1 = lanes_sum(s1, tpr);
+      s2 = lanes_sum(s2, tpr);
+    } else {
+      // Two buffers in turn: one barrier a row is enough.
+      s1 = warp_sum(s1);
+      s2 = warp_sum(s2);
+      if ((tid & 31) == 0) red[parity][tid >> 5] = make_float2(s1, s2);
+      if (blockDim.y == 1)
+        __syncthreads();
+      else
+        asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(tpr) : "memory");
+      s1 = s2 = 0.0f;
+      const float2* r = red[parity] + threadIdx.y * warps;
+      for (int i = 0; i < warps; ++i) {
+        s1 += r[i].x;
+        s2 += r[i].y;
+      }
       parity ^= 1;
     }
-    s1 *= inv_n;
-    s2 *= inv_n;
-    T* dr = dx + row * lddx;
+    if (active) {
+      const float2 m1 = pair_of(-s1 * inv_n), m2 = pair_of(-s2 * inv_n);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * VEC;
-      if (c < cols) {
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = (to_f32(xv[j].v[e]) - mu) * rstd;
-          const float q = to_f32(gv[j].v[e]) * (w ? to_f32(wv[j].v[e]) : 1.0f);
-          o.v[e] = from_f32<T>(rstd * (q - s1 - h * s2));
-        }
-        store_pack<T, VEC>(dr + c, o);
-      }
+      for (int i = 0; i < kPairs; ++i) q[i] = mul2(fma2(h[i], m2, add2(q[i], m1)), r2);
+      repack<T, VEC, NV>(q, xv);
+      store_row<T, VEC, NV>(dr, xv, col);
     }
   }
   if (!part) return;
@@ -241,14 +387,16 @@ __global__ void __launch_bounds__(kMaxRowThreads)
       if (c < cols) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          out[c + e] = dw[j][e];
-          out[cols + c + e] = db[j][e];
+          out[c + e] = element(dw, j * VEC + e);
+          out[cols + c + e] = element(db, j * VEC + e);
         }
       }
     }
     return;
   }
   // The block's rows are added up in shared memory, in order.
+  float* col_sum = reinterpret_cast<float*>(dyn);  // [2][cols]
+  __syncthreads();
   for (int yy = 0; yy < static_cast<int>(blockDim.y); ++yy) {
     if (threadIdx.y == yy) {
 #pragma unroll
@@ -257,15 +405,15 @@ __global__ void __launch_bounds__(kMaxRowThreads)
         if (c < cols) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            col_sum[c + e] = dw[j][e] + (yy ? col_sum[c + e] : 0.0f);
-            col_sum[cols + c + e] = db[j][e] + (yy ? col_sum[cols + c + e] : 0.0f);
+            col_sum[c + e] = element(dw, j * VEC + e) + (yy ? col_sum[c + e] : 0.0f);
+            col_sum[cols + c + e] = element(db, j * VEC + e) + (yy ? col_sum[cols + c + e] : 0.0f);
           }
         }
       }
     }
     __syncthreads();
   }
-  for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * cols; c += blockDim.x * blockDim.y) out[c] = col_sum[c];
+  for (int c = tid; c < 2 * cols; c += threads) out[c] = col_sum[c];
 }
 
 // dx for rows longer than a block's registers hold: one block a row.
@@ -274,7 +422,7 @@ __global__ void __launch_bounds__(kLongThreads) layer_norm_bwd_long_kernel(const
                                            const float* __restrict__ mean, const float* __restrict__ rstd_in,
                                            T* __restrict__ dx, int64_t rows, int cols, int64_t lddy, int64_t ldx,
                                            int64_t lddx) {
-  __shared__ float red[2][32];
+  __shared__ __align__(16) float red[2][32];
   pdl_wait();
   const float inv_n = 1.0f / static_cast<float>(cols);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -287,8 +435,8 @@ __global__ void __launch_bounds__(kLongThreads) layer_norm_bwd_long_kernel(const
       s1 += q;
       s2 = fmaf(q, (to_f32(xr[c]) - mu) * rstd, s2);
     }
-    s1 = row_sum(s1, false, red[0]) * inv_n;
-    s2 = row_sum(s2, false, red[1]) * inv_n;
+    s1 = row_sum(s1, blockDim.x, red[0]) * inv_n;
+    s2 = row_sum(s2, blockDim.x, red[1]) * inv_n;
     for (int c = threadIdx.x; c < cols; c += blockDim.x) {
       const float q = to_f32(gr[c]) * (w ? to_f32(w[c]) : 1.0f);
       dx[row * lddx + c] = from_f32<T>(rstd * (q - s1 - (to_f32(xr[c]) - mu) * rstd * s2));
@@ -338,39 +486,119 @@ __global__ void layer_norm_bwd_reduce_kernel(const float* __restrict__ part, int
   }
 }
 
-struct RowPlan {
-  int nv;       // packs a thread holds (0: the row does not fit a block's registers)
-  int threads;  // threads of a row
-  int rows;     // rows of a block
-};
-
-int round32(int v) { return (v + 31) / 32 * 32; }
-
-// Threads and packs of a row of `packs` packs, at most `max_nv` packs a thread.
-// Rows that one warp holds go four to a block; longer ones take a block each
-// with as few packs a thread as `threads_wanted` threads allow.
-RowPlan plan_rows(int packs, int max_nv, int threads_wanted) {
-  for (int nv = 1; nv <= max_nv; nv *= 2) {
-    const int t = round32((packs + nv - 1) / nv);
-    if (t <= threads_wanted || (nv == max_nv && t <= kMaxRowThreads)) return RowPlan{nv, t, t == 32 ? 4 : 1};
-  }
-  return RowPlan{0, 0, 1};
-}
-
-constexpr int kFwdMaxNv = 8;
-// Columns a thread sums dw and db of, in packs: two registers each, beside the
-// packs of x, dy and w.
-template <int VEC>
-constexpr int kBwdMaxNv = VEC == 1 ? 16 : 4;
-
 template <int V>
 using IntC = std::integral_constant<int, V>;
+
+struct RowPlan {
+  int nv = 0;       // packs a thread holds (0: the row does not fit a block's registers)
+  int threads = 0;  // threads of a row
+  int rows = 1;     // rows of a block
+};
+
+// Threads of a row with `nv` packs a thread: 8 or 16 lanes, or whole warps.
+int row_threads(int packs, int nv) {
+  const int t = (packs + nv - 1) / nv;
+  return t <= 8 ? 8 : t <= 16 ? 16 : (t + 31) / 32 * 32;
+}
+
+// Packs a thread holds, for which kernels are built.  A 16-byte pack; a pair of
+// 16-bit elements, where rows start on 4 bytes only; or one element.
+constexpr int kFwdNv[] = {1, 2, 3, 4, 8, 16};
+constexpr int kBwdNv[] = {1, 2, 4, 8, 16};
+template <int VEC>
+constexpr bool fwd_built(int nv) {
+  return nv <= (VEC >= 4 ? 8 : 16) && (nv != 3 || VEC == 8);
+}
+// Two registers a column for dw and db beside the packs of x, dy and w.
+template <int VEC>
+constexpr bool bwd_built(int nv) {
+  return VEC == 8 ? nv <= 4 : VEC == 4 ? nv == 2 || nv == 4 : VEC == 2 ? nv == 4 || nv == 8 : nv == 8 || nv == 16;
+}
+
+// Threads of a row for which kernels are built that the row fills exactly, with
+// constant offsets and no checks: those bound this kernel otherwise (16384 x
+// 4096 bf16 with fp32 weights: forward 58 us against 69, backward 76 against 84).
+constexpr bool exact_threads(int t) {
+  return t == 32 || t == 64 || t == 96 || t == 128 || t == 160 || t == 192 || t == 256 || t == 320 || t == 512;
+}
+template <int VEC>
+constexpr bool fwd_exact(int nv, int t) {
+  return VEC >= 4 && exact_threads(t) && t <= 256 && (nv * VEC == 24 || nv * VEC == 32 || nv * VEC == 64);
+}
+template <int VEC>
+constexpr bool bwd_exact(int nv, int t) {
+  return VEC >= 4 && exact_threads(t) && (nv * VEC == 8 || nv * VEC == 16);
+}
+
+// Forward: as many columns a thread as leave 12 warps an SM (a thread's share
+// of the reductions and of the addressing is what costs), up to 32, and few
+// idle threads.  Rows of a warp or less go 128 threads to a block, longer ones
+// take a block each.
+template <int VEC>
+RowPlan plan_fwd(int packs, int64_t rows, int sm_count) {
+  RowPlan best;
+  double best_score = 0.0;
+  for (int nv : kFwdNv) {
+    if (!fwd_built<VEC>(nv)) continue;
+    const int t = row_threads(packs, nv);
+    if (t > kMaxRowThreads) continue;
+    const double fill = std::min(1.0, (double)rows * t / (12.0 * 32 * sm_count));
+    const double used = (double)packs / ((double)t * nv);
+    double score = fill * used * std::min(1.0, 0.5 + nv * VEC / 64.0);
+    if (packs == t * nv && fwd_exact<VEC>(nv, t)) score *= 1.3;
+    if (score > best_score) {
+      best_score = score;
+      best = RowPlan{nv, t, t > 32 ? 1 : 128 / t};
+    }
+  }
+  return best;
+}
+
+// Backward: the plan that keeps most of a block's 512 threads busy, of equal
+// ones that with the most columns a thread.
+template <int VEC>
+RowPlan plan_bwd(int packs) {
+  RowPlan best;
+  double best_score = 0.0;
+  for (int nv : kBwdNv) {
+    if (!bwd_built<VEC>(nv)) continue;
+    const int t = row_threads(packs, nv);
+    if (t > kBwdThreads) continue;
+    const int rows = kBwdThreads / t;
+    // Beyond 16 columns a thread, registers spill.
+    double score = (double)packs / ((double)t * nv) * (rows * t) / kBwdThreads * (nv * VEC > 16 ? 0.5 : 1.0);
+    if (packs == t * nv && bwd_exact<VEC>(nv, t)) score = 1.2;
+    if (score >= 0.97 * best_score) {
+      best_score = std::max(score, best_score);
+      best = RowPlan{nv, t, rows};
+    }
+  }
+  return best;
+}
+
+// fn(threads of a row as a constant) for an exact plan, else fn(0).
+template <typename Fn>
+int with_tpr(bool exact, int tpr, Fn&& fn) {
+  switch (exact ? tpr : 0) {
+    case 32: return fn(IntC<32>{});
+    case 64: return fn(IntC<64>{});
+    case 96: return fn(IntC<96>{});
+    case 128: return fn(IntC<128>{});
+    case 160: return fn(IntC<160>{});
+    case 192: return fn(IntC<192>{});
+    case 256: return fn(IntC<256>{});
+    case 320: return fn(IntC<320>{});
+    case 512: return fn(IntC<512>{});
+    default: return fn(IntC<0>{});
+  }
+}
 
 template <typename Fn>
 int with_nv(int nv, Fn&& fn) {
   switch (nv) {
     case 1: return fn(IntC<1>{});
     case 2: return fn(IntC<2>{});
+    case 3: return fn(IntC<3>{});
     case 4: return fn(IntC<4>{});
     case 8: return fn(IntC<8>{});
     case 16: return fn(IntC<16>{});
@@ -396,18 +624,44 @@ int with_types(int dtype, int wdtype, Fn&& fn) {
 bool dtype_ok(int d) { return d == B200_DTYPE_F16 || d == B200_DTYPE_BF16 || d == B200_DTYPE_F32; }
 int dtype_size(int d) { return d == B200_DTYPE_F32 ? 4 : 2; }
 
-// True when rows at `p` with pitch `ld` elements of `size` bytes all start on 16 bytes.
-bool rows_aligned(const void* p, int64_t ld, int size) { return aligned16(p) && (ld * size) % 16 == 0; }
+// Elements that an access to rows of `cols` elements of `size` bytes at `p`
+// (NULL: any) with pitch `ld` may take at once: 16 bytes' worth of the narrower
+// of its own and the `other` operand's type, two, or one.
+int row_vec(int cols, int size, int other, const void* p, int64_t ld) {
+  const int most = 16 / std::min(size, other);
+  for (int v = most; v > 1; v = v > 2 ? 2 : 1) {
+    const int bytes = std::min(16, v * size);
+    if (cols % v == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * size % bytes == 0) return v;
+  }
+  return 1;
+}
+
+// fn(elements of a pack): as many as row_vec() allows.
+template <typename T, typename Fn>
+int with_vec(int elems, Fn&& fn) {
+  if (elems == kVec16<T>) return fn(IntC<kVec16<T>>{});
+  if constexpr (sizeof(T) == 2)
+    if (elems == 2) return fn(IntC<2>{});
+  return fn(IntC<1>{});
+}
 
 int cuda_code(cudaError_t e) { return e == cudaSuccess ? B200_OK : B200_ERR_CUDA; }
 
-// Blocks of `kern` resident on the whole device.
-template <typename Kern>
-int resident_blocks(Kern kern, int threads, size_t smem, int sm_count) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm <= 0) {
-    (void)cudaGetLastError();
-    per_sm = 1;
+// Blocks of a kernel resident on the whole device.  Asked once per device and
+// block size; `kern` fixes the function, so each instantiation has its own table.
+template <auto kern>
+int resident_blocks(int threads, size_t smem, int sm_count) {
+  static std::atomic<int> table[kMaxDevices][kMaxRowThreads / 8 + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sm_count;
+  std::atomic<int>& slot = table[dev][threads / 8];
+  int per_sm = slot.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm <= 0) {
+      (void)cudaGetLastError();
+      per_sm = 1;
+    }
+    slot.store(per_sm, std::memory_order_relaxed);
   }
   return per_sm * sm_count;
 }
@@ -438,32 +692,36 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const int size = dtype_size(dtype), n = static_cast<int>(cols);
-  const int vec16 = 16 / size;
-  const bool vec = n % vec16 == 0 && rows_aligned(x, ldx, size) && rows_aligned(y, ldy, size) &&
-                   (!w || aligned16(w)) && (!b || aligned16(b));
+  const int elems = std::min({row_vec(n, size, dtype_size(wdtype), x, ldx), row_vec(n, size, dtype_size(wdtype), y, ldy),
+                              row_vec(n, dtype_size(wdtype), size, w, 0), row_vec(n, dtype_size(wdtype), size, b, 0)});
   return with_types(dtype, wdtype, [&](auto t, auto wt) {
     using T = decltype(t);
     using W = decltype(wt);
-    const RowPlan p = plan_rows(vec ? n / vec16 : n, kFwdMaxNv, rows >= 4 * dev.sm_count ? 128 : kMaxRowThreads);
-    auto go = [&](auto vc, auto nvc) {
-      auto kern = layer_norm_fwd_kernel<T, W, decltype(vc)::value, decltype(nvc)::value>;
-      const int64_t blocks = (rows + p.rows - 1) / p.rows;
-      const int grid = (int)std::min<int64_t>(blocks, 0x7fffffff);
-      return cuda_code(launch_gemm(kern, dim3(grid), dim3(p.threads, p.rows), 0, stream, static_cast<const T*>(x),
-                                   static_cast<const W*>(w), static_cast<const W*>(b), static_cast<T*>(y), mean, rstd,
-                                   rows, n, ldx, ldy, eps));
-    };
-    if (p.nv == 0) {
-      const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
-      return cuda_code(launch_gemm(layer_norm_fwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream,
-                                   static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b),
-                                   static_cast<T*>(y), mean, rstd, rows, n, ldx, ldy, eps));
-    }
-    return with_nv(p.nv, [&](auto nvc) {
-      if constexpr (decltype(nvc)::value <= kFwdMaxNv)
-        return vec ? go(IntC<kVec16<T>>{}, nvc) : go(IntC<1>{}, nvc);
-      else
-        return B200_ERR_INVALID_ARGUMENT;
+    return with_vec<T>(elems, [&](auto vc) {
+      constexpr int kV = decltype(vc)::value;
+      const RowPlan p = plan_fwd<kV>((n + kV - 1) / kV, rows, dev.sm_count);
+      if (p.nv == 0) {
+        const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
+        return cuda_code(launch_gemm(layer_norm_fwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream,
+                                     static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b),
+                                     static_cast<T*>(y), mean, rstd, rows, n, ldx, ldy, eps));
+      }
+      return with_nv(p.nv, [&](auto nvc) {
+        constexpr int kNv = decltype(nvc)::value;
+        if constexpr (fwd_built<kV>(kNv)) {
+          const bool exact = n == p.threads * kV * kNv && fwd_exact<kV>(kNv, p.threads);
+          return with_tpr(exact, p.threads, [&](auto tc) {
+            constexpr int kT = fwd_exact<kV>(kNv, decltype(tc)::value) ? decltype(tc)::value : 0;
+            constexpr auto kern = layer_norm_fwd_kernel<T, W, kV, kNv, kT>;
+            const int64_t blocks = (rows + p.rows - 1) / p.rows;
+            const int grid = (int)std::min<int64_t>(blocks, resident_blocks<kern>(p.threads * p.rows, 0, dev.sm_count));
+            return cuda_code(launch_gemm(kern, dim3(grid), dim3(p.threads, p.rows), 0, stream,
+                                         static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b),
+                                         static_cast<T*>(y), mean, rstd, rows, n, ldx, ldy, eps));
+          });
+        }
+        return (int)B200_ERR_INVALID_ARGUMENT;
+      });
     });
   });
 }
@@ -497,9 +755,9 @@ extern "C" int b200_layer_norm_bwd(const void* dy, const void* x, const void* w,
   if (int rc = current_device_info(dev)) return rc;
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
   const int size = dtype_size(dtype), n = static_cast<int>(cols);
-  const int vec16 = 16 / size;
-  const bool vec = n % vec16 == 0 && rows_aligned(x, ldx, size) && rows_aligned(dy, lddy, size) &&
-                   rows_aligned(dx, lddx, size) && (!w || aligned16(w));
+  const int wsize = dtype_size(wdtype);
+  const int elems = std::min({row_vec(n, size, wsize, x, ldx), row_vec(n, size, wsize, dy, lddy),
+                              row_vec(n, size, wsize, dx, lddx), row_vec(n, wsize, size, w, 0)});
   float* part = sums ? static_cast<float*>(workspace) : nullptr;
   return with_types(dtype, wdtype, [&](auto t, auto wt) {
     using T = decltype(t);
@@ -509,36 +767,40 @@ extern "C" int b200_layer_norm_bwd(const void* dy, const void* x, const void* w,
     const W* wp = static_cast<const W*>(w);
     T* dxp = static_cast<T*>(dx);
     int parts = 0;
-    int rc;
-    const RowPlan p = vec ? plan_rows(n / vec16, kBwdMaxNv<kVec16<T>>, kMaxRowThreads)
-                          : plan_rows(n, kBwdMaxNv<1>, kMaxRowThreads);
-    if (p.nv == 0) {
-      const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
-      rc = cuda_code(launch_gemm(layer_norm_bwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream, dyp, xp, wp,
-                                 mean, rstd, dxp, rows, n, lddy, ldx, lddx));
-      if (rc || !sums) return rc;
-      parts = (int)std::min<int64_t>(rows, 32);
-      rc = cuda_code(launch_gemm(layer_norm_bwd_columns_kernel<T>, dim3((n + 127) / 128, parts), dim3(128), 0, stream,
-                                 dyp, xp, mean, rstd, part, rows, n, lddy, ldx));
-    } else {
-      auto go = [&](auto vc, auto nvc) {
-        auto kern = layer_norm_bwd_kernel<T, W, decltype(vc)::value, decltype(nvc)::value>;
-        const size_t smem = p.rows > 1 ? (size_t)2 * n * 4 : 0;
-        const int fit = resident_blocks(kern, p.threads * p.rows, smem, dev.sm_count);
-        const int64_t blocks = (rows + p.rows - 1) / p.rows;
-        parts = (int)std::min<int64_t>({blocks, (int64_t)fit, (int64_t)kBwdMaxParts});
-        return cuda_code(launch_gemm(kern, dim3(parts), dim3(p.threads, p.rows), smem, stream, dyp, xp, wp, mean, rstd,
-                                     dxp, part, rows, n, lddy, ldx, lddx));
-      };
-      rc = with_nv(p.nv, [&](auto nvc) {
+    int rc = with_vec<T>(elems, [&](auto vc) {
+      constexpr int kV = decltype(vc)::value;
+      const RowPlan p = plan_bwd<kV>((n + kV - 1) / kV);
+      if (p.nv == 0) {
+        const int grid = (int)std::min<int64_t>(rows, 0x7fffffff);
+        int e = cuda_code(launch_gemm(layer_norm_bwd_long_kernel<T, W>, dim3(grid), dim3(kLongThreads), 0, stream, dyp,
+                                      xp, wp, mean, rstd, dxp, rows, n, lddy, ldx, lddx));
+        if (e || !sums) return e;
+        parts = (int)std::min<int64_t>(rows, 32);
+        return cuda_code(launch_gemm(layer_norm_bwd_columns_kernel<T>, dim3((n + 127) / 128, parts), dim3(128), 0,
+                                     stream, dyp, xp, mean, rstd, part, rows, n, lddy, ldx));
+      }
+      return with_nv(p.nv, [&](auto nvc) {
         constexpr int kNv = decltype(nvc)::value;
-        if (vec) {
-          if constexpr (kNv <= kBwdMaxNv<kVec16<T>>) return go(IntC<kVec16<T>>{}, nvc);
-          return (int)B200_ERR_INVALID_ARGUMENT;
+        if constexpr (bwd_built<kV>(kNv)) {
+          const bool exact = n == p.threads * kV * kNv && bwd_exact<kV>(kNv, p.threads);
+          return with_tpr(exact, p.threads, [&](auto tc) {
+            constexpr int kT = bwd_exact<kV>(kNv, decltype(tc)::value) ? decltype(tc)::value : 0;
+            constexpr auto kern = layer_norm_bwd_kernel<T, W, kV, kNv, kT>;
+            constexpr size_t kPerThread = kV * sizeof(T) == 16 ? (kAhead<kNv> + 1) * 2 * kNv * 16 : 0;
+            constexpr size_t kMost = std::max<size_t>(kPerThread * kBwdThreads, 48 * 1024);
+            static std::atomic<uint8_t> attr_done[kMaxDevices];
+            if (int e = ensure_smem_attr(kern, (int)kMost, attr_done)) return e;
+            const size_t smem = std::max(kPerThread * p.threads * p.rows, p.rows > 1 ? (size_t)2 * n * 4 : 0);
+            const int fit = resident_blocks<kern>(p.threads * p.rows, smem, dev.sm_count);
+            const int64_t blocks = (rows + p.rows - 1) / p.rows;
+            parts = (int)std::min<int64_t>({blocks, (int64_t)fit, (int64_t)kBwdMaxParts});
+            return cuda_code(launch_gemm(kern, dim3(parts), dim3(p.threads, p.rows), smem, stream, dyp, xp, wp, mean,
+                                         rstd, dxp, part, rows, n, lddy, ldx, lddx));
+          });
         }
-        return go(IntC<1>{}, nvc);
+        return (int)B200_ERR_INVALID_ARGUMENT;
       });
-    }
+    });
     if (rc || !sums) return rc;
     return cuda_code(launch_gemm(layer_norm_bwd_reduce_kernel<W>, dim3((n + 31) / 32, 2), dim3(32, 16), 0, stream,
                                  static_cast<const float*>(part), parts, n, static_cast<W*>(dw), static_cast<W*>(db)));
