@@ -30,15 +30,21 @@ constexpr int kMaxTop = B200_LOGPROBS_MAX_TOP;
 // Logits of a group: the maximum of each group of the row is kept in shared
 // memory while the row streams by.  The top k elements of a row lie in its top
 // k groups (groups ordered by maximum, then lower index: an element outside
-// them has k elements before it, one in each), so the row is not read again.
+// them has k elements before it, one in each), so only those are read again.
 constexpr int kGroup = 8;
 // Longest slice of a row that one block takes when alternatives are wanted:
-// 4096 groups, 16 KB of maxima, 16 groups a thread.
-constexpr int kTopSlice = 32768;
+// 8192 groups, 32 KB of maxima, 32 groups a thread.
+constexpr int kTopSlice = 65536;
 constexpr int kTopGroups = kTopSlice / kGroup;
 // Candidate groups after the threshold: those of the k threads whose best
 // group reaches it, kTopGroups / kThreads each at most.
 constexpr int kMaxCand = kMaxTop * (kTopGroups / kThreads);
+// Elements of the top groups, and those before the first and after the last.
+constexpr int kMaxElems = kMaxTop * kGroup + 4 * kGroup;
+// Slices of a row at most when alternatives are wanted: one a thread of the join.
+constexpr int kMaxTopVocab = kTopSlice * kThreads;
+// Groups of a thread that are on their way at once.
+constexpr int kUnroll = 4;
 
 __device__ __forceinline__ void pdl_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -96,27 +102,65 @@ __device__ __forceinline__ Sums warp_merge(Sums s) {
   return s;
 }
 
-// Adds N logits (fp32) whose maximum is `mx`.
-template <int N>
-__device__ __forceinline__ void add_logits(Sums& s, const float (&v)[N], float mx) {
-  if (!(mx <= s.m)) rebase(s, max_nan(s.m, mx));
-  const float m = s.m == kNegInf ? 0.0f : s.m;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float d = v[e] - m;
-    const float x = exp2_approx(d * kLog2e);
-    s.z += x;
-    // exp underflows to 0 long before -1e4: the clamp only keeps 0 * -inf out.
-    s.w = fmaf(x, fmaxf(d, -1.0e4f), s.w);
+// Adds a logit.
+__device__ __forceinline__ void add_logit(Sums& s, float v) {
+  if (!(v <= s.m)) rebase(s, max_nan(s.m, v));
+  const float d = v - (s.m == kNegInf ? 0.0f : s.m);
+  const float x = exp2_approx(d * kLog2e);
+  s.z += x;
+  // exp underflows to 0 long before -1e4: the clamp only keeps 0 * -inf out.
+  s.w = fmaf(x, fmaxf(d, -1.0e4f), s.w);
+}
+
+// Adds a group of logits whose maximum is `mx` and smallest `mn` (NaN in mx if
+// one is).  The sums of a thread are pairs: one instruction adds to both.
+struct PairSums {
+  float m;
+  float2 z, w;
+};
+
+__device__ __forceinline__ void add_group(PairSums& s, const float2 (&v)[kGroup / 2], float mx, float mn) {
+  if (!(mx <= s.m)) {
+    Sums a{s.m, s.z.x, s.w.x}, b{s.m, s.z.y, s.w.y};
+    const float m = max_nan(s.m, mx);
+    rebase(a, m);
+    rebase(b, m);
+    s = PairSums{m, make_float2(a.z, b.z), make_float2(a.w, b.w)};
   }
+  const float2 minus_m = pair_of(s.m == kNegInf ? 0.0f : -s.m);
+  const float2 log2e = pair_of(kLog2e);
+  const bool far = mn < -1.0e30f;  // -inf, or a mask's lowest value: d is clamped, see add_logit
+#pragma unroll
+  for (int i = 0; i < kGroup / 2; ++i) {
+    float2 d = add2(v[i], minus_m);
+    const float2 t = mul2(d, log2e);
+    const float2 x = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+    if (far) d = make_float2(fmaxf(d.x, -1.0e4f), fmaxf(d.y, -1.0e4f));
+    s.z = add2(s.z, x);
+    s.w = fma2(x, d, s.w);
+  }
+}
+
+// Three-input maximum (NaN if one is) and minimum.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // Sorts after every key with a smaller value, or with the same value and a
 // higher index.  NaN is above +inf, and -0 equals +0.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
 __device__ __forceinline__ unsigned long long make_key(float v, uint32_t index) {
-  uint32_t u = __float_as_uint(v + 0.0f);
-  u = v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - index);
+  return (static_cast<unsigned long long>(order_bits(v)) << 32) | (0xffffffffu - index);
 }
 __device__ __forceinline__ uint32_t key_index(unsigned long long k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 __device__ __forceinline__ float key_value(unsigned long long k) {
@@ -151,6 +195,21 @@ __device__ __forceinline__ Sums block_merge(Sums s, Sums* buf) {
   return r;
 }
 
+// The k-th largest of the block's keys (one a thread, 0 for none; all others
+// differ), or 0 when there are no more than k: bit by bit from the top, until
+// exactly k keys are left.
+__device__ __forceinline__ unsigned long long block_kth(unsigned long long key, int k) {
+  if (__syncthreads_count(key != 0) <= k) return 0;
+  unsigned long long t = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long u = t | (1ull << bit);
+    const int c = __syncthreads_count(key >= u);
+    if (c >= k) t = u;
+    if (c == k) break;
+  }
+  return t;
+}
+
 struct Outputs {
   float* logprob;
   float* entropy;
@@ -180,22 +239,21 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
 
 // One slice (blockIdx.x) of one row (blockIdx.y + i * gridDim.y).  With one
 // slice a row, the row's outputs are written here; otherwise the slice's sums
-// and its top keys go to `part_sums` / `part_keys` and logprobs_join_kernel
-// finishes the row.
+// and its top keys, largest first, go to `part_sums` / `part_keys` and
+// logprobs_join_kernel finishes the row.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kThreads)
     logprobs_fwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows, int64_t vocab,
                         int64_t ld, int64_t slice, int top, int64_t ignore, Outputs out, Sums* __restrict__ part_sums,
                         unsigned long long* __restrict__ part_keys) {
   constexpr int kV = kVec16<T>;
+  constexpr int kPacks = kGroup / kV;  // packs of a group
   __shared__ Sums warp_sums[kWarps];
-  // Group maxima while streaming; then the candidates of the selection.
   __shared__ float group_max[kTop ? kTopGroups : 1];
-  __shared__ unsigned long long best[kTop ? kThreads : 1];
-  __shared__ unsigned long long cand[kTop ? kMaxCand : 1];
-  __shared__ unsigned long long elems[kTop ? kMaxTop * kGroup : 1];
-  __shared__ unsigned long long threshold;
-  __shared__ int count;
+  __shared__ uint32_t cand[kTop ? kMaxCand : 1];
+  __shared__ unsigned long long elems[kTop ? kMaxElems : 1];
+  __shared__ unsigned long long bound;
+  __shared__ int count[2];
   pdl_wait();
   const int slices = gridDim.x;
   const int64_t lo = blockIdx.x * slice;
@@ -203,99 +261,88 @@ __global__ void __launch_bounds__(kThreads)
   const int tid = threadIdx.x;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const T* x = logits + row * ld;
-    Sums s{kNegInf, 0.0f, 0.0f};
+    // Groups lie between the slice's first aligned element and its last whole
+    // one; up to kV - 1 elements come before them and kGroup + kV - 1 after.
     const Span<T> span(x, lo, hi);
-    // Group g of the slice is [lo + 8 g, lo + 8 g + 8) counted from the first
-    // aligned element less one group: group 0 is the head (fewer than kV
-    // elements), the last group the tail.
-    constexpr int kPacks = kGroup / kV;  // packs of a group
-    const int64_t body_groups = (span.body_end - span.head_end) / kGroup;
-    if (span.head_end > lo && tid < span.head_end - lo) {
-      const float v[1] = {to_f32(x[lo + tid])};
-      add_logits(s, v, v[0]);
-    }
-    for (int64_t g = tid; g < body_groups; g += kThreads) {
-      float v[kGroup];
+    const T* body = x + span.head_end;
+    const int groups = static_cast<int>((span.body_end - span.head_end) / kGroup);
+    const int64_t tail = span.head_end + static_cast<int64_t>(groups) * kGroup;
+    PairSums ps{kNegInf, make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    auto load = [&](Pack<T, kV> (&q)[kPacks], int g) {
 #pragma unroll
-      for (int p = 0; p < kPacks; ++p) {
-        const Pack<T, kV> q = load_pack<T, kV>(x + span.head_end + g * kGroup + p * kV);
-#pragma unroll
-        for (int e = 0; e < kV / 2; ++e) {
-          const float2 f = q.pair(e);
-          v[p * kV + 2 * e] = f.x;
-          v[p * kV + 2 * e + 1] = f.y;
-        }
-      }
-      float mx = v[0];
-#pragma unroll
-      for (int e = 1; e < kGroup; ++e) mx = max_nan(mx, v[e]);
+      for (int p = 0; p < kPacks; ++p) q[p] = load_pack<T, kV>(body + static_cast<int64_t>(g) * kGroup + p * kV);
+    };
+    auto add = [&](const Pack<T, kV> (&q)[kPacks], int g) {
+      float2 v[kGroup / 2];
+      unpack<T, kV, kPacks>(q, v);
+      const float mx = max_nan(max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x),
+                               max3_nan(v[2].y, v[3].x, v[3].y));
+      const float mn = fminf(min3(min3(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x), min3(v[2].y, v[3].x, v[3].y));
       if (kTop) group_max[g] = mx;
-      add_logits(s, v, mx);
+      add_group(ps, v, mx, mn);
+    };
+    int g = tid;
+    for (; g + (kUnroll - 1) * kThreads < groups; g += kUnroll * kThreads) {
+      Pack<T, kV> q[kUnroll][kPacks];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) load(q[i], g + i * kThreads);
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) add(q[i], g + i * kThreads);
     }
-    const int64_t tail = span.head_end + body_groups * kGroup;  // up to kGroup + kV - 1 elements are left
-    if (tail + tid < hi) {
-      const float v[1] = {to_f32(x[tail + tid])};
-      add_logits(s, v, v[0]);
+    for (; g < groups; g += kThreads) {
+      Pack<T, kV> q[kPacks];
+      load(q, g);
+      add(q, g);
     }
+    Sums s = merge(Sums{ps.m, ps.z.x, ps.w.x}, Sums{ps.m, ps.z.y, ps.w.y});
+    if (lo + tid < span.head_end) add_logit(s, to_f32(x[lo + tid]));
+    if (tail + tid < hi) add_logit(s, to_f32(x[tail + tid]));
     s = block_merge(s, warp_sums);
     if constexpr (kTop) {
       // Threshold: the top-th largest of the threads' best groups.  Keys are
-      // unique, so exactly `top` threads reach it (or all groups qualify).
-      unsigned long long mine = 0;
-      for (int g = tid; g < body_groups; g += kThreads) {
-        const unsigned long long k = make_key(group_max[g], g);
-        mine = k > mine ? k : mine;
+      // unique, so `top` threads reach it (or every group does).
+      unsigned long long best = 0;
+      for (int i = tid; i < groups; i += kThreads) {
+        const unsigned long long k = make_key(group_max[i], i);
+        best = k > best ? k : best;
       }
-      best[tid] = mine;
       if (tid == 0) {
-        threshold = 0;
-        count = 0;
+        count[0] = count[1] = 0;
+        bound = 0;
       }
+      const unsigned long long thr = block_kth(best, top);
+      if (best >= thr)
+        for (int i = tid; i < groups; i += kThreads)
+          if (make_key(group_max[i], i) >= thr) cand[atomicAdd(&count[0], 1)] = i;
       __syncthreads();
-      int rank = 0;
-      for (int i = 0; i < kThreads; ++i) rank += best[i] > mine;
-      if (mine != 0 && rank == top - 1) threshold = mine;
-      __syncthreads();
-      const unsigned long long thr = threshold;
-      for (int g = tid; g < body_groups; g += kThreads) {
-        const unsigned long long k = make_key(group_max[g], g);
-        if (k >= thr) {
-          const int i = atomicAdd(&count, 1);
-          if (i < kMaxCand) cand[i] = k;
-        }
-      }
-      __syncthreads();
-      // With fewer than `top` threads holding a group, every group qualifies:
-      // those are fewer than kThreads <= kMaxCand.
-      const int n_cand = min(count, kMaxCand);
-      __syncthreads();
-      if (tid == 0) count = 0;
-      __syncthreads();
-      // The best `top` groups' elements, and the head's and tail's.
+      // Of the candidates, the best `top` groups; the last of them bounds the
+      // elements that can be among the top from below.
+      const int n_cand = count[0];
       for (int i = tid; i < n_cand; i += kThreads) {
-        const unsigned long long k = cand[i];
+        const unsigned long long k = make_key(group_max[cand[i]], cand[i]);
         int r = 0;
-        for (int j = 0; j < n_cand; ++j) r += cand[j] > k;
-        if (r < top) {
-          const int64_t first = span.head_end + static_cast<int64_t>(key_index(k)) * kGroup;
-          for (int e = 0; e < kGroup; ++e)
-            elems[r * kGroup + e] = make_key(to_f32(x[first + e]), static_cast<uint32_t>(first + e));
-        }
+        for (int j = 0; j < n_cand; ++j) r += make_key(group_max[cand[j]], cand[j]) > k;
+        if (r == top - 1) bound = k;
       }
-      const int n_body = min(n_cand, top) * kGroup;
       __syncthreads();
-      // `cand` now takes head and tail (fewer than 4 groups).
-      const int n_head = static_cast<int>(span.head_end - lo), n_tail = static_cast<int>(hi - tail);
-      if (tid < n_head) cand[tid] = make_key(to_f32(x[lo + tid]), static_cast<uint32_t>(lo + tid));
-      if (tid < n_tail) cand[n_head + tid] = make_key(to_f32(x[tail + tid]), static_cast<uint32_t>(tail + tid));
+      const uint32_t least = static_cast<uint32_t>(bound >> 32);
+      auto offer = [&](int64_t j) {
+        const float v = to_f32(x[j]);
+        if (order_bits(v) >= least) elems[atomicAdd(&count[1], 1)] = make_key(v, static_cast<uint32_t>(j));
+      };
+      for (int i = tid; i < n_cand * kGroup; i += kThreads) {
+        const uint32_t c = cand[i / kGroup];
+        if (make_key(group_max[c], c) >= bound) offer(span.head_end + static_cast<int64_t>(c) * kGroup + i % kGroup);
+      }
+      if (lo + tid < span.head_end) offer(lo + tid);
+      if (tail + tid < hi) offer(tail + tid);
       __syncthreads();
-      const int n_edge = n_head + n_tail, n_all = n_body + n_edge;
+      const int n = count[1];
       const float ln_z = logf(s.z);
-      for (int i = tid; i < n_all; i += kThreads) {
-        const unsigned long long k = i < n_body ? elems[i] : cand[i - n_body];
+      for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long k = elems[i];
         int r = 0;
-        for (int j = 0; j < n_body; ++j) r += elems[j] > k;
-        for (int j = 0; j < n_edge; ++j) r += cand[j] > k;
+        for (int j = 0; j < n; ++j) r += elems[j] > k;
         if (r < top) {
           if (slices == 1) {
             out.top_index[row * top + r] = key_index(k);
@@ -306,7 +353,7 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
       // A slice shorter than `top` leaves keys over: 0 sorts after every logit.
-      if (slices > 1 && tid >= n_all && tid < top) part_keys[(row * slices + blockIdx.x) * top + tid] = 0;
+      if (slices > 1 && tid >= n && tid < top) part_keys[(row * slices + blockIdx.x) * top + tid] = 0;
     }
     if (tid == 0) {
       if (slices == 1)
@@ -318,13 +365,16 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Joins the slices of a row; one block a row.
+// Joins the slices of a row (with alternatives, kThreads of them at most); one
+// block a row.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kThreads)
     logprobs_join_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows,
                          int64_t vocab, int64_t ld, int slices, int top, int64_t ignore, Outputs out,
                          const Sums* __restrict__ part_sums, const unsigned long long* __restrict__ part_keys) {
   __shared__ Sums warp_sums[kWarps];
+  __shared__ unsigned long long elems[kTop ? kMaxTop * kMaxTop : 1];
+  __shared__ int count;
   pdl_wait();
   const int tid = threadIdx.x;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -332,13 +382,25 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = tid; i < slices; i += kThreads) s = merge(s, part_sums[row * slices + i]);
     s = block_merge(s, warp_sums);
     if constexpr (kTop) {
-      const unsigned long long* keys = part_keys + row * slices * top;
+      // As in a slice: the top-th largest of the slices' first keys is a lower
+      // bound, which the keys of at most `top` slices reach.
+      const unsigned long long* keys = part_keys + (row * slices + tid) * top;
+      if (tid == 0) count = 0;
+      const unsigned long long first = tid < slices ? keys[0] : 0;
+      const unsigned long long thr = block_kth(first, top);
+      if (first != 0 && first >= thr)
+        for (int i = 0; i < top; ++i) {
+          const unsigned long long k = keys[i];
+          if (k == 0 || k < thr) break;
+          elems[atomicAdd(&count, 1)] = k;
+        }
+      __syncthreads();
+      const int n = count;
       const float ln_z = logf(s.z);
-      for (int i = tid; i < slices * top; i += kThreads) {
-        const unsigned long long k = keys[i];
-        if (k == 0) continue;
+      for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long k = elems[i];
         int r = 0;
-        for (int j = 0; j < slices * top && r < top; ++j) r += keys[j] > k;
+        for (int j = 0; j < n; ++j) r += elems[j] > k;
         if (r < top) {
           out.top_index[row * top + r] = key_index(k);
           out.top_logprob[row * top + r] = s.m == kNegInf ? kNegInf : (key_value(k) - s.m) - ln_z;
@@ -350,12 +412,17 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// What the gradient of a row's logits needs of the row.
+struct RowGrad {
+  float minus_m, minus_ln_z, entropy, gl, gh;
+};
+
 // gl ([j == t] - p) - gh p (ln p + entropy)
-__device__ __forceinline__ float grad_of(float x, float2 st, float ent, float gl, float gh, bool is_target) {
-  const float d = (x - st.x) - st.y;
+__device__ __forceinline__ float grad_of(float x, const RowGrad& r, bool is_target) {
+  const float d = (x + r.minus_m) + r.minus_ln_z;
   const float p = exp2_approx(d * kLog2e);
-  const float g = -p * fmaf(gh, fmaxf(d, -1.0e4f) + ent, gl);
-  return is_target ? g + gl : g;
+  const float g = -p * fmaf(r.gh, fmaxf(d, -1.0e4f) + r.entropy, r.gl);
+  return is_target ? g + r.gl : g;
 }
 
 template <typename T>
@@ -374,39 +441,53 @@ __global__ void __launch_bounds__(kThreads)
     const T* x = logits + row * ld;
     T* d = dlogits + row * ldd;
     const int64_t target = targets[row];
-    const float2 lse = stats[row];
-    const float ent = entropy[row];
+    const float2 st = stats[row];
     const float gl = g_logprob && target != ignore ? g_logprob[row] : 0.0f;
-    const float gh = g_entropy ? g_entropy[row] : 0.0f;
-    if (lse.x == kNegInf) {
+    const RowGrad r{-st.x, -st.y, entropy[row], gl, g_entropy ? g_entropy[row] : 0.0f};
+    if (st.x == kNegInf) {
       // No probability anywhere: nothing depends on the logits.
       for (int64_t j = lo + tid; j < hi; j += kThreads) d[j] = from_f32<T>(0.0f);
       continue;
     }
     const Span<T> span(x, lo, hi);
-    const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
-    if (!same) {
-      for (int64_t j = lo + tid; j < hi; j += kThreads)
-        d[j] = from_f32<T>(grad_of(to_f32(x[j]), lse, ent, gl, gh, j == target));
+    auto one = [&](int64_t j) { d[j] = from_f32<T>(grad_of(to_f32(x[j]), r, j == target)); };
+    if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) != 0) {
+      // Logits and gradient are aligned differently.
+      for (int64_t j = lo + tid; j < hi; j += kThreads) one(j);
       continue;
     }
-    if (lo + tid < span.head_end)
-      d[lo + tid] = from_f32<T>(grad_of(to_f32(x[lo + tid]), lse, ent, gl, gh, lo + tid == target));
-    for (int64_t j = span.head_end + tid * kV; j < span.body_end; j += kThreads * kV) {
-      const Pack<T, kV> q = load_pack<T, kV>(x + j);
+    const float2 minus_m = pair_of(r.minus_m), minus_ln_z = pair_of(r.minus_ln_z), log2e = pair_of(kLog2e);
+    const float2 ent = pair_of(r.entropy), gl2 = pair_of(r.gl), gh2 = pair_of(r.gh);
+    const T* body = x + span.head_end;
+    T* out = d + span.head_end;
+    const int packs = static_cast<int>((span.body_end - span.head_end) / kV);
+    auto work = [&](const Pack<T, kV>& q, int i) {
       Pack<T, kV> o;
 #pragma unroll
       for (int e = 0; e < kV / 2; ++e) {
-        const float2 f = q.pair(e);
-        o.set_pair(e, make_float2(grad_of(f.x, lse, ent, gl, gh, j + 2 * e == target),
-                                  grad_of(f.y, lse, ent, gl, gh, j + 2 * e + 1 == target)));
+        float2 f = add2(add2(q.pair(e), minus_m), minus_ln_z);
+        const float2 t = mul2(f, log2e);
+        // -p (gl + gh (ln p + entropy)); ln p is clamped where p is 0.
+        const float2 p = make_float2(-exp2_approx(t.x), -exp2_approx(t.y));
+        f = make_float2(fmaxf(f.x, -1.0e4f), fmaxf(f.y, -1.0e4f));
+        o.set_pair(e, mul2(p, fma2(gh2, add2(f, ent), gl2)));
       }
-      store_pack<T, kV>(d + j, o);
+      store_pack<T, kV>(out + static_cast<int64_t>(i) * kV, o);
+    };
+    int i = tid;
+    for (; i + (kUnroll - 1) * kThreads < packs; i += kUnroll * kThreads) {
+      Pack<T, kV> q[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) q[u] = load_pack<T, kV>(body + static_cast<int64_t>(i + u * kThreads) * kV);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) work(q[u], i + u * kThreads);
     }
-    if (span.body_end + tid < hi)
-      d[span.body_end + tid] =
-          from_f32<T>(
-          grad_of(to_f32(x[span.body_end + tid]), lse, ent, gl, gh, span.body_end + tid == target));
+    for (; i < packs; i += kThreads) work(load_pack<T, kV>(body + static_cast<int64_t>(i) * kV), i);
+    if (lo + tid < span.head_end) one(lo + tid);
+    if (span.body_end + tid < hi) one(span.body_end + tid);
+    // The target's element once more, by the thread that wrote its pack.
+    if (target >= span.head_end && target < span.body_end && (target - span.head_end) / kV % kThreads == tid)
+      one(target);
   }
 }
 
@@ -426,7 +507,7 @@ int with_dtype(int dtype, Fn&& fn) {
 int64_t row_slices(int64_t rows, int64_t vocab, int top) {
   constexpr int64_t kBlocks = 4 * 148, kLeast = 4096;
   int64_t s = std::max<int64_t>(1, std::min(kBlocks / std::max<int64_t>(rows, 1), vocab / kLeast));
-  if (top > 0) s = std::max(s, (vocab + kTopSlice - 1) / kTopSlice);
+  if (top > 0) s = std::max(std::min<int64_t>(s, kThreads), (vocab + kTopSlice - 1) / kTopSlice);
   return s;
 }
 
@@ -439,7 +520,7 @@ int64_t slice_length(int64_t vocab, int64_t slices) { return round_up((vocab + s
 extern "C" int64_t b200_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top) {
   using namespace b200;
   if (rows < 0 || vocab < 0 || top < 0 || top > kMaxTop) return -B200_ERR_INVALID_ARGUMENT;
-  if (vocab > 0x7fffffff) return -B200_ERR_TOO_LARGE;
+  if (vocab > (top > 0 ? kMaxTopVocab : 0x7fffffff)) return -B200_ERR_TOO_LARGE;
   const int64_t s = row_slices(rows, vocab, top);
   if (s <= 1) return 0;
   return round_up(rows * s * (int64_t)sizeof(Sums), 256) + rows * s * top * 8;
@@ -452,7 +533,7 @@ extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* target
   using namespace b200;
   if (rows < 0 || vocab < 0 || top < 0 || top > kMaxTop || top > vocab || !dtype_ok(dtype))
     return B200_ERR_INVALID_ARGUMENT;
-  if (vocab > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (vocab > (top > 0 ? kMaxTopVocab : 0x7fffffff)) return B200_ERR_TOO_LARGE;
   if (rows == 0) return B200_OK;
   if (vocab == 0 || !logits || !targets || !logprob || !entropy || !stats || ld < vocab ||
       (top > 0 && (!top_logprob || !top_index)))

@@ -220,7 +220,8 @@ B200_API int b200_layer_norm_bwd(const void* dy, const void* x, const void* w, c
  * with their indices, largest first, equal logits by lower index (NaN first of
  * all).  A target equal to ignore_index gives logprob 0; any other target
  * outside [0, vocab) gives NaN.  A row of -inf throughout gives logprob -inf
- * and entropy 0.  stats (rows x 2 floats) receives the row's maximum and
+ * and entropy 0.  vocab is at most 2^31 - 1, with alternatives 2^24.  stats
+ * (rows x 2 floats) receives the row's maximum and
  * ln(sum exp(x - max)), which the backward call reads.  The workspace
  * (b200_token_logprobs_workspace_size bytes, may be 0; 256-byte aligned)
  * holds the parts of rows that several blocks share.  No counterpart in the
