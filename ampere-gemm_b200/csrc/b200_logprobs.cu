@@ -17,6 +17,7 @@
 // fp32 in a fixed order.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "elem_types.cuh"
 #include "host_common.cuh"
@@ -36,8 +37,8 @@ constexpr int kGroup = 8;
 // 8192 groups, 32 KB of maxima, 32 groups a thread.
 constexpr int kTopSlice = 65536;
 constexpr int kTopGroups = kTopSlice / kGroup;
-// Candidate groups after the threshold: those of the k threads whose best
-// group reaches it, kTopGroups / kThreads each at most.
+// Candidate groups after the threshold: those of the threads whose best group
+// reaches it, kMaxTop of them with kTopGroups / kThreads each at most.
 constexpr int kMaxCand = kMaxTop * (kTopGroups / kThreads);
 // Elements of the top groups, and those before the first and after the last.
 constexpr int kMaxElems = kMaxTop * kGroup + 4 * kGroup;
@@ -51,9 +52,10 @@ __device__ __forceinline__ void pdl_wait() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// 2^v, subnormal results as 0 (handling them would take four instructions more).
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 
@@ -88,18 +90,6 @@ __device__ __forceinline__ Sums merge(Sums a, Sums b) {
   rebase(a, m);
   rebase(b, m);
   return Sums{m, a.z + b.z, a.w + b.w};
-}
-
-__device__ __forceinline__ Sums warp_merge(Sums s) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums t;
-    t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    t.z = __shfl_xor_sync(0xffffffffu, s.z, o);
-    t.w = __shfl_xor_sync(0xffffffffu, s.w, o);
-    s = merge(s, t);
-  }
-  return s;
 }
 
 // Adds a logit.
@@ -155,9 +145,10 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 
 // Sorts after every key with a smaller value, or with the same value and a
 // higher index.  NaN is above +inf, and -0 equals +0.
+constexpr uint32_t kNanOrder = 0xffff0000u;
 __device__ __forceinline__ uint32_t order_bits(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);
-  return v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return v != v ? kNanOrder : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ unsigned long long make_key(float v, uint32_t index) {
   return (static_cast<unsigned long long>(order_bits(v)) << 32) | (0xffffffffu - index);
@@ -165,7 +156,7 @@ __device__ __forceinline__ unsigned long long make_key(float v, uint32_t index) 
 __device__ __forceinline__ uint32_t key_index(unsigned long long k) { return 0xffffffffu - static_cast<uint32_t>(k); }
 __device__ __forceinline__ float key_value(unsigned long long k) {
   const uint32_t u = static_cast<uint32_t>(k >> 32);
-  if (u == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  if (u == kNanOrder) return __uint_as_float(0x7fffffffu);
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
@@ -184,30 +175,90 @@ struct Span {
   }
 };
 
-// Block-wide merge; every thread gets the result.
-__device__ __forceinline__ Sums block_merge(Sums s, Sums* buf) {
-  s = warp_merge(s);
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = s;
-  __syncthreads();
-  Sums r = buf[0];
+// The block's sums, for every thread: the maximum first, then one rebase a
+// thread and plain sums.
+struct MergeBuffer {
+  __align__(16) float m[kWarps];
+  float2 zw[kWarps];
+};
+__device__ __forceinline__ Sums block_merge(Sums s, MergeBuffer& buf) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = s.m;
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) r = merge(r, buf[i]);
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) buf.m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) m = max_nan(m, buf.m[i]);
+  rebase(s, m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+    s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+  }
+  if (lane == 0) buf.zw[warp] = make_float2(s.z, s.w);
+  __syncthreads();
+  Sums r{m, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    r.z += buf.zw[i].x;
+    r.w += buf.zw[i].y;
+  }
   return r;
 }
 
-// The k-th largest of the block's keys (one a thread, 0 for none; all others
-// differ), or 0 when there are no more than k: bit by bit from the top, until
-// exactly k keys are left.
-__device__ __forceinline__ unsigned long long block_kth(unsigned long long key, int k) {
+// A lower bound of the top k of the block's keys (one a thread; 0 for none; all
+// others differ), which at least k of them and at most max(k, kMaxTop) reach;
+// 0 when there are no more than k.  Found bit by bit from the first in which
+// the keys differ: the values' bits, of which those below `low` are alike
+// for values of one sign (16-bit types), then, if too many values are equal, the indexes'.
+// Lowest bit of fp32 that a value of the type can have (other than by its sign).
+template <typename T>
+constexpr int kLowBit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+struct KthBuffer {
+  uint32_t most[kWarps], least[kWarps];
+};
+__device__ __forceinline__ unsigned long long block_bound(unsigned long long key, int k, int low, KthBuffer& buf) {
+  const uint32_t v = static_cast<uint32_t>(key >> 32);
   if (__syncthreads_count(key != 0) <= k) return 0;
-  unsigned long long t = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const unsigned long long u = t | (1ull << bit);
-    const int c = __syncthreads_count(key >= u);
-    if (c >= k) t = u;
+  const uint32_t most = __reduce_max_sync(0xffffffffu, v), least = __reduce_min_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) {
+    buf.most[threadIdx.x >> 5] = most;
+    buf.least[threadIdx.x >> 5] = least;
+  }
+  __syncthreads();
+  uint32_t hi = most, lo = least;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    hi = max(hi, buf.most[i]);
+    lo = min(lo, buf.least[i]);
+  }
+  const int first = 31 - __clz((hi ^ lo) | 1u);
+  uint32_t t = first == 31 ? 0u : hi >> (first + 1) << (first + 1);
+  int reach = kThreads;  // keys that reach t
+  for (int bit = first; bit >= low; --bit) {
+    const uint32_t u = t | (1u << bit);
+    const int c = __syncthreads_count(v >= u);
+    if (c >= k) {
+      t = u;
+      reach = c;
+    }
     if (c == k) break;
   }
-  return t;
+  if (reach <= kMaxTop) return static_cast<unsigned long long>(t) << 32;
+  // Too many equal values at t (whose bits below `low` are all ones for a
+  // negative value, see order_bits): their indexes decide.
+  if ((t & 0x80000000u) == 0) t |= (1u << low) - 1;
+  const bool tied = key != 0 && v == t;
+  const int above = __syncthreads_count(v > t);
+  uint32_t at = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t u = at | (1u << bit);
+    const int c = above + __syncthreads_count(tied && static_cast<uint32_t>(key) >= u);
+    if (c >= k) at = u;
+    if (c == k) break;
+  }
+  return (static_cast<unsigned long long>(t) << 32) | at;
 }
 
 struct Outputs {
@@ -248,7 +299,8 @@ __global__ void __launch_bounds__(kThreads)
                         unsigned long long* __restrict__ part_keys) {
   constexpr int kV = kVec16<T>;
   constexpr int kPacks = kGroup / kV;  // packs of a group
-  __shared__ Sums warp_sums[kWarps];
+  __shared__ MergeBuffer merge_buf;
+  __shared__ KthBuffer kth_buf;
   __shared__ float group_max[kTop ? kTopGroups : 1];
   __shared__ uint32_t cand[kTop ? kMaxCand : 1];
   __shared__ unsigned long long elems[kTop ? kMaxElems : 1];
@@ -268,6 +320,8 @@ __global__ void __launch_bounds__(kThreads)
     const int groups = static_cast<int>((span.body_end - span.head_end) / kGroup);
     const int64_t tail = span.head_end + static_cast<int64_t>(groups) * kGroup;
     PairSums ps{kNegInf, make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    float best_max = __uint_as_float(0x7fffffffu);  // the thread's best group: none yet, so any is better
+    int best_group = -1;
     auto load = [&](Pack<T, kV> (&q)[kPacks], int g) {
 #pragma unroll
       for (int p = 0; p < kPacks; ++p) q[p] = load_pack<T, kV>(body + static_cast<int64_t>(g) * kGroup + p * kV);
@@ -278,7 +332,14 @@ __global__ void __launch_bounds__(kThreads)
       const float mx = max_nan(max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x),
                                max3_nan(v[2].y, v[3].x, v[3].y));
       const float mn = fminf(min3(min3(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x), min3(v[2].y, v[3].x, v[3].y));
-      if (kTop) group_max[g] = mx;
+      if (kTop) {
+        group_max[g] = mx;
+        // Strictly larger only: of equal groups the first stays.
+        if (!(mx <= best_max)) {
+          best_max = mx;
+          best_group = g;
+        }
+      }
       add_group(ps, v, mx, mn);
     };
     int g = tid;
@@ -297,20 +358,23 @@ __global__ void __launch_bounds__(kThreads)
     Sums s = merge(Sums{ps.m, ps.z.x, ps.w.x}, Sums{ps.m, ps.z.y, ps.w.y});
     if (lo + tid < span.head_end) add_logit(s, to_f32(x[lo + tid]));
     if (tail + tid < hi) add_logit(s, to_f32(x[tail + tid]));
-    s = block_merge(s, warp_sums);
+    s = block_merge(s, merge_buf);
     if constexpr (kTop) {
-      // Threshold: the top-th largest of the threads' best groups.  Keys are
-      // unique, so `top` threads reach it (or every group does).
-      unsigned long long best = 0;
-      for (int i = tid; i < groups; i += kThreads) {
-        const unsigned long long k = make_key(group_max[i], i);
-        best = k > best ? k : best;
+      // Threshold: a bound that at least `top` of the threads' best groups and
+      // at most kMaxTop threads reach (or every group does).
+      unsigned long long best = best_group >= 0 ? make_key(best_max, best_group) : 0;
+      if (s.m != s.m) {
+        // A NaN in the row: comparisons above may have dropped it.
+        for (int i = tid; i < groups; i += kThreads) {
+          const unsigned long long k = make_key(group_max[i], i);
+          best = k > best ? k : best;
+        }
       }
       if (tid == 0) {
         count[0] = count[1] = 0;
         bound = 0;
       }
-      const unsigned long long thr = block_kth(best, top);
+      const unsigned long long thr = block_bound(best, top, kLowBit<T>, kth_buf);
       if (best >= thr)
         for (int i = tid; i < groups; i += kThreads)
           if (make_key(group_max[i], i) >= thr) cand[atomicAdd(&count[0], 1)] = i;
@@ -372,7 +436,8 @@ __global__ void __launch_bounds__(kThreads)
     logprobs_join_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows,
                          int64_t vocab, int64_t ld, int slices, int top, int64_t ignore, Outputs out,
                          const Sums* __restrict__ part_sums, const unsigned long long* __restrict__ part_keys) {
-  __shared__ Sums warp_sums[kWarps];
+  __shared__ MergeBuffer merge_buf;
+  __shared__ KthBuffer kth_buf;
   __shared__ unsigned long long elems[kTop ? kMaxTop * kMaxTop : 1];
   __shared__ int count;
   pdl_wait();
@@ -380,14 +445,14 @@ __global__ void __launch_bounds__(kThreads)
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     Sums s{kNegInf, 0.0f, 0.0f};
     for (int i = tid; i < slices; i += kThreads) s = merge(s, part_sums[row * slices + i]);
-    s = block_merge(s, warp_sums);
+    s = block_merge(s, merge_buf);
     if constexpr (kTop) {
-      // As in a slice: the top-th largest of the slices' first keys is a lower
-      // bound, which the keys of at most `top` slices reach.
+      // As in a slice: a lower bound that the first keys of at least `top` and
+      // at most kMaxTop slices reach.
       const unsigned long long* keys = part_keys + (row * slices + tid) * top;
       if (tid == 0) count = 0;
       const unsigned long long first = tid < slices ? keys[0] : 0;
-      const unsigned long long thr = block_kth(first, top);
+      const unsigned long long thr = block_bound(first, top, kLowBit<T>, kth_buf);
       if (first != 0 && first >= thr)
         for (int i = 0; i < top; ++i) {
           const unsigned long long k = keys[i];

@@ -42,7 +42,17 @@ struct ActValue {
   float f, slope;
 };
 
-__device__ __forceinline__ float sigmoid_approx(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float exp_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+// 1 / (1 + exp(-x)); exp(-x) = infinity gives 0.
+__device__ __forceinline__ float sigmoid_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp_approx(-x)));
+  return r;
+}
 
 template <int kAct, bool kSlope>
 __device__ __forceinline__ ActValue activate(float g) {
@@ -55,7 +65,7 @@ __device__ __forceinline__ ActValue activate(float g) {
   } else if constexpr (kAct == 1) {  // gelu: g Phi(g)
     const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
     r.f = g * cdf;
-    if (kSlope) r.slope = cdf + g * (0.39894228040143268f * __expf(-0.5f * g * g));
+    if (kSlope) r.slope = cdf + g * (0.39894228040143268f * exp_approx(-0.5f * g * g));
   } else {  // gelu with tanh: g (1 + tanh z) / 2 = g s(2z), z = sqrt(2/pi) (g + 0.044715 g^3)
     constexpr float kC = 0.79788456080286536f, kA = 0.044715f;
     const float s = sigmoid_approx(2.0f * kC * g * (1.0f + kA * g * g));
