@@ -10,7 +10,12 @@
 // dg, du and a.  The other products are plain GEMMs on the library's kernels.
 // g, u, a, dg and du are kept in the operands' 16-bit type between launches:
 // the tensor cores take 16-bit operands, and each such rounding adds about as
-// much error as the one rounding of the result.
+// much error as the one rounding of the result.  Their rows are padded to a
+// multiple of 8 elements (`hidden_pad`).
+//
+// Operands that TMA cannot address (rows that do not start on 16 bytes) are
+// copied into the workspace by one launch before the products, results that it
+// cannot store by one launch after them.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -25,13 +30,14 @@ namespace {
 
 struct GateShape {
   int rows, hidden, depth;  // of the fused GEMM: M, N (columns of a), K
+  int hidden_pad;           // row pitch of a, and of each half of [g u] and [dg du]
 };
 
 // Launches the pair kernel with a fused epilogue: 256 x 256 accumulator tiles,
 // one cluster per tile, tiles taken dynamically.  A is rows x depth (K-major);
 // B is 2 hidden x depth (gate and up) or depth x hidden row-major (backward).
 template <bool kBf16, int kEpi>
-int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, const GateShape& s,
+int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, const GateShape& s,
                 const FusedArgs<kEpi>& fx, cudaStream_t stream) {
   constexpr bool kUp = kEpi == kEpiGateUp;
   constexpr int kOutN = kUp ? 128 : 256;
@@ -43,7 +49,7 @@ int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B)
            : make_tmap_2d(&tb, B, s.depth, s.hidden, ldb, 64, Cfg::kStageK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (rc) return rc;
-  rc = make_tmap_2d(&tc, C, s.rows, s.hidden, ldc, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+  rc = make_tmap_2d(&tc, C, s.rows, s.hidden_pad, s.hidden_pad, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE);
   if (rc) return rc;
   auto kern = gemm_f16_tcgen05_pair_kernel<3, 2, 1, !kUp, false, 256, true, kBf16, kEpi>;
   static std::atomic<uint8_t> attr_done[kMaxDevices];
@@ -53,20 +59,16 @@ int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
   if (tiles > 0x3fffffffLL) return B200_ERR_TOO_LARGE;
   EpiParams ep;
   ep.m = s.rows;
-  ep.n = s.hidden;
-  ep.n_tma = s.hidden;
-  ep.ldc = ldc;
+  ep.n = ep.n_tma = s.hidden_pad;
+  ep.ldc = s.hidden_pad;
   ep.c = static_cast<uint16_t*>(C);
   const cudaError_t le = launch_gemm(kern, dim3(2 * (unsigned)tiles), dim3(kThreads), Cfg::kSmemBytes, stream, ta, tb,
                                      tc, s.rows, s.hidden, s.depth, 8, ep, SplitTail{}, fx);
   return le == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 
-// Map of a rows x hidden output block that the epilogue warps store.
-int store_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld) {
-  return make_tmap_2d(map, base, rows, cols, ld, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE);
-}
-
+// Columns [hidden, hidden_pad) of a, g and u hold whatever the tile computed
+// there (the up projection's first rows as gates); nothing reads them.
 template <bool kBf16>
 int gate_up(const void* x, int64_t ldx, const void* w_in, int64_t ldw, uint16_t* a, uint16_t* gate_up, int act,
             const GateShape& s, cudaStream_t stream) {
@@ -74,10 +76,12 @@ int gate_up(const void* x, int64_t ldx, const void* w_in, int64_t ldw, uint16_t*
   fx.activation = act;
   fx.save = gate_up != nullptr;
   // Unused maps point at `a`, so that every launch has valid ones.
-  const int64_t ld = gate_up ? 2 * (int64_t)s.hidden : s.hidden;
-  if (int rc = store_map(&fx.tmap_g, gate_up ? gate_up : a, s.rows, s.hidden, ld)) return rc;
-  if (int rc = store_map(&fx.tmap_u, gate_up ? gate_up + s.hidden : a, s.rows, s.hidden, ld)) return rc;
-  return launch_gate<kBf16, kEpiGateUp>(x, ldx, w_in, ldw, a, s.hidden, s, fx, stream);
+  const int64_t ld = gate_up ? 2 * (int64_t)s.hidden_pad : s.hidden_pad;
+  for (int half = 0; half < 2; ++half)
+    if (int rc = make_tmap_2d(half ? &fx.tmap_u : &fx.tmap_g, gate_up ? gate_up + half * s.hidden_pad : a, s.rows,
+                              s.hidden_pad, ld, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE))
+      return rc;
+  return launch_gate<kBf16, kEpiGateUp>(x, ldx, w_in, ldw, a, s, fx, stream);
 }
 
 template <bool kBf16>
@@ -86,12 +90,104 @@ int gate_bwd(const void* dy, int64_t lddy, const void* w_out, int64_t ldw, const
   FusedArgs<kEpiGateBwd> fx;
   fx.activation = act;
   fx.g = gate_up;
-  fx.u = gate_up + s.hidden;
-  fx.ld = 2 * (int64_t)s.hidden;
-  if (int rc = store_map(&fx.tmap_dg, dgu, s.rows, s.hidden, fx.ld)) return rc;
-  if (int rc = store_map(&fx.tmap_du, dgu + s.hidden, s.rows, s.hidden, fx.ld)) return rc;
-  if (int rc = store_map(&fx.tmap_a, a, s.rows, s.hidden, s.hidden)) return rc;
-  return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s.hidden, s, fx, stream);
+  fx.u = gate_up + s.hidden_pad;
+  fx.dg = dgu;
+  fx.du = dgu + s.hidden_pad;
+  fx.a = a;
+  fx.ld = 2 * (int64_t)s.hidden_pad;
+  fx.ld_a = s.hidden_pad;
+  return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s, fx, stream);
+}
+
+// A matrix copied between pitches; columns [cols, dst_cols) of the copy, and
+// `zero_rows` rows after it, are zero.
+struct CopyJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t src_ld, dst_ld, rows, zero_rows;
+  int64_t cols, dst_cols;
+};
+constexpr int kMaxJobs = 6;
+struct CopyJobs {
+  CopyJob job[kMaxJobs];
+  int n = 0;
+  void add(const void* src, int64_t src_ld, void* dst, int64_t dst_ld, int64_t rows, int64_t cols, int64_t dst_cols,
+           int64_t zero_rows = 0) {
+    job[n++] = CopyJob{static_cast<const uint16_t*>(src), static_cast<uint16_t*>(dst), src_ld, dst_ld, rows,
+                       zero_rows, cols, dst_cols};
+  }
+};
+
+// blockIdx.y = job, a block a row in turn, a thread eight columns in turn.
+__global__ void copy_jobs_kernel(const __grid_constant__ CopyJobs jobs) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const CopyJob& j = jobs.job[blockIdx.y];
+  const bool src16 = (reinterpret_cast<uintptr_t>(j.src) & 15u) == 0 && j.src_ld % 8 == 0;
+  const bool dst16 = (reinterpret_cast<uintptr_t>(j.dst) & 15u) == 0 && j.dst_ld % 8 == 0;
+  for (int64_t r = blockIdx.x; r < j.rows + j.zero_rows; r += gridDim.x) {
+    const uint16_t* src = j.src + r * j.src_ld;
+    uint16_t* dst = j.dst + r * j.dst_ld;
+    const int64_t cols = r < j.rows ? j.cols : 0;
+    for (int64_t c = threadIdx.x * 8; c < j.dst_cols; c += blockDim.x * 8) {
+      uint16_t v[8] = {};
+      if (src16 && c + 8 <= cols) {
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) v[e] = src[c + e];
+      }
+      if (dst16 && c + 8 <= j.dst_cols) {
+        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < j.dst_cols) dst[c + e] = v[e];
+      }
+    }
+  }
+}
+
+int run_copies(const CopyJobs& jobs, cudaStream_t stream) {
+  if (jobs.n == 0) return B200_OK;
+  int64_t rows = 1;
+  for (int i = 0; i < jobs.n; ++i) rows = std::max(rows, jobs.job[i].rows + jobs.job[i].zero_rows);
+  const cudaError_t e = launch_gemm(copy_jobs_kernel, dim3((unsigned)std::min<int64_t>(rows, 8 * 148), jobs.n),
+                                    dim3(128), 0, stream, jobs);
+  return e == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
+int64_t pad8(int64_t n) { return round_up(n, 8); }
+
+// Bytes of a rows x cols 16-bit matrix with padded rows in a workspace.
+int64_t part_bytes(int64_t rows, int64_t cols) { return round_up(rows * pad8(cols) * 2, 256); }
+
+// Takes padded matrices out of a workspace.
+struct Carver {
+  uint8_t* at;
+  uint16_t* take(int64_t rows, int64_t cols) {
+    uint16_t* p = reinterpret_cast<uint16_t*>(at);
+    at += part_bytes(rows, cols);
+    return p;
+  }
+};
+
+// The operand as TMA can read it: itself, or a copy that `jobs` will make.
+const void* readable(const void* p, int64_t& ld, int64_t rows, int64_t cols, Carver& ws, CopyJobs& jobs) {
+  if (pitch_ok(p, ld)) return p;
+  uint16_t* copy = ws.take(rows, cols);
+  jobs.add(p, ld, copy, pad8(cols), rows, cols, pad8(cols));
+  ld = pad8(cols);
+  return copy;
+}
+// The result as TMA can store it: itself, or a matrix that `jobs` will copy.
+void* writable(void* p, int64_t& ld, int64_t rows, int64_t cols, Carver& ws, CopyJobs& jobs) {
+  if (pitch_ok(p, ld)) return p;
+  uint16_t* copy = ws.take(rows, cols);
+  jobs.add(copy, pad8(cols), p, ld, rows, cols, cols);
+  ld = pad8(cols);
+  return copy;
 }
 
 int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
@@ -223,7 +319,6 @@ int check_ffn(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int ac
   if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) return B200_ERR_INVALID_ARGUMENT;
   if (dtype != B200_DTYPE_F16 && dtype != B200_DTYPE_BF16) return B200_ERR_INVALID_ARGUMENT;
   if (rows > 0x7fffffff || dim > 0x7fffffff || hidden > 0x3fffffff || out_dim > 0x7fffffff) return B200_ERR_TOO_LARGE;
-  if (hidden % 8 != 0) return B200_ERR_MISALIGNED;
   *empty = rows == 0 || dim == 0 || hidden == 0 || out_dim == 0;
   return B200_OK;
 }
@@ -232,9 +327,6 @@ int zero_rows(void* p, int64_t ld, int64_t rows, int64_t cols, cudaStream_t stre
   if (!p || rows == 0 || cols == 0) return B200_OK;
   return cudaMemset2DAsync(p, ld * 2, 0, cols * 2, rows, stream) == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
-
-// Bytes of a rows x cols 16-bit matrix in a workspace.
-int64_t part_bytes(int64_t rows, int64_t cols) { return round_up(rows * cols * 2, 256); }
 
 bool workspace_ok(const void* ws, int64_t bytes, int64_t need) {
   return need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255u) == 0);
@@ -252,10 +344,20 @@ int take_error_word_ffn() {
 
 }  // namespace b200
 
-extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int backward) {
-  if (rows < 0 || hidden < 0) return -B200_ERR_INVALID_ARGUMENT;
-  if (rows > 0x7fffffff || hidden > 0x3fffffff) return -B200_ERR_TOO_LARGE;
-  return b200::part_bytes(rows, hidden) + (backward ? b200::part_bytes(rows, 2 * hidden) : 0);
+extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim,
+                                                 int backward, int unaligned) {
+  using namespace b200;
+  if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return -B200_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7fffffff || dim > 0x7fffffff || hidden > 0x3fffffff || out_dim > 0x7fffffff)
+    return -B200_ERR_TOO_LARGE;
+  const int64_t hp = pad8(hidden);
+  int64_t n = part_bytes(rows, hp) + (backward ? part_bytes(rows, 2 * hp) : 0);
+  if (unaligned || hidden % 8 != 0 || dim % 8 != 0 || out_dim % 8 != 0) {
+    const int64_t in = part_bytes(rows, dim), w_in = part_bytes(2 * hp, dim), w_out = part_bytes(out_dim, hp),
+                  out = part_bytes(rows, out_dim);
+    n += in + w_in + w_out + out + (backward ? in + w_in + w_out : 0);
+  }
+  return n;
 }
 
 extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w_out, void* y, void* gate_up,
@@ -266,37 +368,46 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   bool empty = false;
   if (int rc = check_ffn(rows, dim, hidden, out_dim, activation, dtype, &empty)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const int64_t hp = pad8(hidden);
   if (empty) {
     if (rows > 0 && out_dim > 0 && (!y || ldy < out_dim)) return B200_ERR_INVALID_ARGUMENT;
-    if (int rc = zero_rows(gate_up, 2 * hidden, rows, 2 * hidden, stream)) return rc;
+    if (int rc = zero_rows(gate_up, 2 * hp, rows, 2 * hp, stream)) return rc;
     return zero_rows(y, ldy, rows, out_dim, stream);
   }
   if (!x || !w_in || !w_out || !y || ldx < dim || ldw_in < dim || ldw_out < hidden || ldy < out_dim)
     return B200_ERR_INVALID_ARGUMENT;
-  if (!pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) || !pitch_ok(y, ldy) ||
-      (gate_up && !aligned16(gate_up)))
-    return B200_ERR_MISALIGNED;
-  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, hidden, 0)))
+  if (gate_up && !aligned16(gate_up)) return B200_ERR_MISALIGNED;
+  const bool few = few_rows(rows, dim, hidden) && !gate_up;
+  const bool copies = !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) || !pitch_ok(y, ldy);
+  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, dim, hidden, out_dim, 0, copies)))
     return B200_ERR_WORKSPACE;
   DeviceInfo dev;
   if (int rc = current_device_info(dev)) return rc;
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
   const bool bf16 = dtype == B200_DTYPE_BF16;
-  uint16_t* a = static_cast<uint16_t*>(workspace);
-  const GateShape s{(int)rows, (int)hidden, (int)dim};
-  if (few_rows(rows, dim, hidden) && !gate_up) {
+  Carver ws{static_cast<uint8_t*>(workspace)};
+  CopyJobs before, after;
+  uint16_t* a = ws.take(rows, hp);
+  x = readable(x, ldx, rows, dim, ws, before);
+  w_in = readable(w_in, ldw_in, 2 * hidden, dim, ws, before);
+  w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
+  if (int rc = run_copies(before, stream)) return rc;
+  if (few) {
     const int rc = (bf16 ? launch_rows<true, true> : launch_rows<false, true>)(
-        x, ldx, w_in, ldw_in, a, hidden, (int)rows, (int)hidden, (int)dim, activation, false, dev, stream);
+        x, ldx, w_in, ldw_in, a, hp, (int)rows, (int)hidden, (int)dim, activation, false, dev, stream);
     if (rc) return rc;
+    // w_out was written two kernels ago at the latest: its loads may start early.
     return (bf16 ? launch_rows<true, false> : launch_rows<false, false>)(
-        a, hidden, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim, (int)hidden, 0, true, dev, stream);
+        a, hp, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim, (int)hidden, 0, true, dev, stream);
   }
-  const int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(x, ldx, w_in, ldw_in, a,
-                                                                     static_cast<uint16_t*>(gate_up), activation, s,
-                                                                     stream);
+  const GateShape s{(int)rows, (int)hidden, (int)dim, (int)hp};
+  int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(x, ldx, w_in, ldw_in, a,
+                                                               static_cast<uint16_t*>(gate_up), activation, s, stream);
   if (rc) return rc;
-  return plain_gemm(bf16, a, w_out, y, rows, out_dim, hidden, hidden, ldw_out, ldy, B200_A_ROW_MAJOR, B200_B_COL_MAJOR,
-                    stream_ptr);
+  y = writable(y, ldy, rows, out_dim, ws, after);
+  rc = plain_gemm(bf16, a, w_out, y, rows, out_dim, hidden, hp, ldw_out, ldy, B200_A_ROW_MAJOR, B200_B_COL_MAJOR,
+                  stream_ptr);
+  return rc ? rc : run_copies(after, stream);
 }
 
 extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_in, const void* w_out,
@@ -316,34 +427,64 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
   }
   if (!dy || !x || !w_in || !w_out || !gate_up || lddy < out_dim || ldx < dim || ldw_in < dim || ldw_out < hidden)
     return B200_ERR_INVALID_ARGUMENT;
-  if (!pitch_ok(dy, lddy) || !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) ||
-      !aligned16(gate_up) || (dx && !pitch_ok(dx, lddx)) || (dw_in && !pitch_ok(dw_in, lddw_in)) ||
-      (dw_out && !pitch_ok(dw_out, lddw_out)))
-    return B200_ERR_MISALIGNED;
-  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, hidden, 1)))
+  if (!aligned16(gate_up)) return B200_ERR_MISALIGNED;
+  const bool copies = !pitch_ok(dy, lddy) || !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) ||
+                      !pitch_ok(w_out, ldw_out) || (dx && !pitch_ok(dx, lddx)) ||
+                      (dw_in && !pitch_ok(dw_in, lddw_in)) || (dw_out && !pitch_ok(dw_out, lddw_out));
+  if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, dim, hidden, out_dim, 1, copies)))
     return B200_ERR_WORKSPACE;
   DeviceInfo dev;
   if (int rc = current_device_info(dev)) return rc;
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
   const bool bf16 = dtype == B200_DTYPE_BF16;
-  uint16_t* dgu = static_cast<uint16_t*>(workspace);
-  uint16_t* a = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + part_bytes(rows, 2 * hidden));
-  const GateShape s{(int)rows, (int)hidden, (int)out_dim};
+  const int64_t hp = pad8(hidden);
+  Carver ws{static_cast<uint8_t*>(workspace)};
+  CopyJobs before, after;
+  uint16_t* a = ws.take(rows, hp);
+  uint16_t* dgu = ws.take(rows, 2 * hp);
+  dy = readable(dy, lddy, rows, out_dim, ws, before);
+  w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
+  if (dw_in) x = readable(x, ldx, rows, dim, ws, before);
+  if (dx) {
+    if (hidden == hp) {
+      w_in = readable(w_in, ldw_in, 2 * hidden, dim, ws, before);
+    } else {
+      // dx sums over the padded rows of [dg du]: w_in with zero rows in their places.
+      uint16_t* copy = ws.take(2 * hp, dim);
+      const uint16_t* src = static_cast<const uint16_t*>(w_in);
+      for (int half = 0; half < 2; ++half)
+        before.add(src + half * hidden * ldw_in, ldw_in, copy + half * hp * pad8(dim), pad8(dim), hidden, dim,
+                   pad8(dim), hp - hidden);
+      w_in = copy;
+      ldw_in = pad8(dim);
+    }
+  }
+  if (int rc = run_copies(before, stream)) return rc;
+  const GateShape s{(int)rows, (int)hidden, (int)out_dim, (int)hp};
   int rc = (bf16 ? gate_bwd<true> : gate_bwd<false>)(dy, lddy, w_out, ldw_out, static_cast<const uint16_t*>(gate_up),
                                                      dgu, a, activation, s, stream);
   if (rc) return rc;
   if (dx) {
-    rc = plain_gemm(bf16, dgu, w_in, dx, rows, dim, 2 * hidden, 2 * hidden, ldw_in, lddx, B200_A_ROW_MAJOR,
-                    B200_B_ROW_MAJOR, stream_ptr);
+    dx = writable(dx, lddx, rows, dim, ws, after);
+    rc = plain_gemm(bf16, dgu, w_in, dx, rows, dim, 2 * hp, 2 * hp, ldw_in, lddx, B200_A_ROW_MAJOR, B200_B_ROW_MAJOR,
+                    stream_ptr);
     if (rc) return rc;
   }
   if (dw_in) {
-    rc = plain_gemm(bf16, dgu, x, dw_in, 2 * hidden, dim, rows, 2 * hidden, ldx, lddw_in, B200_A_COL_MAJOR,
+    uint16_t* out = static_cast<uint16_t*>(writable(dw_in, lddw_in, 2 * hidden, dim, ws, after));
+    // One product when the halves of [dg du] follow one another, else one for each.
+    const int parts = hidden == hp ? 1 : 2;
+    for (int half = 0; half < parts; ++half) {
+      rc = plain_gemm(bf16, dgu + half * hp, x, out + half * hidden * lddw_in, 2 * hidden / parts, dim, rows, 2 * hp,
+                      ldx, lddw_in, B200_A_COL_MAJOR, B200_B_ROW_MAJOR, stream_ptr);
+      if (rc) return rc;
+    }
+  }
+  if (dw_out) {
+    dw_out = writable(dw_out, lddw_out, out_dim, hidden, ws, after);
+    rc = plain_gemm(bf16, dy, a, dw_out, out_dim, hidden, rows, lddy, hp, lddw_out, B200_A_COL_MAJOR,
                     B200_B_ROW_MAJOR, stream_ptr);
     if (rc) return rc;
   }
-  if (dw_out)
-    rc = plain_gemm(bf16, dy, a, dw_out, out_dim, hidden, rows, lddy, hidden, lddw_out, B200_A_COL_MAJOR,
-                    B200_B_ROW_MAJOR, stream_ptr);
-  return rc;
+  return run_copies(after, stream);
 }

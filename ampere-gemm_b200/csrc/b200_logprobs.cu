@@ -264,7 +264,7 @@ __device__ __forceinline__ unsigned long long block_bound(unsigned long long key
 struct Outputs {
   float* logprob;
   float* entropy;
-  float2* stats;       // m, ln z
+  float2* stats;       // m, ln z (may be NULL)
   float* top_logprob;  // rows x top
   int64_t* top_index;
 };
@@ -274,7 +274,7 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
                                           int64_t ignore, Sums s) {
   const bool empty = s.m == kNegInf;
   const float ln_z = logf(s.z);
-  out.stats[row] = make_float2(s.m, ln_z);
+  if (out.stats) out.stats[row] = make_float2(s.m, ln_z);
   out.entropy[row] = empty ? 0.0f : ln_z - s.w / s.z;
   float lp = 0.0f;
   if (target != ignore) {
@@ -600,7 +600,7 @@ extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* target
     return B200_ERR_INVALID_ARGUMENT;
   if (vocab > (top > 0 ? kMaxTopVocab : 0x7fffffff)) return B200_ERR_TOO_LARGE;
   if (rows == 0) return B200_OK;
-  if (vocab == 0 || !logits || !targets || !logprob || !entropy || !stats || ld < vocab ||
+  if (vocab == 0 || !logits || !targets || !logprob || !entropy || ld < vocab ||
       (top > 0 && (!top_logprob || !top_index)))
     return B200_ERR_INVALID_ARGUMENT;
   const int64_t need = b200_token_logprobs_workspace_size(rows, vocab, top);

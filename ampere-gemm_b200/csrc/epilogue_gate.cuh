@@ -28,10 +28,12 @@ struct FusedArgs<kEpiGateUp> {
 
 template <>
 struct FusedArgs<kEpiGateBwd> {
-  CUtensorMap tmap_dg, tmap_du, tmap_a;
   const uint16_t* g = nullptr;  // the saved g and u, row pitch ld (elements)
   const uint16_t* u = nullptr;
-  int64_t ld = 0;
+  uint16_t* dg = nullptr;       // their gradients, the same pitch
+  uint16_t* du = nullptr;
+  uint16_t* a = nullptr;
+  int64_t ld = 0, ld_a = 0;
   int activation = 0;
 };
 
@@ -128,10 +130,18 @@ __device__ __forceinline__ void gate_up_epilogue(const FusedArgs<kEpiGateUp>& fx
     gate_up_chunks<kBf16, 2>(fx, tmap_c, sc, t_row, epi_buf, epi_addr, sbuf, lane, n0, y, release);
 }
 
+// Keeps the first `n` of a piece's eight elements (n <= 0: none), zeroes the others.
+__device__ __forceinline__ uint4 keep_first(uint4 v, int n) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = n >= 2 * i + 2 ? w[i] : n == 2 * i + 1 ? (w[i] & 0xffffu) : 0u;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Reads the 32 x 64 blocks of the saved g and u at column x, row y: lane l
 // takes 16-byte piece l % 8 of rows l / 8, l / 8 + 4, ... (whole 128-byte row
-// pieces per instruction).  N is a multiple of 8, so a piece is in or out as a
-// whole; pieces out of range read as 0.
+// pieces per instruction).  Their rows are padded to whole pieces; what lies
+// past column N, or in pieces out of range, counts as 0.
 __device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx, uint4 (&g)[8], uint4 (&u)[8],
                                                int lane, int x, int y, int M, int N) {
   const int col = x + (lane & 7) * 8;
@@ -143,15 +153,34 @@ __device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx,
       const int64_t off = static_cast<int64_t>(row) * fx.ld + col;
       g[i] = *reinterpret_cast<const uint4*>(fx.g + off);
       u[i] = *reinterpret_cast<const uint4*>(fx.u + off);
+      if (col + 8 > N) {
+        g[i] = keep_first(g[i], N - col);
+        u[i] = keep_first(u[i], N - col);
+      }
     }
+  }
+}
+
+// Stores the 32 x 64 block staged at `buf` (row r at r * 128, 16-byte pieces
+// swizzled) to column x, row y: the mapping of gate_bwd_fetch.
+__device__ __forceinline__ void gate_bwd_store(const uint8_t* buf, uint16_t* out, int64_t ld, int lane, int x, int y,
+                                               int M, int N) {
+  const int col = x + (lane & 7) * 8;
+  if (col >= N) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    if (y + r < M)
+      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(y + r) * ld + col) =
+          *reinterpret_cast<const uint4*>(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
   }
 }
 
 // Backward: the accumulator row holds da at columns [n0, n0 + 256).  Per 64
 // columns, g and u go through the warp's two staging buffers into the layout
 // of the accumulator (lane = row), dg and du replace them there and leave by
-// TMA, then a takes the first buffer.  The next block's g and u are fetched
-// meanwhile.
+// plain stores of whole 128-byte row pieces (zeros past column N), then a takes
+// the first buffer.  The next block's g and u are fetched meanwhile.
 template <bool kBf16, int kAct, typename Release>
 __device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[8], uint4 (&uv)[8],
                                                 uint32_t t_row, uint8_t* epi_buf, int lane, int n0, int y, int M,
@@ -168,8 +197,6 @@ __device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx
     tmem_ld_wait_regs(hi);
     if (c == 3) release();
     if (x >= N) continue;
-    if (lane == 0) bulk_wait_group_read<0>();
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = i * 4 + (lane >> 3);
@@ -200,25 +227,17 @@ __device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx
       *reinterpret_cast<uint4*>(buf0 + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
       *reinterpret_cast<uint4*>(buf1 + at) = make_uint4(du[0], du[1], du[2], du[3]);
     }
-    fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(&fx.tmap_dg, buf0, x, y);
-      tma_store_2d(&fx.tmap_du, buf1, x, y);
-      bulk_commit_group();
-      bulk_wait_group_read<0>();
-    }
+    gate_bwd_store(buf0, fx.dg, fx.ld, lane, x, y, M, N);
+    gate_bwd_store(buf1, fx.du, fx.ld, lane, x, y, M, N);
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       *reinterpret_cast<uint4*>(buf0 + lane * 128 + ((j ^ (lane & 7)) << 4)) =
           make_uint4(pa[4 * j], pa[4 * j + 1], pa[4 * j + 2], pa[4 * j + 3]);
-    fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(&fx.tmap_a, buf0, x, y);
-      bulk_commit_group();
-    }
+    gate_bwd_store(buf0, fx.a, fx.ld_a, lane, x, y, M, N);
+    __syncwarp();
   }
 }
 

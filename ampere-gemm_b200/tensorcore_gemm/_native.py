@@ -120,7 +120,7 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_void_p] * 7 + [ctypes.c_int64] * 5 + [ctypes.c_int, ctypes.c_void_p],
     ),
-    "b200_gated_ffn_workspace_size": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "b200_gated_ffn_workspace_size": (ctypes.c_int64, [ctypes.c_int64] * 4 + [ctypes.c_int] * 2),
     "b200_gated_ffn_fwd": (
         ctypes.c_int,
         [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 8 +

@@ -45,89 +45,50 @@ def _pad8(n: int) -> int:
     return -(-n // 8) * 8
 
 
-def _pitched(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """`t` as a matrix that TMA can read (unit column stride, 16-byte aligned
-    base and pitch) and its pitch; copied only when it is not one already."""
-    t, ld = as_rows(t)
-    if ld % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, ld
-    rows, cols = t.shape
-    if rows == 1 and t.data_ptr() % 16 == 0:
-        return t, _pad8(cols)                   # one row: its pitch is never used
-    buf = torch.empty((rows, _pad8(cols)), dtype=t.dtype, device=t.device)
-    buf[:, :cols].copy_(t)
-    return buf, buf.shape[1]
-
-
-def _padded_weights(w_in, w_out):
-    """The weights with a hidden width that is a multiple of 8: zero rows after
-    the gate's and after the up projection's, zero columns in w_out.  The
-    hidden units added are 0 throughout."""
-    f = w_out.shape[1]
-    fp = _pad8(f)
-    if fp == f:
-        return w_in, w_out
-    wi = w_in.new_zeros((2, fp, w_in.shape[1]))
-    wi[:, :f].copy_(w_in.reshape(2, f, w_in.shape[1]))
-    wo = w_out.new_zeros((w_out.shape[0], fp))
-    wo[:, :f].copy_(w_out)
-    return wi.view(2 * fp, -1), wo
-
-
-def _result(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
-    """A matrix for the kernels to write: dense when its rows start on 16 bytes, else with padded rows."""
-    buf = torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device)
-    return buf[:, :cols]
+def _unaligned(*operands) -> int:
+    """1 when the rows of some (matrix, pitch) do not start on 16 bytes."""
+    return int(any(ld % 8 or t.data_ptr() % 16 for t, ld in operands))
 
 
 def _forward(x, w_in, w_out, activation: str, save: bool):
-    """y, and with `save` [g u] (rows x 2 hidden, hidden rounded up to 8) for the backward pass."""
-    dim, out_dim = x.shape[-1], w_out.shape[0]
+    """y, and with `save` [g u] (rows x 2 hidden, each half padded to a multiple of 8) for the backward pass."""
+    dim, (out_dim, hidden) = x.shape[-1], w_out.shape
     rows = x.numel() // dim if dim else x.shape[:-1].numel()
-    w_in, w_out = _padded_weights(w_in, w_out)
-    hidden = w_out.shape[1]
-    gate_up = torch.empty((rows, 2 * hidden), dtype=x.dtype, device=x.device) if save else None
+    gate_up = torch.empty((rows, 2 * _pad8(hidden)), dtype=x.dtype, device=x.device) if save else None
     if rows == 0 or out_dim == 0 or dim == 0 or hidden == 0:
         return x.new_zeros((*x.shape[:-1], out_dim)), gate_up
-    x2, ldx = _pitched(x)
-    wi, ldi = _pitched(w_in)
-    wo, ldo = _pitched(w_out)
-    y = _result(rows, out_dim, x)
-    ws_bytes = _native.load().b200_gated_ffn_workspace_size(rows, hidden, 0)
+    x2, ldx = as_rows(x)
+    wi, ldi = as_rows(w_in)
+    wo, ldo = as_rows(w_out)
+    y = torch.empty((*x.shape[:-1], out_dim), dtype=x.dtype, device=x.device)
+    ws_bytes = _native.load().b200_gated_ffn_workspace_size(
+        rows, dim, hidden, out_dim, 0, _unaligned((x2, ldx), (wi, ldi), (wo, ldo), (y, out_dim)))
     ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
     launch("b200_gated_ffn_fwd", x.get_device(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr(),
-           ptr(gate_up), rows, dim, hidden, out_dim, ldx, ldi, ldo, _pad8(out_dim), ACTIVATIONS[activation],
+           ptr(gate_up), rows, dim, hidden, out_dim, ldx, ldi, ldo, out_dim, ACTIVATIONS[activation],
            DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
-    return y.contiguous().view(*x.shape[:-1], out_dim), gate_up
+    return y, gate_up
 
 
 def _backward(dy, x, w_in, w_out, gate_up, activation: str, need_x: bool, need_in: bool, need_out: bool):
     """dx, dw_in and dw_out (None where not needed)."""
-    dim, (out_dim, f) = x.shape[-1], w_out.shape
+    dim, (out_dim, hidden) = x.shape[-1], w_out.shape
     rows = gate_up.shape[0]
-    if rows == 0 or out_dim == 0 or dim == 0 or f == 0:
-        return (torch.zeros_like(x, memory_format=torch.contiguous_format) if need_x else None,
-                w_in.new_zeros(w_in.shape) if need_in else None, w_out.new_zeros(w_out.shape) if need_out else None)
-    wi, wo = _padded_weights(w_in, w_out)
-    hidden = wo.shape[1]
-    dy2, lddy = _pitched(dy)
-    x2, ldx = _pitched(x)
-    wi, ldi = _pitched(wi)
-    wo, ldo = _pitched(wo)
-    dx = _result(rows, dim, x) if need_x else None
-    dwi = _result(2 * hidden, dim, x) if need_in else None
-    dwo = _result(out_dim, hidden, x) if need_out else None
-    ws_bytes = _native.load().b200_gated_ffn_workspace_size(rows, hidden, 1)
+    new = torch.zeros_like if rows == 0 or out_dim == 0 or dim == 0 or hidden == 0 else torch.empty_like
+    dx, dwi, dwo = (new(t, memory_format=torch.contiguous_format) if need else None
+                    for t, need in ((x, need_x), (w_in, need_in), (w_out, need_out)))
+    if new is torch.zeros_like:
+        return dx, dwi, dwo
+    dy2, lddy = as_rows(dy)
+    x2, ldx = as_rows(x)
+    wi, ldi = as_rows(w_in)
+    wo, ldo = as_rows(w_out)
+    ws_bytes = _native.load().b200_gated_ffn_workspace_size(
+        rows, dim, hidden, out_dim, 1, _unaligned((dy2, lddy), (x2, ldx), (wi, ldi), (wo, ldo)))
     ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
     launch("b200_gated_ffn_bwd", x.get_device(), dy2.data_ptr(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(),
-           gate_up.data_ptr(), ptr(dx), ptr(dwi), ptr(dwo), rows, dim, hidden, out_dim, lddy, ldx, ldi, ldo,
-           _pad8(dim), _pad8(dim), hidden, ACTIVATIONS[activation], DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
-    if need_x:
-        dx = dx.contiguous().view(x.shape)
-    if need_in:
-        dwi = dwi.contiguous() if hidden == f else dwi.unflatten(0, (2, hidden))[:, :f].reshape(2 * f, dim)
-    if need_out:
-        dwo = dwo[:, :f].contiguous()
+           gate_up.data_ptr(), ptr(dx), ptr(dwi), ptr(dwo), rows, dim, hidden, out_dim, lddy, ldx, ldi, ldo, dim, dim,
+           hidden, ACTIVATIONS[activation], DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
     return dx, dwi, dwo
 
 
@@ -149,8 +110,8 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
     """y = (act(x Wg^T) * (x Wu^T)) w_out^T for x (..., D), w_in = [Wg; Wu] (2F x D) and w_out (N x F).
 
     All float16 or all bfloat16.  activation: "silu", "gelu" or "gelu_tanh".
-    Any sizes and strides; operands whose rows do not start on 16 bytes, and
-    weights whose F is not a multiple of 8, are copied first.  Differentiable
+    Any sizes and strides; operands whose rows do not start on 16 bytes are
+    copied first.  Differentiable
     in x, w_in and w_out (once).  a = act(g) u (and, for the backward pass, g
     and u) are rounded to x's type.
     """

@@ -46,32 +46,38 @@ def _check(logits, targets, top_k: int) -> None:
         raise RuntimeError(f"top_k must be between 0 and {min(MAX_TOP, logits.shape[-1])}")
 
 
-def _forward(logits, targets, top_k: int, ignore_index: int):
-    """logprobs, entropy, stats (..., 2), top_logprobs and top_indices (..., top_k)."""
+def _targets(t):
+    return t.contiguous() if t.dtype == torch.int64 else t.to(torch.int64).contiguous()
+
+
+def _forward(logits, targets, top_k: int, ignore_index: int, stats: bool = True):
+    """logprobs, entropy, stats (..., 2) for the backward pass, top_logprobs and top_indices (..., top_k).
+
+    None in the place of stats when they are not wanted, and of the last two for top_k = 0."""
     shape, dev = targets.shape, logits.device
     logprob = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-    stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev)
-    top_logprob = torch.empty((*shape, top_k), dtype=torch.float32, device=dev)
-    top_index = torch.empty((*shape, top_k), dtype=torch.int64, device=dev)
+    entropy = torch.empty_like(logprob)
+    stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev) if stats else None
+    top_logprob = torch.empty((*shape, top_k), dtype=torch.float32, device=dev) if top_k else None
+    top_index = torch.empty((*shape, top_k), dtype=torch.int64, device=dev) if top_k else None
     rows, vocab = targets.numel(), logits.shape[-1]
     if rows:
         x, ld = as_rows(logits)
-        t = targets.to(torch.int64).contiguous()
+        t = _targets(targets)
         ws_bytes = _native.load().b200_token_logprobs_workspace_size(rows, vocab, top_k)
         ws = workspace(ws_bytes, dev, "b200_token_logprobs_workspace_size")
         launch("b200_token_logprobs_fwd", logits.get_device(), x.data_ptr(), t.data_ptr(), logprob.data_ptr(),
-               entropy.data_ptr(), stats.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), rows, vocab, ld,
-               top_k, ignore_index, DTYPE_CODES[logits.dtype], ptr(ws), ws_bytes)
+               entropy.data_ptr(), ptr(stats), ptr(top_logprob), ptr(top_index), rows, vocab, ld, top_k,
+               ignore_index, DTYPE_CODES[logits.dtype], ptr(ws), ws_bytes)
     return logprob, entropy, stats, top_logprob, top_index
 
 
 def _backward(logits, targets, stats, entropy, g_logprob, g_entropy, ignore_index: int):
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d = torch.empty_like(logits, memory_format=torch.contiguous_format)
     rows, vocab = targets.numel(), logits.shape[-1]
     if rows:
         x, ld = as_rows(logits)
-        t = targets.to(torch.int64).contiguous()
+        t = _targets(targets)
         gl = None if g_logprob is None else g_logprob.contiguous()
         gh = None if g_entropy is None else g_entropy.contiguous()
         launch("b200_token_logprobs_bwd", logits.get_device(), x.data_ptr(), t.data_ptr(), stats.data_ptr(),
@@ -87,7 +93,8 @@ class _TokenLogprobs(torch.autograd.Function):
         logprob, entropy, stats, top_logprob, top_index = _forward(logits, targets, top_k, ignore_index)
         ctx.save_for_backward(logits, targets, stats, entropy)
         ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(top_logprob, top_index)
+        if top_k:
+            ctx.mark_non_differentiable(top_logprob, top_index)
         return logprob, entropy, top_logprob, top_index
 
     @staticmethod
@@ -117,7 +124,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
         if wants_grad(logits):
             lp, ent, tv, ti = _TokenLogprobs.apply(logits, targets, top_k, ignore_index)
         else:
-            lp, ent, _, tv, ti = _forward(logits, targets, top_k, ignore_index)
+            lp, ent, _, tv, ti = _forward(logits, targets, top_k, ignore_index, False)
     return TokenLogprobs(lp, ent, tv if top_k else None, ti if top_k else None)
 
 
@@ -130,7 +137,10 @@ def _token_logprobs_op(
         ignore_index: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """logprobs, entropy, stats, top_logprobs, top_indices (the last three are not differentiable)."""
     _check(logits, targets, top_k)
-    return _forward(logits, targets, top_k, ignore_index)
+    lp, ent, stats, tv, ti = _forward(logits, targets, top_k, ignore_index)
+    if not top_k:
+        tv, ti = (torch.empty((*targets.shape, 0), dtype=d, device=logits.device) for d in (torch.float32, torch.int64))
+    return lp, ent, stats, tv, ti
 
 
 @_token_logprobs_op.register_fake

@@ -43,13 +43,13 @@ def _wdtype(x, weight, bias):
 
 def _forward(x, weight, bias, eps: float, stats: bool):
     """y, and with `stats` the rows' mean and 1 / standard deviation (fp32)."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
     mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
     if rows:
         x2, ldx = as_rows(x)
-        cols = x.shape[-1]
         weight = None if weight is None else weight.contiguous()
         bias = None if bias is None else bias.contiguous()
         launch("b200_layer_norm_fwd", x.get_device(), x2.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), ptr(mean),
@@ -60,7 +60,7 @@ def _forward(x, weight, bias, eps: float, stats: bool):
 def _backward(dy, x, weight, mean, rstd, wdtype, need_weight: bool, need_bias: bool):
     """dx, dweight and dbias (None where not needed)."""
     cols = x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = torch.empty(cols, dtype=wdtype, device=x.device) if need_weight else None
     db = torch.empty(cols, dtype=wdtype, device=x.device) if need_bias else None
     if cols:

@@ -221,7 +221,7 @@ B200_API int b200_layer_norm_bwd(const void* dy, const void* x, const void* w, c
  * all).  A target equal to ignore_index gives logprob 0; any other target
  * outside [0, vocab) gives NaN.  A row of -inf throughout gives logprob -inf
  * and entropy 0.  vocab is at most 2^31 - 1, with alternatives 2^24.  stats
- * (rows x 2 floats) receives the row's maximum and
+ * (rows x 2 floats, may be NULL) receives the row's maximum and
  * ln(sum exp(x - max)), which the backward call reads.  The workspace
  * (b200_token_logprobs_workspace_size bytes, may be 0; 256-byte aligned)
  * holds the parts of rows that several blocks share.  No counterpart in the
@@ -250,18 +250,19 @@ B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets,
  *   g = x Wg^T, u = x Wu^T, a = act(g) u, y = a w_out^T
  * for `rows` rows of x, all of `dtype` (B200_DTYPE_F16 or B200_DTYPE_BF16) with
  * fp32 accumulation and activation; a is rounded to `dtype` between the two
- * launches.  gate_up (rows x 2 hidden, dense; may be NULL) receives [g u] for
- * the backward call.  Operands as for b200_gemm_f16 (16-byte bases, pitches a
- * multiple of 8 elements), and hidden a multiple of 8: B200_ERR_MISALIGNED
- * otherwise.  The workspace (b200_gated_ffn_workspace_size bytes, 256-byte
- * aligned) holds a, in the backward also dg and du; it must not be reused
- * until the call's work on `stream` has finished.  No counterpart in the
- * reference.
+ * launches.  gate_up (may be NULL) receives g and u for the backward call: rows
+ * of 2 P elements, P = hidden rounded up to a multiple of 8, 16-byte aligned.
+ * Other operands are taken at any alignment and pitch; those whose rows do not
+ * start on 16 bytes cost a copy.  The workspace (256-byte aligned) must not be
+ * reused until the call's work on `stream` has finished; its size is
+ * b200_gated_ffn_workspace_size(), with `unaligned` != 0 when the rows of any
+ * operand do not start on 16 bytes.  No counterpart in the reference.
  */
 #define B200_ACT_SILU 0      /* g / (1 + exp(-g)) */
 #define B200_ACT_GELU 1      /* g Phi(g), Phi the normal distribution function */
 #define B200_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
-B200_API int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t hidden, int backward);
+B200_API int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim,
+                                               int backward, int unaligned);
 B200_API int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w_out, void* y, void* gate_up,
                                 int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int64_t ldx,
                                 int64_t ldw_in, int64_t ldw_out, int64_t ldy, int activation, int dtype,

@@ -315,15 +315,16 @@ def test_c_argument_checks_without_gpu(native_lib):
     size, fwd, bwd = (native_lib.b200_gated_ffn_workspace_size, native_lib.b200_gated_ffn_fwd,
                       native_lib.b200_gated_ffn_bwd)
     p = 4096
-    assert size(-1, 8, 0) == -1 and size(4, 64, 0) == 512 and size(4, 64, 1) == 512 + 1024
+    assert size(-1, 8, 8, 8, 0, 0) == -1 and size(4, 64, 64, 64, 0, 0) == 512 and size(4, 64, 64, 64, 1, 0) == 1536
+    assert size(4, 64, 64, 1 << 31, 0, 0) == -3 and size(4, 64, 60, 64, 0, 0) > 512 and size(4, 64, 64, 64, 0, 1) > 512
     args = [p] * 5 + [4, 64, 64, 64, 64, 64, 64, 64, 0, 1, p, 1 << 20, None]
     def with_(a, i, v):
         return [v if j == i else q for j, q in enumerate(a)]
-    for i, v, code in [(0, None, 1), (1, None, 1), (2, None, 1), (3, None, 1), (5, -1, 1), (5, 1 << 31, 3), (7, 63, 2),
-                       (9, 63, 1), (9, 68, 2), (12, 60, 1), (13, 3, 1), (14, 2, 1), (15, None, 8), (15, p + 8, 8),
-                       (16, 511, 8), (0, p + 2, 2), (4, p + 2, 2)]:
+    for i, v, code in [(0, None, 1), (1, None, 1), (2, None, 1), (3, None, 1), (5, -1, 1), (5, 1 << 31, 3), (7, -1, 1),
+                       (9, 63, 1), (12, 60, 1), (13, 3, 1), (14, 2, 1), (15, None, 8), (15, p + 8, 8),
+                       (16, 511, 8), (4, p + 2, 2)]:
         assert fwd(*with_(args, i, v)) == code, (i, v)
     args = [p] * 8 + [4, 64, 64, 64] + [64] * 7 + [0, 1, p, 1 << 20, None]
-    for i, v, code in [(0, None, 1), (4, None, 1), (4, p + 2, 2), (5, p + 2, 2), (16, 63, 1), (16, 68, 2), (18, 60, 1),
+    for i, v, code in [(0, None, 1), (4, None, 1), (4, p + 2, 2), (16, 63, 1), (18, 60, 1),
                        (21, p + 8, 8), (22, 1535, 8)]:
         assert bwd(*with_(args, i, v)) == code, (i, v)

@@ -340,7 +340,7 @@ def test_c_argument_checks_without_gpu(native_lib):
     args = [p] * 7 + [4, 100, 100, 2, -100, 0, None, 0, None]
     def with_(i, v):
         return [v if j == i else a for j, a in enumerate(args)]
-    for i, v in [(0, None), (1, None), (2, None), (3, None), (4, None), (5, None), (7, -1), (8, 0), (9, 99), (10, 65), (12, 3)]:
+    for i, v in [(0, None), (1, None), (2, None), (3, None), (5, None), (6, None), (7, -1), (8, 0), (9, 99), (10, 65), (12, 3)]:
         assert fwd(*with_(i, v)) == 1, i
     assert fwd(*with_(8, 1 << 31)) == 3
     assert fwd(*with_(7, 0)) == 0
