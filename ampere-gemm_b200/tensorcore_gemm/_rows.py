@@ -29,15 +29,22 @@ def as_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
 
     A row-strided view (a column slice) is used in place; anything else, an
     expanded tensor among them, is made contiguous."""
-    cols = t.shape[-1]
     if t.dim() != 2:
+        cols = t.shape[-1]
         t = t.reshape(-1, cols) if cols else t.reshape(0, 0)
-    if t.stride(1) == 1 or cols <= 1:
-        if t.shape[0] <= 1:
-            return t, max(1, cols)
-        if t.stride(0) >= max(1, cols):
-            return t, t.stride(0)
-    return t.contiguous(), max(1, cols)
+    rows, cols = t.shape
+    if cols <= 1:
+        cols = 1
+        if rows <= 1 or t.stride(0) >= 1:
+            return t, cols if rows <= 1 else t.stride(0)
+    else:
+        pitch, unit = t.stride()
+        if unit == 1:
+            if rows <= 1:
+                return t, cols
+            if pitch >= cols:
+                return t, pitch
+    return t.contiguous(), cols
 
 
 def workspace(nbytes: int, device: torch.device, what: str) -> torch.Tensor | None:
@@ -52,9 +59,14 @@ def ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+_FUNCTIONS: dict = {}
+
+
 def launch(name: str, dev: int, *args) -> None:
     """Calls C entry point `name` with `args` and the current stream of device `dev`; raises on an error code."""
-    fn = getattr(_native.load(), name)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_native.load(), name)
     if dev != _GET_DEVICE():
         with torch.cuda.device(dev):
             code = fn(*args, _current_stream(dev))
@@ -98,11 +110,10 @@ def once_differentiable(backward):
 
     @functools.wraps(backward)
     def wrapper(ctx, *grads):
-        again = torch.is_grad_enabled()          # create_graph=True
+        if not torch.is_grad_enabled():          # the usual case: no create_graph=True
+            return backward(ctx, *grads)
         with torch.no_grad():
             out = backward(ctx, *grads)
-        if not again:
-            return out
         at = [i for i, t in enumerate(out) if t is not None]
         refused = _Refuse.apply(*(out[i].detach().requires_grad_() for i in at)) if at else ()
         out = list(out)

@@ -45,9 +45,9 @@ def _pad8(n: int) -> int:
     return -(-n // 8) * 8
 
 
-def _unaligned(*operands) -> int:
-    """1 when the rows of some (matrix, pitch) do not start on 16 bytes."""
-    return int(any(ld % 8 or t.data_ptr() % 16 for t, ld in operands))
+def _unaligned(pointers: int, pitches: int) -> int:
+    """1 when the rows of some operand do not start on 16 bytes, from the operands' addresses and pitches or-ed."""
+    return 1 if pointers % 16 or pitches % 8 else 0
 
 
 def _forward(x, w_in, w_out, activation: str, save: bool):
@@ -61,12 +61,12 @@ def _forward(x, w_in, w_out, activation: str, save: bool):
     wi, ldi = as_rows(w_in)
     wo, ldo = as_rows(w_out)
     y = torch.empty((*x.shape[:-1], out_dim), dtype=x.dtype, device=x.device)
+    xp, wip, wop, yp = x2.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr()
     ws_bytes = _native.load().b200_gated_ffn_workspace_size(
-        rows, dim, hidden, out_dim, 0, _unaligned((x2, ldx), (wi, ldi), (wo, ldo), (y, out_dim)))
+        rows, dim, hidden, out_dim, 0, _unaligned(xp | wip | wop | yp, ldx | ldi | ldo | out_dim))
     ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
-    launch("b200_gated_ffn_fwd", x.get_device(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr(),
-           ptr(gate_up), rows, dim, hidden, out_dim, ldx, ldi, ldo, out_dim, ACTIVATIONS[activation],
-           DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
+    launch("b200_gated_ffn_fwd", x.get_device(), xp, wip, wop, yp, ptr(gate_up), rows, dim, hidden,
+           out_dim, ldx, ldi, ldo, out_dim, ACTIVATIONS[activation], DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
     return y, gate_up
 
 
@@ -83,12 +83,13 @@ def _backward(dy, x, w_in, w_out, gate_up, activation: str, need_x: bool, need_i
     x2, ldx = as_rows(x)
     wi, ldi = as_rows(w_in)
     wo, ldo = as_rows(w_out)
+    dyp, xp, wip, wop = dy2.data_ptr(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr()
     ws_bytes = _native.load().b200_gated_ffn_workspace_size(
-        rows, dim, hidden, out_dim, 1, _unaligned((dy2, lddy), (x2, ldx), (wi, ldi), (wo, ldo)))
+        rows, dim, hidden, out_dim, 1, _unaligned(dyp | xp | wip | wop, lddy | ldx | ldi | ldo))
     ws = workspace(ws_bytes, x.device, "b200_gated_ffn_workspace_size")
-    launch("b200_gated_ffn_bwd", x.get_device(), dy2.data_ptr(), x2.data_ptr(), wi.data_ptr(), wo.data_ptr(),
-           gate_up.data_ptr(), ptr(dx), ptr(dwi), ptr(dwo), rows, dim, hidden, out_dim, lddy, ldx, ldi, ldo, dim, dim,
-           hidden, ACTIVATIONS[activation], DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
+    launch("b200_gated_ffn_bwd", x.get_device(), dyp, xp, wip, wop, gate_up.data_ptr(), ptr(dx), ptr(dwi), ptr(dwo),
+           rows, dim, hidden, out_dim, lddy, ldx, ldi, ldo, dim, dim, hidden, ACTIVATIONS[activation],
+           DTYPE_CODES[x.dtype], ptr(ws), ws_bytes)
     return dx, dwi, dwo
 
 
@@ -111,9 +112,8 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
 
     All float16 or all bfloat16.  activation: "silu", "gelu" or "gelu_tanh".
     Any sizes and strides; operands whose rows do not start on 16 bytes are
-    copied first.  Differentiable
-    in x, w_in and w_out (once).  a = act(g) u (and, for the backward pass, g
-    and u) are rounded to x's type.
+    copied first.  Differentiable in x, w_in and w_out (once).  a = act(g) u
+    (and, for the backward pass, g and u) are rounded to x's type.
     """
     if not plain_eager(x, w_in, w_out):
         return torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, activation)[0]

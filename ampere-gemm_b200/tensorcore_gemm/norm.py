@@ -42,22 +42,22 @@ def _wdtype(x, weight, bias):
 
 
 def _forward(x, weight, bias, eps: float, stats: bool):
-    """y, and with `stats` the rows' mean and 1 / standard deviation (fp32)."""
+    """y, and with `stats` the rows' mean and 1 / standard deviation (fp32, 2 x rows)."""
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     cols = x.shape[-1]
     rows = x.numel() // cols if cols else 0
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     if rows:
         x2, ldx = as_rows(x)
         weight = None if weight is None else weight.contiguous()
         bias = None if bias is None else bias.contiguous()
-        launch("b200_layer_norm_fwd", x.get_device(), x2.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), ptr(mean),
-               ptr(rstd), rows, cols, ldx, cols, DTYPE_CODES[x.dtype], DTYPE_CODES[_wdtype(x, weight, bias)], eps)
-    return y, mean, rstd
+        mean = ptr(stats)
+        launch("b200_layer_norm_fwd", x.get_device(), x2.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), mean,
+               None if mean is None else mean + 4 * rows, rows, cols, ldx, cols, DTYPE_CODES[x.dtype], DTYPE_CODES[_wdtype(x, weight, bias)], eps)
+    return y, stats
 
 
-def _backward(dy, x, weight, mean, rstd, wdtype, need_weight: bool, need_bias: bool):
+def _backward(dy, x, weight, stats, wdtype, need_weight: bool, need_bias: bool):
     """dx, dweight and dbias (None where not needed)."""
     cols = x.shape[-1]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -68,12 +68,13 @@ def _backward(dy, x, weight, mean, rstd, wdtype, need_weight: bool, need_bias: b
         x2, ldx = as_rows(x)
         dy2, lddy = as_rows(dy)
         weight = None if weight is None else weight.contiguous()
+        mean = stats.data_ptr()
         ws_bytes = 0
         if need_weight or need_bias:
             ws_bytes = _native.load().b200_layer_norm_bwd_workspace_size(rows, cols)
         ws = workspace(ws_bytes, x.device, "b200_layer_norm_bwd_workspace_size")
-        launch("b200_layer_norm_bwd", x.get_device(), dy2.data_ptr(), x2.data_ptr(), ptr(weight), mean.data_ptr(),
-               rstd.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), rows, cols, lddy, ldx, cols, DTYPE_CODES[x.dtype],
+        launch("b200_layer_norm_bwd", x.get_device(), dy2.data_ptr(), x2.data_ptr(), ptr(weight), mean,
+               mean + 4 * rows, dx.data_ptr(), ptr(dw), ptr(db), rows, cols, lddy, ldx, cols, DTYPE_CODES[x.dtype],
                DTYPE_CODES[wdtype], ptr(ws), ws_bytes)
     return dx, dw, db
 
@@ -81,17 +82,17 @@ def _backward(dy, x, weight, mean, rstd, wdtype, need_weight: bool, need_bias: b
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.wdtype = _wdtype(x, weight, bias)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = _backward(dy, x, weight, mean, rstd, ctx.wdtype, need_w, need_b)
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx, dw, db = _backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
         return dx if need_x else None, dw, db, None
 
 
@@ -116,8 +117,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("tensorcore_gemm::layer_norm", mutates_args=())
 def _layer_norm_op(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
-                   eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """y, mean and rstd of `layer_norm` (the statistics are not differentiable)."""
+                   eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """y of `layer_norm`, and the rows' mean and 1 / standard deviation (not differentiable)."""
     _check(x, weight, bias)
     return _forward(x, weight, bias, eps, True)
 
@@ -126,35 +127,33 @@ def _layer_norm_op(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
 def _(x, weight, bias, eps):
     _check(x, weight, bias)
     rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-    stats = [torch.empty(rows, dtype=torch.float32, device=x.device) for _ in range(2)]
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device), *stats
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device),
+            torch.empty((2, rows), dtype=torch.float32, device=x.device))
 
 
 @torch.library.custom_op("tensorcore_gemm::layer_norm_backward", mutates_args=())
-def _layer_norm_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
-                            rstd: torch.Tensor,
+def _layer_norm_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
                             wdtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _backward(dy, x, weight, mean, rstd, wdtype, True, True)
+    return _backward(dy, x, weight, stats, wdtype, True, True)
 
 
 @_layer_norm_backward_op.register_fake
-def _(dy, x, weight, mean, rstd, wdtype):
+def _(dy, x, weight, stats, wdtype):
     sums = [torch.empty(x.shape[-1], dtype=wdtype, device=x.device) for _ in range(2)]
     return torch.empty(x.shape, dtype=x.dtype, device=x.device), *sums
 
 
 def _setup_context(ctx, inputs, output) -> None:
     x, weight, bias, _ = inputs
-    _, mean, rstd = output
-    ctx.save_for_backward(x, weight, mean, rstd)
+    ctx.save_for_backward(x, weight, output[1])
     ctx.wdtype = _wdtype(x, weight, bias)
     ctx.has = (weight is not None, bias is not None)
-    ctx.mark_non_differentiable(mean, rstd)
+    ctx.mark_non_differentiable(output[1])
 
 
-def _op_backward(ctx, dy, _dmean, _drstd):
-    x, weight, mean, rstd = ctx.saved_tensors
-    dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, mean, rstd, ctx.wdtype)
+def _op_backward(ctx, dy, _dstats):
+    x, weight, stats = ctx.saved_tensors
+    dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype)
     return dx, dw if ctx.has[0] else None, db if ctx.has[1] else None, None
 
 

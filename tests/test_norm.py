@@ -215,7 +215,8 @@ def test_other_stream_and_graph(cuda_device, native_lib):
 def test_dispatcher_operator(cuda_device, native_lib):
     x, w, b, dy = make(20, 48, F32, F32, cuda_device)
     leaves = [t.clone().requires_grad_() for t in (x, w, b)]
-    y, mean, rstd = torch.ops.tensorcore_gemm.layer_norm(*leaves, EPS)
+    y, stats = torch.ops.tensorcore_gemm.layer_norm(*leaves, EPS)
+    assert stats.shape == (2, 20)
     assert torch.equal(y, norm.layer_norm(x, w, b))
     check_backward(*torch.autograd.grad(y, leaves, dy), x, w, dy)
     torch.library.opcheck(torch.ops.tensorcore_gemm.layer_norm, (*leaves, EPS),
