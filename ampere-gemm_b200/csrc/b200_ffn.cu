@@ -67,38 +67,6 @@ int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
   return le == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 
-// Columns [hidden, hidden_pad) of a, g and u hold whatever the tile computed
-// there (the up projection's first rows as gates); nothing reads them.
-template <bool kBf16>
-int gate_up(const void* x, int64_t ldx, const void* w_in, int64_t ldw, uint16_t* a, uint16_t* gate_up, int act,
-            const GateShape& s, cudaStream_t stream) {
-  FusedArgs<kEpiGateUp> fx;
-  fx.activation = act;
-  fx.save = gate_up != nullptr;
-  // Unused maps point at `a`, so that every launch has valid ones.
-  const int64_t ld = gate_up ? 2 * (int64_t)s.hidden_pad : s.hidden_pad;
-  for (int half = 0; half < 2; ++half)
-    if (int rc = make_tmap_2d(half ? &fx.tmap_u : &fx.tmap_g, gate_up ? gate_up + half * s.hidden_pad : a, s.rows,
-                              s.hidden_pad, ld, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE))
-      return rc;
-  return launch_gate<kBf16, kEpiGateUp>(x, ldx, w_in, ldw, a, s, fx, stream);
-}
-
-template <bool kBf16>
-int gate_bwd(const void* dy, int64_t lddy, const void* w_out, int64_t ldw, const uint16_t* gate_up, uint16_t* dgu,
-             uint16_t* a, int act, const GateShape& s, cudaStream_t stream) {
-  FusedArgs<kEpiGateBwd> fx;
-  fx.activation = act;
-  fx.g = gate_up;
-  fx.u = gate_up + s.hidden_pad;
-  fx.dg = dgu;
-  fx.du = dgu + s.hidden_pad;
-  fx.a = a;
-  fx.ld = 2 * (int64_t)s.hidden_pad;
-  fx.ld_a = s.hidden_pad;
-  return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s, fx, stream);
-}
-
 // A matrix copied between pitches; columns [cols, dst_cols) of the copy, and
 // `zero_rows` rows after it, are zero.
 struct CopyJob {
@@ -190,11 +158,6 @@ void* writable(void* p, int64_t& ld, int64_t rows, int64_t cols, Carver& ws, Cop
   return copy;
 }
 
-int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
-               int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* stream) {
-  return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, stream);
-}
-
 // ---- few rows of x (kernel_rows.cuh) ----
 
 constexpr int kRowsMaxSmem = 220 * 1024;
@@ -209,9 +172,10 @@ int rows_clusters(Kern kern, int parts, int sm_count) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sm_count / parts;
   int& n = cache[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3];
   if (n > 0) return n;
+  (void)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsMaxSmem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count / parts * parts);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kRowsThreads);
   cfg.dynamicSmemBytes = kRowsMaxSmem;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -227,56 +191,88 @@ int rows_clusters(Kern kern, int parts, int sm_count) {
   return n = std::min(got, sm_count / parts);
 }
 
-// Few enough rows of x for the rows kernel.  It reads the weights once, evenly
-// over the SMs (4096 x 12288: 54 us for 1 token, 69 for 128, 119 for 256,
-// against 294, 131 and 133 with the pair kernel, whose loads of a mostly empty
-// tile of x collide); its epilogue grows with the tokens, which small weights
-// do not hide (512 x 1408: 18 us for 128 tokens, 22 for 160, pair 22; 128 x
-// 400: 10 for 32, 13.5 for 64, pair 13).
-bool few_rows(int64_t rows, int64_t dim, int64_t hidden) {
-  return rows <= kRowsMaxTokens && 25 * rows * rows <= dim * hidden;
+// How the rows kernel cuts a product up: CTAs of a cluster, rows of w per
+// cluster and rows of x per tile, and the estimated time in cycles.
+struct RowsPlan {
+  int parts = 0, block = 0, tile = 0;
+  double cycles = 0.0;
+};
+
+// The least estimated time over cluster sizes, tiles of x and row blocks of w
+// (an even share for every cluster, 128 rows or 64).  A CTA's 64-deep block of
+// K costs 5.1 cycles a row of w (128 bytes at the 25 bytes a cycle that an SM
+// gets of the memory's rate; 2 when another tile brought it into L2), 2 a row
+// of x, and its MMAs (4 an accumulator, 42 each or N / 2), which hide loads or
+// are hidden in part; a cluster's reduction costs 700, a wave 4500, a row of x
+// 16 in the epilogue.  Fitted to sweeps over 512 x 1408 to 4096 x 12288 and 1
+// to 128 rows of x (one row block an SM without clusters was 1.3-2.3x slower
+// for w_out).
+RowsPlan plan_rows(int tokens, int n, int k, int accs, bool w_major_n, const int (&slots_of)[4]) {
+  RowsPlan best;
+  const int k_blocks = (k + kBK - 1) / kBK;
+  const int least_tiles = (tokens + kRowsMaxTokens - 1) / kRowsMaxTokens;
+  for (int t_tiles = least_tiles; t_tiles < least_tiles + 3; ++t_tiles) {
+    const int tile = (tokens + t_tiles - 1) / t_tiles, pad = (tile + 15) / 16 * 16;
+    if (t_tiles > least_tiles && tile < 64) break;
+    const double row_cost = (5.1 + 2.0 * (t_tiles - 1)) / t_tiles;
+    for (int i = 0, s = 1; s <= kRowsMaxParts && s <= k_blocks; ++i, s *= 2) {
+      const int slots = slots_of[i], share = (k_blocks + s - 1) / s;
+      for (int choice = 0; choice < 3; ++choice) {
+        int block = choice == 0 ? 128 : 64;
+        if (choice == 2) {
+          if (t_tiles > 1 || w_major_n) continue;  // an even share
+          const int even_waves = (n + slots * 128 - 1) / (slots * 128);
+          block = (n + slots * even_waves - 1) / (slots * even_waves);
+        }
+        const long long tiles = (long long)((n + block - 1) / block) * t_tiles;
+        const double waves = (double)((tiles + slots - 1) / slots);
+        const double mma = accs * 4.0 * std::max(42, pad / 2);
+        const double load = row_cost * accs * block + 2.0 * pad;
+        const double cycles =
+            waves * (share * (std::max(mma, load) + 0.4 * std::min(mma, load)) + 16.0 * accs * pad + 4500.0) +
+            (s > 1 ? 700.0 : 0.0);
+        if (best.parts == 0 || cycles < best.cycles) best = RowsPlan{s, block, tile, cycles};
+      }
+    }
+  }
+  return best;
 }
 
-template <bool kBf16, bool kGate>
-int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ld_out, int tokens, int n,
-                int k, int act, bool w_early, const DeviceInfo& dev, cudaStream_t stream) {
-  auto kern = gemm_rows_kernel<kBf16, kGate>;
+// Estimated cycles of the pair kernel: waves of 256 x 256 accumulator tiles
+// (`out_n` columns of the result each), 512 a 64-deep block of K, or 800 where
+// w comes from memory and not, for another row of tiles, from L2; and a tile's
+// epilogue after the last wave.
+double pair_cycles(int tokens, int n, int k, int out_n, int sm_count) {
+  const int row_tiles = (tokens + 255) / 256;
+  const long long tiles = (long long)row_tiles * ((n + out_n - 1) / out_n);
+  const long long waves = (tiles + sm_count / 2 - 1) / (sm_count / 2);
+  return (double)waves * (std::max(512.0, 800.0 / row_tiles) * ((k + kBK - 1) / kBK) + 2000.0) + 9000.0;
+}
+
+// One product on the rows kernel; `w` has `n` rows (2 n with kRowsGateUp) of k
+// elements, or is stored k x n (kWMajorN).
+template <bool kBf16, int kMode, bool kWMajorN>
+int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, const RowsOut& io, int tokens, int n, int n_pad,
+                int k, int act, bool w_early, const RowsPlan& plan, cudaStream_t stream) {
+  auto kern = gemm_rows_kernel<kBf16, kMode, kWMajorN>;
   static std::atomic<uint8_t> attr_done[kMaxDevices];
   if (int e = ensure_smem_attr(kern, kRowsMaxSmem, attr_done)) return e;
+  constexpr bool kGate = kMode == kRowsGateUp;
   constexpr int kAccs = kGate ? 2 : 1;
   RowsShape sh;
   sh.tokens = tokens;
-  sh.tokens_pad = (tokens + 15) / 16 * 16;
+  sh.tile = plan.tile;
+  sh.tokens_pad = (plan.tile + 15) / 16 * 16;
   sh.n = n;
+  sh.n_pad = n_pad;
+  sh.n_blocks = (n + plan.block - 1) / plan.block;
   sh.k_blocks = (k + kBK - 1) / kBK;
+  sh.block = plan.block;
+  sh.block_pad = (sh.block + 7) / 8 * 8;
   sh.activation = act;
   sh.w_early = w_early ? 1 : 0;
-  // CTAs of a cluster: the least estimated time of a CTA, in cycles.  A 64-deep
-  // block of K costs 5.1 a row of w (128 bytes at the 25 bytes a cycle that an
-  // SM gets of the memory's rate), 2 a token (from L2), and 0.4 of its MMAs'
-  // time (4 an accumulator, 42 each or N / 2), which the loads hide in part; a
-  // cluster's reduction costs 700, another wave 3000.  Fitted to sweeps over
-  // 512 x 1408 to 4096 x 12288 and 1 to 128 tokens (a row block per SM, no
-  // clusters, was 1.3-2.3x slower for w_out).
-  int parts = 1;
-  double best = -1.0;
-  for (int s = 1; s <= kRowsMaxParts && s <= sh.k_blocks; s *= 2) {
-    const int slots = rows_clusters(kern, s, dev.sm_count);
-    const int waves = (n + slots * 128 - 1) / (slots * 128);
-    const int block = (n + slots * waves - 1) / (slots * waves);
-    const int share = (sh.k_blocks + s - 1) / s;
-    const double mma = 0.4 * kAccs * 4 * std::max(42, sh.tokens_pad / 2);
-    const double cycles = waves * share * (5.1 * kAccs * block + 2.0 * sh.tokens_pad + mma) + (s > 1 ? 700.0 : 0.0) +
-                          3000.0 * (waves - 1);
-    if (best < 0.0 || cycles < best) {
-      best = cycles;
-      parts = s;
-      sh.block = block;
-    }
-  }
-  sh.block_pad = (sh.block + 7) / 8 * 8;
   const int sub = rows_sub_bytes(sh, kGate);
-  const int share = (sh.k_blocks + parts - 1) / parts;
+  const int share = (sh.k_blocks + plan.parts - 1) / plan.parts;
   // 48 KB a stage (16 KB: 10-30 % slower, each stage costs its commit) in a
   // ring of 200 KB (94 KB, beside the next launch's: 4-8 % slower).
   constexpr int kStageTarget = 48 * 1024, kRing = 200 * 1024;
@@ -291,26 +287,115 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, void* ou
   const int smem = sh.stages * stage + sh.tail + kRowsBarBytes + 1024;
   if (smem > kRowsMaxSmem) return B200_ERR_CUDA;
   CUtensorMap tw, tx;
-  int rc = make_tmap_2d(&tw, w, (uint64_t)kAccs * n, k, ldw, kBK, sh.block, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  int rc = kWMajorN ? make_tmap_2d(&tw, w, k, n, ldw, 64, kBK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)
+                    : make_tmap_2d(&tw, w, (uint64_t)kAccs * n, k, ldw, kBK, sh.block,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (rc) return rc;
   rc = make_tmap_2d(&tx, x, tokens, k, ldx, kBK, sh.tokens_pad, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((n + sh.block - 1) / sh.block * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(sh.n_blocks * ((tokens + sh.tile - 1) / sh.tile) * plan.parts));
+  cfg.blockDim = dim3(kRowsThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.x = plan.parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, static_cast<uint16_t*>(out), ld_out, sh);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, io, sh);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
+// Whether a product goes to the rows kernel, and how.  Both ways were measured
+// over 64 to 3000 rows: at 4096 x 12288 the block takes 54 us for 1 row and 64
+// for 128 (pair kernel 287 and 131: its loads of a mostly empty tile of x
+// collide), from 300 rows on the pair kernel is as fast; at 1000 x 2731 a
+// training step takes 102 us for 300 rows (152) and 169 for 1111 (191).
+template <bool kBf16, int kMode, bool kWMajorN>
+bool rows_wins(int tokens, int n, int k, int sm_count, RowsPlan& plan) {
+  constexpr bool kGate = kMode == kRowsGateUp;
+  if (tokens > 16 * kRowsMaxTokens) return false;
+  auto kern = gemm_rows_kernel<kBf16, kMode, kWMajorN>;
+  int slots[4];
+  for (int i = 0; i < 4; ++i) slots[i] = rows_clusters(kern, 1 << i, sm_count);
+  plan = plan_rows(tokens, n, k, kGate ? 2 : 1, kWMajorN, slots);
+  return plan.cycles < pair_cycles(tokens, n, k, kGate ? 128 : 256, sm_count);
+}
+
+// Columns [hidden, hidden_pad) of a, g and u hold whatever the tile computed
+// there (the up projection's first rows as gates); nothing reads them.
+template <bool kBf16>
+int gate_up(const void* x, int64_t ldx, const void* w_in, int64_t ldw, uint16_t* a, uint16_t* gate_up, int act,
+            const GateShape& s, const DeviceInfo& dev, cudaStream_t stream) {
+  RowsPlan plan;
+  if (rows_wins<kBf16, kRowsGateUp, false>(s.rows, s.hidden, s.depth, dev.sm_count, plan)) {
+    RowsOut io{a, s.hidden_pad};
+    if (gate_up) {
+      io.g = gate_up;
+      io.u = gate_up + s.hidden_pad;
+      io.ld_gu = 2 * (int64_t)s.hidden_pad;
+    }
+    return launch_rows<kBf16, kRowsGateUp, false>(x, ldx, w_in, ldw, io, s.rows, s.hidden, s.hidden_pad, s.depth, act,
+                                                  false, plan, stream);
+  }
+  FusedArgs<kEpiGateUp> fx;
+  fx.activation = act;
+  fx.save = gate_up != nullptr;
+  // Unused maps point at `a`, so that every launch has valid ones.
+  const int64_t ld = gate_up ? 2 * (int64_t)s.hidden_pad : s.hidden_pad;
+  for (int half = 0; half < 2; ++half)
+    if (int rc = make_tmap_2d(half ? &fx.tmap_u : &fx.tmap_g, gate_up ? gate_up + half * s.hidden_pad : a, s.rows,
+                              s.hidden_pad, ld, kEpiCols, kEpiRows, CU_TENSOR_MAP_L2_PROMOTION_NONE))
+      return rc;
+  return launch_gate<kBf16, kEpiGateUp>(x, ldx, w_in, ldw, a, s, fx, stream);
+}
+
+template <bool kBf16>
+int gate_bwd(const void* dy, int64_t lddy, const void* w_out, int64_t ldw, const uint16_t* gate_up, uint16_t* dgu,
+             uint16_t* a, int act, const GateShape& s, const DeviceInfo& dev, cudaStream_t stream) {
+  RowsPlan plan;
+  if (rows_wins<kBf16, kRowsGateBwd, true>(s.rows, s.hidden, s.depth, dev.sm_count, plan)) {
+    RowsOut io{a, s.hidden_pad};
+    io.saved_g = gate_up;
+    io.saved_u = gate_up + s.hidden_pad;
+    io.dg = dgu;
+    io.du = dgu + s.hidden_pad;
+    io.ld_gu = 2 * (int64_t)s.hidden_pad;
+    return launch_rows<kBf16, kRowsGateBwd, true>(dy, lddy, w_out, ldw, io, s.rows, s.hidden, s.hidden_pad, s.depth,
+                                                  act, false, plan, stream);
+  }
+  FusedArgs<kEpiGateBwd> fx;
+  fx.activation = act;
+  fx.g = gate_up;
+  fx.u = gate_up + s.hidden_pad;
+  fx.dg = dgu;
+  fx.du = dgu + s.hidden_pad;
+  fx.a = a;
+  fx.ld = 2 * (int64_t)s.hidden_pad;
+  fx.ld_a = s.hidden_pad;
+  return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s, fx, stream);
+}
+
+int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
+               int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* stream) {
+  return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, stream);
+}
+
+// C = A B with A rows x k, B stored n x k or k x n (kWMajorN), on the kernel that is faster.
+template <bool kBf16, bool kWMajorN>
+int product(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int rows, int n, int k,
+            bool b_early, const DeviceInfo& dev, cudaStream_t stream) {
+  RowsPlan plan;
+  if (rows_wins<kBf16, kRowsPlain, kWMajorN>(rows, n, k, dev.sm_count, plan))
+    return launch_rows<kBf16, kRowsPlain, kWMajorN>(A, lda, B, ldb, RowsOut{static_cast<uint16_t*>(C), ldc}, rows, n, n,
+                                                    k, 0, b_early, plan, stream);
+  return plain_gemm(kBf16, A, B, C, rows, n, k, lda, ldb, ldc, B200_A_ROW_MAJOR,
+                    kWMajorN ? B200_B_ROW_MAJOR : B200_B_COL_MAJOR, stream);
 }
 
 // Checks shared by the two directions; *empty: some dimension is 0.
@@ -377,7 +462,6 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   if (!x || !w_in || !w_out || !y || ldx < dim || ldw_in < dim || ldw_out < hidden || ldy < out_dim)
     return B200_ERR_INVALID_ARGUMENT;
   if (gate_up && !aligned16(gate_up)) return B200_ERR_MISALIGNED;
-  const bool few = few_rows(rows, dim, hidden) && !gate_up;
   const bool copies = !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) || !pitch_ok(y, ldy);
   if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, dim, hidden, out_dim, 0, copies)))
     return B200_ERR_WORKSPACE;
@@ -392,21 +476,14 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   w_in = readable(w_in, ldw_in, 2 * hidden, dim, ws, before);
   w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
   if (int rc = run_copies(before, stream)) return rc;
-  if (few) {
-    const int rc = (bf16 ? launch_rows<true, true> : launch_rows<false, true>)(
-        x, ldx, w_in, ldw_in, a, hp, (int)rows, (int)hidden, (int)dim, activation, false, dev, stream);
-    if (rc) return rc;
-    // w_out was written two kernels ago at the latest: its loads may start early.
-    return (bf16 ? launch_rows<true, false> : launch_rows<false, false>)(
-        a, hp, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim, (int)hidden, 0, true, dev, stream);
-  }
   const GateShape s{(int)rows, (int)hidden, (int)dim, (int)hp};
-  int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(x, ldx, w_in, ldw_in, a,
-                                                               static_cast<uint16_t*>(gate_up), activation, s, stream);
+  int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(
+      x, ldx, w_in, ldw_in, a, static_cast<uint16_t*>(gate_up), activation, s, dev, stream);
   if (rc) return rc;
   y = writable(y, ldy, rows, out_dim, ws, after);
-  rc = plain_gemm(bf16, a, w_out, y, rows, out_dim, hidden, hp, ldw_out, ldy, B200_A_ROW_MAJOR, B200_B_COL_MAJOR,
-                  stream_ptr);
+  // w_out was written two kernels ago at the latest: its loads may start early.
+  rc = (bf16 ? product<true, false> : product<false, false>)(a, hp, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim,
+                                                             (int)hidden, true, dev, stream);
   return rc ? rc : run_copies(after, stream);
 }
 
@@ -462,12 +539,12 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
   if (int rc = run_copies(before, stream)) return rc;
   const GateShape s{(int)rows, (int)hidden, (int)out_dim, (int)hp};
   int rc = (bf16 ? gate_bwd<true> : gate_bwd<false>)(dy, lddy, w_out, ldw_out, static_cast<const uint16_t*>(gate_up),
-                                                     dgu, a, activation, s, stream);
+                                                     dgu, a, activation, s, dev, stream);
   if (rc) return rc;
   if (dx) {
     dx = writable(dx, lddx, rows, dim, ws, after);
-    rc = plain_gemm(bf16, dgu, w_in, dx, rows, dim, 2 * hp, 2 * hp, ldw_in, lddx, B200_A_ROW_MAJOR, B200_B_ROW_MAJOR,
-                    stream_ptr);
+    rc = (bf16 ? product<true, true> : product<false, true>)(dgu, 2 * hp, w_in, ldw_in, dx, lddx, (int)rows, (int)dim,
+                                                             (int)(2 * hp), true, dev, stream);
     if (rc) return rc;
   }
   if (dw_in) {

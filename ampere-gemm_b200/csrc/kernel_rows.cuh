@@ -1,22 +1,27 @@
-// GEMM kernel for few rows of x (decoding): out[t][n] = sum_k x[t][k] w[n][k],
-// or, with kGate, out[t][n] = act(g) u for w = [Wg; Wu].
+// GEMM kernel for few to some hundred rows of x: out[t][n] = sum_k x[t][k] w[n][k],
+// with the gated feed-forward block's epilogues (see RowsMode).
 //
-// Such a product is bound by reading w once.  So the operands change places:
-// a block of rows of w is the 128-row operand of the MMA (lane = row of w) and
-// all rows of x, rounded up to 16, are its N columns.  Rows of w are dealt out
-// evenly: every CTA takes `block` of them (not 128: lanes past `block` compute
-// on whatever lies behind the tile in shared memory and are never read), so
-// one wave of CTAs streams equal shares of w.  With a cluster of S CTAs each
-// takes 1/S of K for S times as many rows, which cuts the re-reading of x (all
-// of it, by every cluster) by S; the S parts are added up through distributed
-// shared memory in a fixed order.
+// With few rows such a product is bound by reading w once.  So the operands
+// change places: a block of rows of w is the 128-row operand of the MMA (lane =
+// row of w) and up to 256 rows of x, rounded up to 16, are its N columns.  Rows
+// of w are dealt out evenly: every CTA takes `block` of them (not 128: lanes
+// past `block` compute on whatever lies behind the tile in shared memory and
+// are never read), so one wave of CTAs streams equal shares of w.  With a
+// cluster of S CTAs each takes 1/S of K for S times as many rows, which cuts
+// the re-reading of x (all of it, by every cluster) by S and fills the SMs when
+// there are few tiles; the S parts are added up through distributed shared
+// memory in a fixed order.  More rows of x than one tile holds are split evenly
+// over several.
 //
-//   warp 0      TMA producer; warp 1 MMA issuer; warps 2..5 epilogue.
+//   warp 0      TMA producer; warp 1 MMA issuer; warps 2..9 epilogue, which all
+//               ten share once the MMAs are over.
 //
 // Launched with programmatic stream serialisation.  With `w_early`, w was not
 // written by the kernel before this one on the stream: the first stages of w
 // are requested before that kernel has finished, only x waits for it.
 #pragma once
+
+#include <type_traits>
 
 #include "epilogue_gate.cuh"
 #include "gemm_common.cuh"
@@ -26,10 +31,20 @@ namespace b200 {
 constexpr int kRowsMaxTokens = 256;  // N of one MMA
 constexpr int kRowsMaxStages = 16;
 constexpr int kRowsMaxParts = 8;     // CTAs of a cluster
+constexpr int kRowsThreads = 320;    // producer, issuer and eight epilogue warps
+
+// Epilogues.
+enum RowsMode : int {
+  kRowsPlain = 0,    // out = the product
+  kRowsGateUp = 1,   // w = [Wg; Wu]: out = act(g) u, optionally g and u too
+  kRowsGateBwd = 2,  // the product is da: dg, du and out = a from it and the saved g, u
+};
 
 struct RowsShape {
   int tokens;      // rows of x
-  int tokens_pad;  // rounded up to 16: N of the MMAs
+  int tile;        // rows of x per tile
+  int tokens_pad;  // `tile` rounded up to 16: N of the MMAs
+  int n_blocks;    // row blocks of w
   int n;           // rows of w (of each half with kGate)
   int k_blocks;    // 64-wide blocks of K
   int block;       // rows of w per cluster (of each half), <= 128
@@ -39,7 +54,21 @@ struct RowsShape {
   int chunk;       // tokens per reduction round of a cluster
   int activation;
   int w_early;
+  int n_pad;       // columns that kRowsGateBwd writes: n, and zeros up to here
   int tail;        // bytes after the stages that an MMA may read: a tile of fewer than 128 rows is read past its end
+};
+
+// Where the epilogue writes and reads, row pitches in elements.
+struct RowsOut {
+  uint16_t* out;
+  int64_t ld;
+  uint16_t* g = nullptr;  // kRowsGateUp: g and u are stored here unless NULL
+  uint16_t* u = nullptr;
+  const uint16_t* saved_g = nullptr;  // kRowsGateBwd
+  const uint16_t* saved_u = nullptr;
+  uint16_t* dg = nullptr;
+  uint16_t* du = nullptr;
+  int64_t ld_gu = 0;      // of all of these
 };
 
 __host__ __device__ inline int rows_sub_bytes(const RowsShape& s, bool gate) {
@@ -134,10 +163,63 @@ __device__ __forceinline__ float gate_value(int activation, float g, float u) {
   return activate<2, false>(g).f * u;
 }
 
-template <bool kBf16, bool kGate>
-__global__ void __launch_bounds__(kThreads, 2)
+// dg, du and a of one element.
+template <int kAct>
+__device__ __forceinline__ float3 gate_grad(float da, float g, float u) {
+  const ActValue v = activate<kAct, true>(g);
+  return make_float3(da * u * v.slope, da * v.f, v.f * u);
+}
+__device__ __forceinline__ float3 gate_grads(int activation, float da, float g, float u) {
+  if (activation == 0) return gate_grad<0>(da, g, u);
+  if (activation == 1) return gate_grad<1>(da, g, u);
+  return gate_grad<2>(da, g, u);
+}
+
+// The first `n` (<= 4) of four values to 16-bit elements at p, in one store when it is a whole, aligned one.
+template <bool kBf16>
+__device__ __forceinline__ void store_quad(uint16_t* p, const float (&v)[4], int n) {
+  const uint32_t lo = pack_16bit_rn<kBf16>(__float_as_uint(v[0]), __float_as_uint(v[1]));
+  const uint32_t hi = pack_16bit_rn<kBf16>(__float_as_uint(v[2]), __float_as_uint(v[3]));
+  if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) p[e] = static_cast<uint16_t>((e < 2 ? lo : hi) >> ((e & 1) * 16));
+}
+
+// The accumulators' four rows of w of one token, staged at `at` in each of the
+// kP CTAs of the cluster: all parts are requested, then added up in order.
+template <int kP, int kAccs>
+__device__ __forceinline__ void sum_parts(const float* at, int acc_step, float4 (&r)[kAccs]) {
+  float4 v[kAccs][kP];
+#pragma unroll
+  for (int a = 0; a < kAccs; ++a) {
+#pragma unroll
+    for (int p = 0; p < kP; ++p)
+      v[a][p] = kP == 1 ? *reinterpret_cast<const float4*>(at + a * acc_step)
+                        : ld_shared_cluster_v4(mapa_shared(smem_u32(at + a * acc_step), p));
+  }
+#pragma unroll
+  for (int a = 0; a < kAccs; ++a) {
+    r[a] = v[a][0];
+#pragma unroll
+    for (int p = 1; p < kP; ++p) {
+      r[a].x += v[a][p].x;
+      r[a].y += v[a][p].y;
+      r[a].z += v[a][p].z;
+      r[a].w += v[a][p].w;
+    }
+  }
+}
+
+// kWMajorN: w is stored K x N (N contiguous); `block` is then a multiple of 64.
+template <bool kBf16, int kMode, bool kWMajorN>
+__global__ void __launch_bounds__(kRowsThreads, 1)
     gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                     uint16_t* __restrict__ out, int64_t ld_out, const __grid_constant__ RowsShape sh) {
+                     const __grid_constant__ RowsOut io, const __grid_constant__ RowsShape sh) {
+  constexpr bool kGate = kMode == kRowsGateUp;
   constexpr int kAccs = kGate ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -154,13 +236,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int lane = threadIdx.x & 31;
   const int parts = static_cast<int>(cluster_nctarank());
   const int rank = static_cast<int>(cluster_ctarank());
-  const int n0 = static_cast<int>(blockIdx.x) / parts * sh.block;
+  // Row blocks of w are the faster index: the tiles that run together share x.
+  const int cluster = static_cast<int>(blockIdx.x) / parts;
+  const int n0 = cluster % sh.n_blocks * sh.block;
+  const int t_tile = cluster / sh.n_blocks * sh.tile;
+  const int tokens = min(sh.tile, sh.tokens - t_tile);
   const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * sh.k_blocks / parts);
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * sh.k_blocks / parts);
   const int num_stages = (kb1 - kb0 + sh.k_sub - 1) / sh.k_sub;
   // Every cluster reads all of x.  Clusters start at different places of K and
   // wrap around: in step, they would all ask one L2 slice for the same line.
-  const int start = static_cast<int>(static_cast<int64_t>(blockIdx.x) / parts * num_stages / (gridDim.x / parts));
+  const int start = static_cast<int>(static_cast<int64_t>(cluster) * num_stages / (gridDim.x / parts));
   auto k_stage = [&](int it) { return it + start < num_stages ? it + start : it + start - num_stages; };
   auto subs = [&](int it) { return min(sh.k_sub, kb1 - kb0 - k_stage(it) * sh.k_sub); };
   uint32_t tmem_cols = 32;
@@ -188,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) {
     const uint32_t el = elect_lane();
-    const uint64_t pol_w = policy_evict_first();  // read once
+    // Read once, unless several tiles of x follow one another.
+    const uint64_t pol_w = sh.tile < sh.tokens ? policy_evict_normal() : policy_evict_first();
     const uint64_t pol_x = policy_evict_last();   // read by every cluster
     const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full_bar);
     const uint32_t sub_tx = static_cast<uint32_t>((kAccs * sh.block + sh.tokens_pad) * 128);
@@ -199,7 +286,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       int k = (kb0 + k_stage(it) * sh.k_sub) * kBK;
       mbar_expect_tx_if(el, bar, static_cast<uint32_t>(n_sub) * sub_tx);
       for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) {
-        tma_load_2d_if(el, dst, &tmap_w, bar, k, n0, pol_w);
+        if constexpr (kWMajorN) {
+          // Panels of 64 rows of w x 64 of K.
+          for (int p = 0; p < sh.block; p += 64) tma_load_2d_if(el, dst + p * 128, &tmap_w, bar, n0 + p, k, pol_w);
+        } else {
+          tma_load_2d_if(el, dst, &tmap_w, bar, k, n0, pol_w);
+        }
         if (kGate) tma_load_2d_if(el, dst + sh.block_pad * 128, &tmap_w, bar, k, sh.n + n0, pol_w);
       }
     };
@@ -208,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t bar = full0 + stage * 8;
       uint32_t dst = smem0 + stage * stage_bytes + kAccs * sh.block_pad * 128;
       int k = (kb0 + k_stage(it) * sh.k_sub) * kBK;
-      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) tma_load_2d_if(el, dst, &tmap_x, bar, k, 0, pol_x);
+      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) tma_load_2d_if(el, dst, &tmap_x, bar, k, t_tile, pol_x);
     };
     const int first = min(num_stages, sh.stages);
     if (sh.w_early)
@@ -237,10 +329,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 1) {
     const uint32_t el = elect_lane();
-    const uint32_t idesc = make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad), Major::kK, Major::kK, kBf16);
+    const uint32_t idesc = make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad), kWMajorN ? Major::kMN : Major::kK,
+                                              Major::kK, kBf16);
     // Descriptors advance by adding to their address field (units of 16 bytes;
     // addresses stay below 2^18).
-    const uint64_t w_desc0 = make_desc_kmajor_sw128(smem_u32(smem));
+    const uint64_t x_desc0 = make_desc_kmajor_sw128(smem_u32(smem));
+    const uint64_t w_desc0 = kWMajorN ? make_desc_mnmajor_sw128(smem_u32(smem), kBK * 128) : x_desc0;
+    constexpr uint64_t kWStep = (kWMajorN ? kUmmaK * 128 : kUmmaK * 2) >> 4, kXStep = (kUmmaK * 2) >> 4;
     const uint64_t up_off = static_cast<uint64_t>(sh.block_pad * 128) >> 4;
     const uint64_t x_off = static_cast<uint64_t>(kAccs * sh.block_pad * 128) >> 4;
     const uint64_t sub_off = static_cast<uint64_t>(sub_bytes) >> 4;
@@ -254,13 +349,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!ok) break;
       tc_fence_after_sync();
       const int n_sub = subs(it);
-      uint64_t wd = w_desc0 + (static_cast<uint64_t>(stage * stage_bytes) >> 4);
-      for (int j = 0; j < n_sub; ++j, wd += sub_off) {
+      uint64_t at = static_cast<uint64_t>(stage * stage_bytes) >> 4;
+      for (int j = 0; j < n_sub; ++j, at += sub_off) {
+        const uint64_t wd = w_desc0 + at, xd = x_desc0 + at + x_off;
 #pragma unroll
         for (int k = 0; k < kBK / kUmmaK; ++k) {
-          const uint64_t step = static_cast<uint64_t>(k * (kUmmaK * 2)) >> 4;
-          umma_f16_cta1_if(el, tmem_base, wd + step, wd + (x_off + step), idesc, acc);
-          if (kGate) umma_f16_cta1_if(el, d_up, wd + (up_off + step), wd + (x_off + step), idesc, acc);
+          umma_f16_cta1_if(el, tmem_base, wd + k * kWStep, xd + k * kXStep, idesc, acc);
+          if (kGate) umma_f16_cta1_if(el, d_up, wd + up_off + k * kWStep, xd + k * kXStep, idesc, acc);
           acc = 1;
         }
       }
@@ -276,25 +371,25 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncwarp();
 
-  // ---- epilogue: warps 2..5 ----
+  // ---- epilogue ----
   // Rounds of `chunk` tokens: each CTA stages its accumulators in the idle
-  // pipeline stages ([accumulator][token][row of w], fp32), then takes every
-  // S-th token, adds up the S parts and stores.  An item is one token's next
-  // four rows of w; items are dealt to all 128 threads, whatever `block` is.
+  // pipeline stages ([accumulator][token][row of w], fp32; warps 2..9, two to a
+  // quarter of the lanes), then takes every S-th token, adds up the S parts and
+  // stores.  An item is one token's next four rows of w; items are dealt to all
+  // threads, whatever `block` is.
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
   bool got = true;
-  if (warp >= 2) {
-    if (lane == 0) got = mbar_wait(done_bar, 0, kDevTimeoutEpilogue);
-    got = __shfl_sync(0xffffffffu, got, 0);
-    tc_fence_after_sync();
-  }
+  if (warp >= 2 && lane == 0) got = mbar_wait(done_bar, 0, kDevTimeoutEpilogue);
+  got = __shfl_sync(0xffffffffu, got, 0);
+  tc_fence_after_sync();
   float* part = reinterpret_cast<float*>(smem);
-  const int quads = (min(sh.block, sh.n - n0) + 3) >> 2;
-  for (int c0 = 0; c0 < sh.tokens; c0 += sh.chunk) {
+  const int quads = (min(sh.block, (kMode == kRowsGateBwd ? sh.n_pad : sh.n) - n0) + 3) >> 2;
+  const int step_t = kRowsThreads / quads, step_q = kRowsThreads - step_t * quads;
+  for (int c0 = 0; c0 < tokens; c0 += sh.chunk) {
     const int c1 = min(sh.tokens_pad, c0 + sh.chunk);
     const int row = (warp & 3) * 32 + lane;
     if (warp >= 2 && (warp & 3) * 32 < sh.block) {
-      for (int t0 = c0; t0 < c1; t0 += 16) {
+      for (int t0 = c0 + (warp >= 6 ? 16 : 0); t0 < c1; t0 += 32) {
 #pragma unroll
         for (int a = 0; a < kAccs; ++a) {
           uint32_t g[16];
@@ -306,39 +401,62 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     cluster_sync();
-    if (warp >= 2 && got) {
-      const int tokens = (min(c1, sh.tokens) - c0 - rank + parts - 1) / parts;  // of this CTA (0 or less: none)
-      for (int i = threadIdx.x - 64; i < tokens * quads; i += kEpiWarps * 32) {
-        const int q = i % quads, t = c0 + rank + parts * (i / quads);
-        float4 v[kAccs][kRowsMaxParts];
+    const int share = got ? (min(c1, tokens) - c0 - rank + parts - 1) / parts : 0;  // tokens of this CTA
+    int i = threadIdx.x / quads, q = threadIdx.x - i * quads;
+    for (; i < share; i += step_t, q += step_q) {
+      if (q >= quads) {
+        q -= quads;
+        if (++i >= share) break;
+      }
+      const int t = c0 + rank + parts * i;
+      const int n = n0 + 4 * q;
+      const int64_t row_t = t_tile + t;
+      [[maybe_unused]] uint2 sg = make_uint2(0, 0), su = sg;
+      if constexpr (kMode == kRowsGateBwd) {
+        // Rows of g and u are padded to whole quads (what lies past n counts as 0).
+        sg = *reinterpret_cast<const uint2*>(io.saved_g + row_t * io.ld_gu + n);
+        su = *reinterpret_cast<const uint2*>(io.saved_u + row_t * io.ld_gu + n);
+      }
+      float4 r[kAccs];
+      const float* at = part + (t - c0) * 128 + 4 * q;
+      const int acc_step = sh.chunk * 128;
+      switch (parts) {
+        case 1: sum_parts<1, kAccs>(at, acc_step, r); break;
+        case 2: sum_parts<2, kAccs>(at, acc_step, r); break;
+        case 4: sum_parts<4, kAccs>(at, acc_step, r); break;
+        default: sum_parts<8, kAccs>(at, acc_step, r); break;
+      }
+      const float v0[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+      const float v1[4] = {r[kAccs - 1].x, r[kAccs - 1].y, r[kAccs - 1].z, r[kAccs - 1].w};
+      const int left = min(sh.block - 4 * q, sh.n - n);  // rows of w from n on
+      uint16_t* o = io.out + row_t * io.ld + n;
+      if constexpr (kMode == kRowsPlain) {
+        store_quad<kBf16>(o, v0, left);
+      } else if constexpr (kMode == kRowsGateUp) {
+        float y[4];
 #pragma unroll
-        for (int a = 0; a < kAccs; ++a) {
-          const uint32_t at = smem_u32(part + (a * sh.chunk + t - c0) * 128 + 4 * q);
-#pragma unroll
-          for (int p = 0; p < kRowsMaxParts; ++p)
-            v[a][p] = p < parts ? ld_shared_cluster_v4(mapa_shared(at, p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int e = 0; e < 4; ++e) y[e] = gate_value(sh.activation, v0[e], v1[e]);
+        store_quad<kBf16>(o, y, left);
+        if (io.g) {
+          store_quad<kBf16>(io.g + row_t * io.ld_gu + n, v0, left);
+          store_quad<kBf16>(io.u + row_t * io.ld_gu + n, v1, left);
         }
-        float4 r[kAccs];
-#pragma unroll
-        for (int a = 0; a < kAccs; ++a) {
-          r[a] = v[a][0];
-#pragma unroll
-          for (int p = 1; p < kRowsMaxParts; ++p) {
-            r[a].x += v[a][p].x;
-            r[a].y += v[a][p].y;
-            r[a].z += v[a][p].z;
-            r[a].w += v[a][p].w;
-          }
-        }
-        const float g[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
-        const float u[4] = {r[kAccs - 1].x, r[kAccs - 1].y, r[kAccs - 1].z, r[kAccs - 1].w};
-        uint16_t* o = out + static_cast<int64_t>(t) * ld_out + n0 + 4 * q;
+      } else {
+        const float2 g0 = unpack_16bit<kBf16>(sg.x), g1 = unpack_16bit<kBf16>(sg.y);
+        const float2 u0 = unpack_16bit<kBf16>(su.x), u1 = unpack_16bit<kBf16>(su.y);
+        const float g[4] = {g0.x, g0.y, g1.x, g1.y}, u[4] = {u0.x, u0.y, u1.x, u1.y};
+        float dg[4], du[4], a[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y = kGate ? gate_value(sh.activation, g[e], u[e]) : g[e];
-          if (4 * q + e < sh.block && n0 + 4 * q + e < sh.n)
-            o[e] = static_cast<uint16_t>(pack_16bit_rn<kBf16>(__float_as_uint(y), 0u));
+          const float3 v = gate_grads(sh.activation, v0[e], g[e], u[e]);
+          dg[e] = e < left ? v.x : 0.0f;
+          du[e] = e < left ? v.y : 0.0f;
+          a[e] = e < left ? v.z : 0.0f;
         }
+        const int pad_left = sh.n_pad - n;
+        store_quad<kBf16>(io.dg + row_t * io.ld_gu + n, dg, pad_left);
+        store_quad<kBf16>(io.du + row_t * io.ld_gu + n, du, pad_left);
+        store_quad<kBf16>(o, a, pad_left);
       }
     }
     cluster_sync();
