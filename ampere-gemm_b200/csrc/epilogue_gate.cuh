@@ -56,6 +56,24 @@ __device__ __forceinline__ float sigmoid_approx(float x) {
   return r;
 }
 
+// The normal distribution function Phi(x), from erf(z) = 1 - (a1 t + ... + a5
+// t^5) exp(-z^2), t = 1 / (1 + p z), z = |x| / sqrt 2 >= 0 (Abramowitz and
+// Stegun 7.1.26, within 1.5e-7); `e` receives exp(-x^2 / 2).  A third of
+// erfcf()'s instructions, which the epilogue does not hide altogether (at 4001
+// x 4096 x 12288 the gate-and-up product takes 2.16 times the output
+// projection's time with erfcf, 1.98 with this, 1.92 with silu).
+__device__ __forceinline__ float normal_cdf(float x, float& e) {
+  e = exp_approx(-0.5f * x * x);
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.0f)));
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  const float tail = 0.5f * q * t * e;  // Phi(-|x|)
+  return x < 0.0f ? tail : 1.0f - tail;
+}
+
 template <int kAct, bool kSlope>
 __device__ __forceinline__ ActValue activate(float g) {
   ActValue r;
@@ -65,9 +83,10 @@ __device__ __forceinline__ ActValue activate(float g) {
     r.f = g * s;
     if (kSlope) r.slope = s * (1.0f + g * (1.0f - s));
   } else if constexpr (kAct == 1) {  // gelu: g Phi(g)
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    float e;
+    const float cdf = normal_cdf(g, e);
     r.f = g * cdf;
-    if (kSlope) r.slope = cdf + g * (0.39894228040143268f * exp_approx(-0.5f * g * g));
+    if (kSlope) r.slope = cdf + g * (0.39894228040143268f * e);
   } else {  // gelu with tanh: g (1 + tanh z) / 2 = g s(2z), z = sqrt(2/pi) (g + 0.044715 g^3)
     constexpr float kC = 0.79788456080286536f, kA = 0.044715f;
     const float s = sigmoid_approx(2.0f * kC * g * (1.0f + kA * g * g));
