@@ -62,8 +62,8 @@ int launch_gate(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
   ep.n = ep.n_tma = s.hidden_pad;
   ep.ldc = s.hidden_pad;
   ep.c = static_cast<uint16_t*>(C);
-  const cudaError_t le = launch_gemm(kern, dim3(2 * (unsigned)tiles), dim3(kThreads), Cfg::kSmemBytes, stream, ta, tb,
-                                     tc, s.rows, s.hidden, s.depth, 8, ep, SplitTail{}, fx);
+  const cudaError_t le = launch_gemm(kern, dim3(2 * (unsigned)tiles), dim3(pair_threads(kEpi)), Cfg::kSmemBytes, stream,
+                                     ta, tb, tc, s.rows, s.hidden, s.depth, 8, ep, SplitTail{}, fx);
   return le == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 

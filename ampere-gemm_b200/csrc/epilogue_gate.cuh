@@ -157,16 +157,25 @@ __device__ __forceinline__ uint4 keep_first(uint4 v, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Reads the 32 x 64 blocks of the saved g and u at column x, row y: lane l
-// takes 16-byte piece l % 8 of rows l / 8, l / 8 + 4, ... (whole 128-byte row
-// pieces per instruction).  Their rows are padded to whole pieces; what lies
-// past column N, or in pieces out of range, counts as 0.
-__device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx, uint4 (&g)[8], uint4 (&u)[8],
+// Blocks of 32 rows x 32 columns in the backward epilogue.  In global memory
+// lane l handles 16-byte piece l % 4 of rows l / 4, l / 4 + 8, ... (64-byte row
+// pieces, eight rows an instruction).  In shared memory row r is at r * 64, its
+// piece p at p ^ (r / 2) % 4: neither that mapping nor lane = row conflicts.
+constexpr int kGateBlockBytes = 32 * 64;
+
+__device__ __forceinline__ int gate_piece(int row, int piece) {
+  return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
+}
+
+// Reads the blocks of the saved g and u at column x, row y.  Their rows are
+// padded to whole pieces; what lies past column N, or in pieces out of range,
+// counts as 0.
+__device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx, uint4 (&g)[4], uint4 (&u)[4],
                                                int lane, int x, int y, int M, int N) {
-  const int col = x + (lane & 7) * 8;
+  const int col = x + (lane & 3) * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = y + i * 4 + (lane >> 3);
+  for (int i = 0; i < 4; ++i) {
+    const int row = y + i * 8 + (lane >> 2);
     g[i] = u[i] = make_uint4(0, 0, 0, 0);
     if (row < M && col < N) {
       const int64_t off = static_cast<int64_t>(row) * fx.ld + col;
@@ -180,65 +189,62 @@ __device__ __forceinline__ void gate_bwd_fetch(const FusedArgs<kEpiGateBwd>& fx,
   }
 }
 
-// Stores the 32 x 64 block staged at `buf` (row r at r * 128, 16-byte pieces
-// swizzled) to column x, row y: the mapping of gate_bwd_fetch.
+// Stores the block staged at `buf` to column x, row y of `out`.
 __device__ __forceinline__ void gate_bwd_store(const uint8_t* buf, uint16_t* out, int64_t ld, int lane, int x, int y,
                                                int M, int N) {
-  const int col = x + (lane & 7) * 8;
+  const int col = x + (lane & 3) * 8;
   if (col >= N) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
     if (y + r < M)
       *reinterpret_cast<uint4*>(out + static_cast<int64_t>(y + r) * ld + col) =
-          *reinterpret_cast<const uint4*>(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          *reinterpret_cast<const uint4*>(buf + gate_piece(r, lane & 3));
   }
 }
 
-// Backward: the accumulator row holds da at columns [n0, n0 + 256).  Per 64
-// columns, g and u go through the warp's two staging buffers into the layout
-// of the accumulator (lane = row), dg and du replace them there and leave by
-// plain stores of whole 128-byte row pieces (zeros past column N), then a takes
-// the first buffer.  The next block's g and u are fetched meanwhile.
+// Backward: the accumulator row holds da at columns [n0, n0 + 128) from t_row
+// on.  Per 32 columns, g and u go through the warp's staging buffers into the
+// layout of the accumulator (lane = row), dg and du replace them there and
+// leave by plain stores (zeros past column N), then a takes the first buffer.
+// The next block's g and u are fetched meanwhile.  Eight warps share a tile:
+// four took 43000 cycles for it (silu; measured at a depth of 512, where the
+// MMAs take 4100), which a depth of 4096 (32800) does not hide.
 template <bool kBf16, int kAct, typename Release>
-__device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[8], uint4 (&uv)[8],
+__device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[4], uint4 (&uv)[4],
                                                 uint32_t t_row, uint8_t* epi_buf, int lane, int n0, int y, int M,
                                                 int N, Release&& release) {
   uint8_t* buf0 = epi_buf;
-  uint8_t* buf1 = epi_buf + kEpiBufBytes;
+  uint8_t* buf1 = epi_buf + kGateBlockBytes;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
-    const int x = n0 + c * kEpiCols;
-    uint32_t lo[32], hi[32];
-    tmem_ld_32x32b_x32(t_row + c * kEpiCols, lo);
-    tmem_ld_32x32b_x32(t_row + c * kEpiCols + 32, hi);
-    tmem_ld_wait_regs(lo);
-    tmem_ld_wait_regs(hi);
+    const int x = n0 + c * 32;
+    uint32_t d[32];
+    tmem_ld_32x32b_x32(t_row + c * 32, d);
+    tmem_ld_wait_regs(d);
     if (c == 3) release();
     if (x >= N) continue;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3);
-      const int at = r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+    for (int i = 0; i < 4; ++i) {
+      const int at = gate_piece(i * 8 + (lane >> 2), lane & 3);
       *reinterpret_cast<uint4*>(buf0 + at) = gv[i];
       *reinterpret_cast<uint4*>(buf1 + at) = uv[i];
     }
     __syncwarp();
-    if (c < 3) gate_bwd_fetch(fx, gv, uv, lane, x + kEpiCols, y, M, N);
-    uint32_t pa[32];
+    if (c < 3) gate_bwd_fetch(fx, gv, uv, lane, x + 32, y, M, N);
+    uint32_t pa[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = lane * 128 + ((j ^ (lane & 7)) << 4);
+    for (int j = 0; j < 4; ++j) {
+      const int at = gate_piece(lane, j);
       const uint4 gq = *reinterpret_cast<const uint4*>(buf0 + at);
       const uint4 uq = *reinterpret_cast<const uint4*>(buf1 + at);
       const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w}, uw[4] = {uq.x, uq.y, uq.z, uq.w};
-      const uint32_t* d = (j < 4) ? (lo + 8 * j) : (hi + 8 * (j - 4));
       uint32_t dg[4], du[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 g = unpack_16bit<kBf16>(gw[e]), u = unpack_16bit<kBf16>(uw[e]);
         const ActValue v0 = activate<kAct, true>(g.x), v1 = activate<kAct, true>(g.y);
-        const float d0 = __uint_as_float(d[2 * e]), d1 = __uint_as_float(d[2 * e + 1]);
+        const float d0 = __uint_as_float(d[8 * j + 2 * e]), d1 = __uint_as_float(d[8 * j + 2 * e + 1]);
         pa[4 * j + e] = pack_16bit_rn<kBf16>(__float_as_uint(v0.f * u.x), __float_as_uint(v1.f * u.y));
         dg[e] = pack_16bit_rn<kBf16>(__float_as_uint(d0 * u.x * v0.slope), __float_as_uint(d1 * u.y * v1.slope));
         du[e] = pack_16bit_rn<kBf16>(__float_as_uint(d0 * v0.f), __float_as_uint(d1 * v1.f));
@@ -251,8 +257,8 @@ __device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx
     gate_bwd_store(buf1, fx.du, fx.ld, lane, x, y, M, N);
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<uint4*>(buf0 + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(buf0 + gate_piece(lane, j)) =
           make_uint4(pa[4 * j], pa[4 * j + 1], pa[4 * j + 2], pa[4 * j + 3]);
     __syncwarp();
     gate_bwd_store(buf0, fx.a, fx.ld_a, lane, x, y, M, N);
@@ -261,7 +267,7 @@ __device__ __forceinline__ void gate_bwd_chunks(const FusedArgs<kEpiGateBwd>& fx
 }
 
 template <bool kBf16, typename Release>
-__device__ __forceinline__ void gate_bwd_epilogue(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[8], uint4 (&uv)[8],
+__device__ __forceinline__ void gate_bwd_epilogue(const FusedArgs<kEpiGateBwd>& fx, uint4 (&gv)[4], uint4 (&uv)[4],
                                                   uint32_t t_row, uint8_t* epi_buf, int lane, int n0, int y, int M,
                                                   int N, Release&& release) {
   if (fx.activation == 0)

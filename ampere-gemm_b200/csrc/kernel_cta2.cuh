@@ -69,6 +69,11 @@ struct PairConfig {
                 "split-tail fixup buffers must fit in the pipeline stages");
 };
 
+// Epilogue warps and threads of a CTA.  The backward gate's epilogue has twice
+// as much to do per element as four warps hide behind the MMAs.
+constexpr int pair_epi_warps(int epi) { return epi == kEpiGateBwd ? 8 : kEpiWarps; }
+constexpr int pair_threads(int epi) { return 64 + 32 * pair_epi_warps(epi); }
+
 // kDyn (no split tail): the grid has one cluster per tile; a running pair
 // processes its own tile, then takes the tiles of clusters that have not
 // started yet by cancelling their launch (cluster launch control), so pairs
@@ -78,7 +83,7 @@ struct PairConfig {
 // two-slot queue in shared memory (tile -1 ends the loop).
 template <int STAGES, int KSUB, int MSUB, bool kBRowMajor, bool kAColMajor, int BN = 256, bool kDyn = false,
           bool kBf16 = false, int kEpi = kEpiPlain>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(kEpi), 1)
     gemm_f16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                                  const __grid_constant__ CUtensorMap tmap_b,
                                  const __grid_constant__ CUtensorMap tmap_c, int M, int N, int K, int group_m,
@@ -86,6 +91,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                  const __grid_constant__ FusedArgs<kEpi> fx) {
   using Cfg = PairConfig<STAGES, KSUB, MSUB, BN>;
   constexpr int kAcc = Cfg::kAccBufs;
+  constexpr int kEW = kEpi == kEpiGateBwd ? 8 : kEpiWarps;
   // Columns of C per tile: the gate-and-up tile pairs 128 columns of each.
   constexpr int kOutN = kEpi == kEpiGateUp ? Cfg::kTileN / 2 : Cfg::kTileN;
   static_assert(kEpi == kEpiPlain || (MSUB == 1 && BN == 256), "fused epilogues: 256 x 256 pair tiles");
@@ -137,14 +143,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < kAcc * MSUB; ++a) mbar_init(&tmem_full[a], 1);
-    for (int a = 0; a < kAcc * MSUB; ++a) mbar_init(&tmem_empty[a], 2 * kEpiWarps);
+    for (int a = 0; a < kAcc * MSUB; ++a) mbar_init(&tmem_empty[a], 2 * kEW);
     mbar_init(mma_drain, 1);
     for (int e = 0; e < kEpiWarps; ++e) mbar_init(&c_bar[e], 1);
     for (int e = 0; e < kEpiWarps * kFixBufs; ++e) mbar_init(&fix_bar[e], 1);
     if constexpr (kDyn) {
       for (int q = 0; q < 2; ++q) {
         mbar_init(&tq_full[q], 1);
-        mbar_init(&tq_empty[q], 2 + 2 * kEpiWarps);  // leader MMA, peer producer, both CTAs' epilogue warps
+        mbar_init(&tq_empty[q], 2 + 2 * kEW);  // leader MMA, peer producer, both CTAs' epilogue warps
       }
       mbar_init(clc_bar, 1);
     }
@@ -484,15 +490,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    // ---------------- epilogue warps 2..5 (both CTAs) ----------------
+    // ---------------- epilogue warps 2..5 or 2..9 (both CTAs) ----------------
     const int quad = warp & 3;
     const int ew = warp - 2;
-    uint8_t* epi_buf = smem_epi + ew * 2 * kEpiBufBytes;
+    uint8_t* epi_buf = smem_epi + ew * (Cfg::kEpiBytes / kEW);
     const uint32_t epi_addr = smem_u32(epi_buf);
     int sbuf = 0;
     uint32_t c_phase = 0;
     int local = 0;
-    [[maybe_unused]] uint4 saved_g[8], saved_u[8];
+    // Backward gate: warps 2..5 take the tile's first 128 columns, 6..9 the others.
+    [[maybe_unused]] const int half_col = ew < 4 ? 0 : 128;
+    [[maybe_unused]] uint4 saved_g[4], saved_u[4];
     WorkUnit u;
     auto next_unit = [&](int it, WorkUnit& w) -> bool {
       if constexpr (!kDyn) {
@@ -519,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if constexpr (kEpi == kEpiGateBwd) {
         // The tile's first block of g and u arrives while the MMAs still run.
         const int y = mb * Cfg::kTileM + static_cast<int>(rank) * kBM + quad * 32;
-        gate_bwd_fetch(fx, saved_g, saved_u, lane, n0, y, M, N);
+        gate_bwd_fetch(fx, saved_g, saved_u, lane, n0 + half_col, y, M, N);
       }
       const uint32_t acc_phase = (local / kAcc) & 1;
       bool got = true;
@@ -697,7 +705,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           continue;
         }
         if constexpr (kEpi == kEpiGateBwd) {
-          gate_bwd_epilogue<kBf16>(fx, saved_g, saved_u, t_row, epi_buf, lane, n0, m0 + quad * 32, M, N, [&] {
+          gate_bwd_epilogue<kBf16>(fx, saved_g, saved_u, t_row + half_col, epi_buf, lane, n0 + half_col,
+                                   m0 + quad * 32, M, N, [&] {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[buf * MSUB + s]), 0));
