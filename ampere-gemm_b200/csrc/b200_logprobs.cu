@@ -261,6 +261,20 @@ __device__ __forceinline__ unsigned long long block_bound(unsigned long long key
   return (static_cast<unsigned long long>(t) << 32) | at;
 }
 
+// The same within a warp.
+__device__ __forceinline__ Sums warp_merge(Sums s) {
+  float m = s.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  rebase(s, m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+    s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+  }
+  return s;
+}
+
 struct Outputs {
   float* logprob;
   float* entropy;
@@ -288,15 +302,17 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
   out.logprob[row] = lp;
 }
 
-// One slice (blockIdx.x) of one row (blockIdx.y + i * gridDim.y).  With one
-// slice a row, the row's outputs are written here; otherwise the slice's sums
-// and its top keys, largest first, go to `part_sums` / `part_keys` and
-// logprobs_join_kernel finishes the row.
-template <typename T, bool kTop>
+// One slice (blockIdx.x) of a row, by a block or, for short rows without
+// alternatives, by each of its warps (kRowThreads = 32).  With one slice a row,
+// the row's outputs are written here; otherwise the slice's sums and its top
+// keys, largest first, go to `part_sums` / `part_keys` and logprobs_join_kernel
+// finishes the row.
+template <typename T, bool kTop, int kRowThreads>
 __global__ void __launch_bounds__(kThreads)
     logprobs_fwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows, int64_t vocab,
                         int64_t ld, int64_t slice, int top, int64_t ignore, Outputs out, Sums* __restrict__ part_sums,
                         unsigned long long* __restrict__ part_keys) {
+  static_assert(kRowThreads == kThreads || (kRowThreads == 32 && !kTop), "a block, or a warp without alternatives");
   constexpr int kV = kVec16<T>;
   constexpr int kPacks = kGroup / kV;  // packs of a group
   __shared__ MergeBuffer merge_buf;
@@ -310,8 +326,10 @@ __global__ void __launch_bounds__(kThreads)
   const int slices = gridDim.x;
   const int64_t lo = blockIdx.x * slice;
   const int64_t hi = min(lo + slice, vocab);
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+  constexpr int kRows = kThreads / kRowThreads;  // of a block
+  const int tid = threadIdx.x % kRowThreads;
+  for (int64_t row = static_cast<int64_t>(blockIdx.y) * kRows + threadIdx.x / kRowThreads; row < rows;
+       row += static_cast<int64_t>(gridDim.y) * kRows) {
     const T* x = logits + row * ld;
     // Groups lie between the slice's first aligned element and its last whole
     // one; up to kV - 1 elements come before them and kGroup + kV - 1 after.
@@ -343,14 +361,14 @@ __global__ void __launch_bounds__(kThreads)
       add_group(ps, v, mx, mn);
     };
     int g = tid;
-    for (; g + (kUnroll - 1) * kThreads < groups; g += kUnroll * kThreads) {
+    for (; g + (kUnroll - 1) * kRowThreads < groups; g += kUnroll * kRowThreads) {
       Pack<T, kV> q[kUnroll][kPacks];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) load(q[i], g + i * kThreads);
+      for (int i = 0; i < kUnroll; ++i) load(q[i], g + i * kRowThreads);
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) add(q[i], g + i * kThreads);
+      for (int i = 0; i < kUnroll; ++i) add(q[i], g + i * kRowThreads);
     }
-    for (; g < groups; g += kThreads) {
+    for (; g < groups; g += kRowThreads) {
       Pack<T, kV> q[kPacks];
       load(q, g);
       add(q, g);
@@ -358,7 +376,7 @@ __global__ void __launch_bounds__(kThreads)
     Sums s = merge(Sums{ps.m, ps.z.x, ps.w.x}, Sums{ps.m, ps.z.y, ps.w.y});
     if (lo + tid < span.head_end) add_logit(s, to_f32(x[lo + tid]));
     if (tail + tid < hi) add_logit(s, to_f32(x[tail + tid]));
-    s = block_merge(s, merge_buf);
+    s = kRowThreads == 32 ? warp_merge(s) : block_merge(s, merge_buf);
     if constexpr (kTop) {
       // Threshold: a bound that at least `top` of the threads' best groups and
       // at most kMaxTop threads reach (or every group does).
@@ -425,7 +443,7 @@ __global__ void __launch_bounds__(kThreads)
       else
         part_sums[row * slices + blockIdx.x] = s;
     }
-    __syncthreads();  // the next row reuses the shared arrays
+    if (kRowThreads != 32) __syncthreads();  // the next row reuses the shared arrays
   }
 }
 
@@ -490,7 +508,8 @@ __device__ __forceinline__ float grad_of(float x, const RowGrad& r, bool is_targ
   return is_target ? g + r.gl : g;
 }
 
-template <typename T>
+// One slice (blockIdx.x) of a row, by a block or, for short rows, by each of its warps.
+template <typename T, int kRowThreads>
 __global__ void __launch_bounds__(kThreads)
     logprobs_bwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets,
                         const float2* __restrict__ stats, const float* __restrict__ entropy,
@@ -501,8 +520,10 @@ __global__ void __launch_bounds__(kThreads)
   pdl_wait();
   const int64_t lo = blockIdx.x * slice;
   const int64_t hi = min(lo + slice, vocab);
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+  constexpr int kRows = kThreads / kRowThreads;  // of a block
+  const int tid = threadIdx.x % kRowThreads;
+  for (int64_t row = static_cast<int64_t>(blockIdx.y) * kRows + threadIdx.x / kRowThreads; row < rows;
+       row += static_cast<int64_t>(gridDim.y) * kRows) {
     const T* x = logits + row * ld;
     T* d = dlogits + row * ldd;
     const int64_t target = targets[row];
@@ -511,14 +532,14 @@ __global__ void __launch_bounds__(kThreads)
     const RowGrad r{-st.x, -st.y, entropy[row], gl, g_entropy ? g_entropy[row] : 0.0f};
     if (st.x == kNegInf) {
       // No probability anywhere: nothing depends on the logits.
-      for (int64_t j = lo + tid; j < hi; j += kThreads) d[j] = from_f32<T>(0.0f);
+      for (int64_t j = lo + tid; j < hi; j += kRowThreads) d[j] = from_f32<T>(0.0f);
       continue;
     }
     const Span<T> span(x, lo, hi);
     auto one = [&](int64_t j) { d[j] = from_f32<T>(grad_of(to_f32(x[j]), r, j == target)); };
     if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) != 0) {
       // Logits and gradient are aligned differently.
-      for (int64_t j = lo + tid; j < hi; j += kThreads) one(j);
+      for (int64_t j = lo + tid; j < hi; j += kRowThreads) one(j);
       continue;
     }
     const float2 minus_m = pair_of(r.minus_m), minus_ln_z = pair_of(r.minus_ln_z), log2e = pair_of(kLog2e);
@@ -540,18 +561,18 @@ __global__ void __launch_bounds__(kThreads)
       store_pack<T, kV>(out + static_cast<int64_t>(i) * kV, o);
     };
     int i = tid;
-    for (; i + (kUnroll - 1) * kThreads < packs; i += kUnroll * kThreads) {
+    for (; i + (kUnroll - 1) * kRowThreads < packs; i += kUnroll * kRowThreads) {
       Pack<T, kV> q[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) q[u] = load_pack<T, kV>(body + static_cast<int64_t>(i + u * kThreads) * kV);
+      for (int u = 0; u < kUnroll; ++u) q[u] = load_pack<T, kV>(body + static_cast<int64_t>(i + u * kRowThreads) * kV);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) work(q[u], i + u * kThreads);
+      for (int u = 0; u < kUnroll; ++u) work(q[u], i + u * kRowThreads);
     }
-    for (; i < packs; i += kThreads) work(load_pack<T, kV>(body + static_cast<int64_t>(i) * kV), i);
+    for (; i < packs; i += kRowThreads) work(load_pack<T, kV>(body + static_cast<int64_t>(i) * kV), i);
     if (lo + tid < span.head_end) one(lo + tid);
     if (span.body_end + tid < hi) one(span.body_end + tid);
     // The target's element once more, by the thread that wrote its pack.
-    if (target >= span.head_end && target < span.body_end && (target - span.head_end) / kV % kThreads == tid)
+    if (target >= span.head_end && target < span.body_end && (target - span.head_end) / kV % kRowThreads == tid)
       one(target);
   }
 }
@@ -565,6 +586,18 @@ int with_dtype(int dtype, Fn&& fn) {
   if (dtype == B200_DTYPE_F16) return fn(__half{});
   if (dtype == B200_DTYPE_BF16) return fn(__nv_bfloat16{});
   return fn(float{});
+}
+
+// Rows this short go to a warp each, without alternatives and when there are
+// enough of them to give every SM a block: no barriers, and eight rows' loads
+// side by side.  bf16, us, a block a row -> a warp a row, forward and backward:
+// 100000 x 500: 270 -> 55 and 214 -> 63; 20000 x 5000: 98 -> 54 and 98 -> 79;
+// 8192 x 8192: 40 -> 32 and 47.5 -> 50.5 (2000 x 8192: 11 -> 13 backward).
+constexpr int64_t kWarpRow = 6144;
+
+// Rows of a launch that are not taken by other blocks: gridDim.y.
+unsigned row_blocks(int64_t rows, int per_block) {
+  return (unsigned)std::min<int64_t>((rows + per_block - 1) / per_block, 65535);
 }
 
 // Slices a row is cut into: enough blocks for the device when rows are few
@@ -592,9 +625,9 @@ extern "C" int64_t b200_token_logprobs_workspace_size(int64_t rows, int64_t voca
 }
 
 extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* targets, float* logprob, float* entropy,
-                                       float* stats, float* top_logprob, int64_t* top_index, int64_t rows, int64_t vocab,
-                                       int64_t ld, int top, int64_t ignore_index, int dtype, void* workspace,
-                                       int64_t workspace_bytes, void* stream_ptr) {
+                                       float* stats, float* top_logprob, int64_t* top_index, int64_t rows,
+                                       int64_t vocab, int64_t ld, int top, int64_t ignore_index, int dtype,
+                                       void* workspace, int64_t workspace_bytes, void* stream_ptr) {
   using namespace b200;
   if (rows < 0 || vocab < 0 || top < 0 || top > kMaxTop || top > vocab || !dtype_ok(dtype))
     return B200_ERR_INVALID_ARGUMENT;
@@ -616,14 +649,16 @@ extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* target
   Sums* sums = static_cast<Sums*>(workspace);
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(
       static_cast<uint8_t*>(workspace) + round_up(rows * slices * (int64_t)sizeof(Sums), 256));
-  const dim3 grid((unsigned)slices, (unsigned)std::min<int64_t>(rows, 65535));
+  const bool warp_rows = top == 0 && slices == 1 && vocab <= kWarpRow && rows >= kWarps * dev.sm_count;
+  const dim3 grid((unsigned)slices, row_blocks(rows, warp_rows ? kWarps : 1));
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
-    int rc = cuda_code(top > 0 ? launch_gemm(logprobs_fwd_kernel<T, true>, grid, dim3(kThreads), 0, stream, x, targets,
-                                             rows, vocab, ld, slice, top, ignore_index, out, sums, keys)
-                               : launch_gemm(logprobs_fwd_kernel<T, false>, grid, dim3(kThreads), 0, stream, x,
-                                             targets, rows, vocab, ld, slice, top, ignore_index, out, sums, keys));
+    auto kern = top > 0     ? logprobs_fwd_kernel<T, true, kThreads>
+                : warp_rows ? logprobs_fwd_kernel<T, false, 32>
+                            : logprobs_fwd_kernel<T, false, kThreads>;
+    int rc = cuda_code(launch_gemm(kern, grid, dim3(kThreads), 0, stream, x, targets, rows, vocab, ld, slice, top,
+                                   ignore_index, out, sums, keys));
     if (rc || slices == 1) return rc;
     const dim3 jgrid((unsigned)std::min<int64_t>(rows, 0x7fffffff));
     return cuda_code(top > 0 ? launch_gemm(logprobs_join_kernel<T, true>, jgrid, dim3(kThreads), 0, stream, x, targets,
@@ -650,11 +685,13 @@ extern "C" int b200_token_logprobs_bwd(const void* logits, const int64_t* target
   constexpr int64_t kSlice = 16384;
   const int64_t slice = std::min(kSlice, round_up(vocab, kGroup));
   const int64_t slices = (vocab + slice - 1) / slice;
-  const dim3 grid((unsigned)slices, (unsigned)std::min<int64_t>(rows, 65535));
+  const bool warp_rows = vocab <= kWarpRow && rows >= kWarps * dev.sm_count;
+  const dim3 grid((unsigned)slices, row_blocks(rows, warp_rows ? kWarps : 1));
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    return cuda_code(launch_gemm(logprobs_bwd_kernel<T>, grid, dim3(kThreads), 0, stream,
-                                 static_cast<const T*>(logits), targets, reinterpret_cast<const float2*>(stats), entropy, g_logprob, g_entropy,
-                                 static_cast<T*>(dlogits), rows, vocab, ld, ldd, slice, ignore_index));
+    auto kern = warp_rows ? logprobs_bwd_kernel<T, 32> : logprobs_bwd_kernel<T, kThreads>;
+    return cuda_code(launch_gemm(kern, grid, dim3(kThreads), 0, stream,
+                                 static_cast<const T*>(logits), targets, reinterpret_cast<const float2*>(stats),
+                                 entropy, g_logprob, g_entropy, static_cast<T*>(dlogits), rows, vocab, ld, ldd, slice, ignore_index));
   });
 }

@@ -207,10 +207,10 @@ __global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads
 // Forward for rows longer than the registers of a block hold: one block a
 // row, which is read three times (the second and third from L2).
 template <typename T, typename W>
-__global__ void __launch_bounds__(kLongThreads) layer_norm_fwd_long_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
-                                           T* __restrict__ y, float* __restrict__ mean_out,
-                                           float* __restrict__ rstd_out, int64_t rows, int cols, int64_t ldx,
-                                           int64_t ldy, float eps) {
+__global__ void __launch_bounds__(kLongThreads)
+    layer_norm_fwd_long_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
+                               T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                               int64_t rows, int cols, int64_t ldx, int64_t ldy, float eps) {
   __shared__ __align__(16) float red[2][32];
   pdl_wait();
   const float inv_n = 1.0f / static_cast<float>(cols);
@@ -418,10 +418,10 @@ __global__ void __launch_bounds__(TPR == 320 ? TPR : kBwdThreads, TPR == 320 ? 2
 
 // dx for rows longer than a block's registers hold: one block a row.
 template <typename T, typename W>
-__global__ void __launch_bounds__(kLongThreads) layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
-                                           const float* __restrict__ mean, const float* __restrict__ rstd_in,
-                                           T* __restrict__ dx, int64_t rows, int cols, int64_t lddy, int64_t ldx,
-                                           int64_t lddx) {
+__global__ void __launch_bounds__(kLongThreads)
+    layer_norm_bwd_long_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
+                               const float* __restrict__ mean, const float* __restrict__ rstd_in, T* __restrict__ dx,
+                               int64_t rows, int cols, int64_t lddy, int64_t ldx, int64_t lddx) {
   __shared__ __align__(16) float red[2][32];
   pdl_wait();
   const float inv_n = 1.0f / static_cast<float>(cols);
@@ -692,8 +692,9 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const int size = dtype_size(dtype), n = static_cast<int>(cols);
-  const int elems = std::min({row_vec(n, size, dtype_size(wdtype), x, ldx), row_vec(n, size, dtype_size(wdtype), y, ldy),
-                              row_vec(n, dtype_size(wdtype), size, w, 0), row_vec(n, dtype_size(wdtype), size, b, 0)});
+  const int w_size = dtype_size(wdtype);
+  const int elems = std::min({row_vec(n, size, w_size, x, ldx), row_vec(n, size, w_size, y, ldy),
+                              row_vec(n, w_size, size, w, 0), row_vec(n, w_size, size, b, 0)});
   return with_types(dtype, wdtype, [&](auto t, auto wt) {
     using T = decltype(t);
     using W = decltype(wt);

@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       const uint32_t bar = full0 + stage * 8;
       uint32_t dst = smem0 + stage * stage_bytes + kAccs * sh.block_pad * 128;
       int k = (kb0 + k_stage(it) * sh.k_sub) * kBK;
-      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK) tma_load_2d_if(el, dst, &tmap_x, bar, k, t_tile, pol_x);
+      for (int j = 0; j < n_sub; ++j, dst += sub_bytes, k += kBK)
+        tma_load_2d_if(el, dst, &tmap_x, bar, k, t_tile, pol_x);
     };
     const int first = min(num_stages, sh.stages);
     if (sh.w_early)
@@ -329,7 +330,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     }
   } else if (warp == 1) {
     const uint32_t el = elect_lane();
-    const uint32_t idesc = make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad), kWMajorN ? Major::kMN : Major::kK,
+    const uint32_t idesc = make_idesc_f16_f32(128, static_cast<uint32_t>(sh.tokens_pad),
+                                              kWMajorN ? Major::kMN : Major::kK,
                                               Major::kK, kBf16);
     // Descriptors advance by adding to their address field (units of 16 bytes;
     // addresses stay below 2^18).

@@ -53,7 +53,8 @@ def _forward(x, weight, bias, eps: float, stats: bool):
         bias = None if bias is None else bias.contiguous()
         mean = ptr(stats)
         launch("b200_layer_norm_fwd", x.get_device(), x2.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), mean,
-               None if mean is None else mean + 4 * rows, rows, cols, ldx, cols, DTYPE_CODES[x.dtype], DTYPE_CODES[_wdtype(x, weight, bias)], eps)
+               None if mean is None else mean + 4 * rows, rows, cols, ldx, cols, DTYPE_CODES[x.dtype],
+               DTYPE_CODES[_wdtype(x, weight, bias)], eps)
     return y, stats
 
 

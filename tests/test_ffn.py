@@ -26,7 +26,8 @@ E19 = 2.0 ** -19
 def make(rows, dim, hidden, out_dim, dtype, dev, seed=0):
     gen = torch.Generator().manual_seed(rows + 10 * dim + 100 * hidden + seed)
     t = lambda r, c, s: (s * torch.randn((r, c), generator=gen)).to(dtype).to(dev)
-    return (t(rows, dim, 1.0), t(2 * hidden, dim, dim ** -0.5), t(out_dim, hidden, hidden ** -0.5), t(rows, out_dim, 1.0))
+    return (t(rows, dim, 1.0), t(2 * hidden, dim, dim ** -0.5), t(out_dim, hidden, hidden ** -0.5),
+            t(rows, out_dim, 1.0))
 
 
 def act64(kind, g):
@@ -114,7 +115,8 @@ def check_all(x, w_in, w_out, kind, dy):
 
 
 # rows, dim, hidden, out_dim: one row, few, odd ones, sizes around the tiles (256 rows, 128 hidden units, 64 deep)
-SIZES = [(1, 8, 8, 8), (1, 256, 512, 256), (3, 64, 128, 64), (17, 100, 60, 100), (33, 129, 131, 65), (128, 128, 128, 128),
+SIZES = [(1, 8, 8, 8), (1, 256, 512, 256), (3, 64, 128, 64), (17, 100, 60, 100), (33, 129, 131, 65),
+         (128, 128, 128, 128),
          (130, 200, 264, 200), (256, 512, 1000, 512), (257, 511, 1001, 510), (700, 96, 384, 104), (1500, 320, 72, 320),
          (64, 1024, 2816, 1024), (2, 2000, 33, 7), (520, 384, 776, 392), (1111, 130, 267, 131), (300, 2048, 136, 72),
          (2600, 64, 200, 264)]
