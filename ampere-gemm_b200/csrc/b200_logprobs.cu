@@ -207,20 +207,51 @@ __device__ __forceinline__ Sums block_merge(Sums s, MergeBuffer& buf) {
   return r;
 }
 
-// A lower bound of the top k of the block's keys (one a thread; 0 for none; all
-// others differ), which at least k of them and at most max(k, kMaxTop) reach;
-// 0 when there are no more than k.  Found bit by bit from the first in which
-// the keys differ: the values' bits, of which those below `low` are alike
-// for values of one sign (16-bit types), then, if too many values are equal, the indexes'.
 // Lowest bit of fp32 that a value of the type can have (other than by its sign).
 template <typename T>
 constexpr int kLowBit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
 struct KthBuffer {
+  __align__(16) uint32_t part[kMaxTop];
+  uint32_t kth;
   uint32_t most[kWarps], least[kWarps];
 };
-__device__ __forceinline__ unsigned long long block_bound(unsigned long long key, int k, int low, KthBuffer& buf) {
+
+// A lower bound of the top k of the block's keys (one a thread; 0 for none; all
+// others differ), which at least k of them (or all) and at most kMaxTop reach.
+// First try: the value of the k-th best of the maxima of `per` neighbouring
+// threads, 1 (keys in the first kMaxTop threads only), 4 or 32 (k <= kWarps).
+// If too many reach that, bit by bit from the first in which the keys differ:
+// the values' bits, of which those below `low` are alike for values of one sign
+// (16-bit types), then, if too many values are equal, the indexes'.  Bits alone,
+// a barrier each, took SLOW_NOTE us for 4096 x 50257 bf16, top 5, instead of FAST_NOTE.
+__device__ __forceinline__ unsigned long long block_bound(unsigned long long key, int k, int per, int low,
+                                                          KthBuffer& buf) {
   const uint32_t v = static_cast<uint32_t>(key >> 32);
-  if (__syncthreads_count(key != 0) <= k) return 0;
+  const int parts = per == 32 ? kWarps : kMaxTop;
+  uint32_t b = v;
+  if (per == 4) {
+    b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
+    b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
+  } else if (per == 32) {
+    b = __reduce_max_sync(0xffffffffu, b);
+  }
+  const int part = static_cast<int>(threadIdx.x) / per;
+  if (threadIdx.x % per == 0 && part < parts) buf.part[part] = b;
+  __syncthreads();
+  if (threadIdx.x < parts) {
+    const uint32_t own = buf.part[threadIdx.x];
+    int before = 0;
+    for (int j = 0; j < parts; j += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(&buf.part[j]);
+      const int i = static_cast<int>(threadIdx.x);
+      before += (q.x > own || (q.x == own && j < i)) + (q.y > own || (q.y == own && j + 1 < i)) +
+                (q.z > own || (q.z == own && j + 2 < i)) + (q.w > own || (q.w == own && j + 3 < i));
+    }
+    if (before == k - 1) buf.kth = own;
+  }
+  __syncthreads();
+  const uint32_t kth = buf.kth;
+  if (__syncthreads_count(key != 0 && v >= kth) <= kMaxTop) return static_cast<unsigned long long>(kth) << 32;
   const uint32_t most = __reduce_max_sync(0xffffffffu, v), least = __reduce_min_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) {
     buf.most[threadIdx.x >> 5] = most;
@@ -283,22 +314,19 @@ struct Outputs {
   int64_t* top_index;
 };
 
+// The given token's logit; a target outside the vocabulary has no probability to give.
 template <typename T>
-__device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const T* x, int64_t vocab, int64_t target,
-                                          int64_t ignore, Sums s) {
+__device__ __forceinline__ float target_logit(const T* x, int64_t vocab, int64_t target) {
+  return target < 0 || target >= vocab ? __uint_as_float(0x7fffffffu) : to_f32(x[target]);
+}
+
+__device__ __forceinline__ void write_row(const Outputs& out, int64_t row, bool given, float logit, Sums s) {
   const bool empty = s.m == kNegInf;
   const float ln_z = logf(s.z);
   if (out.stats) out.stats[row] = make_float2(s.m, ln_z);
   out.entropy[row] = empty ? 0.0f : ln_z - s.w / s.z;
   float lp = 0.0f;
-  if (target != ignore) {
-    // A target outside the vocabulary has no probability to give.
-    if (target < 0 || target >= vocab) {
-      lp = __uint_as_float(0x7fffffffu);
-    } else {
-      lp = empty ? kNegInf : (to_f32(x[target]) - s.m) - ln_z;
-    }
-  }
+  if (given) lp = empty && logit == kNegInf ? kNegInf : (logit - s.m) - ln_z;
   out.logprob[row] = lp;
 }
 
@@ -318,7 +346,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ MergeBuffer merge_buf;
   __shared__ KthBuffer kth_buf;
   __shared__ float group_max[kTop ? kTopGroups : 1];
-  __shared__ uint32_t cand[kTop ? kMaxCand : 1];
+  __shared__ uint16_t cand[kTop ? kMaxCand : 1];
   __shared__ unsigned long long elems[kTop ? kMaxElems : 1];
   __shared__ unsigned long long bound;
   __shared__ int count[2];
@@ -331,6 +359,8 @@ __global__ void __launch_bounds__(kThreads)
   for (int64_t row = static_cast<int64_t>(blockIdx.y) * kRows + threadIdx.x / kRowThreads; row < rows;
        row += static_cast<int64_t>(gridDim.y) * kRows) {
     const T* x = logits + row * ld;
+    // Requested now, needed at the row's end.
+    const int64_t target = tid == 0 && slices == 1 ? targets[row] : ignore;
     // Groups lie between the slice's first aligned element and its last whole
     // one; up to kV - 1 elements come before them and kGroup + kV - 1 after.
     const Span<T> span(x, lo, hi);
@@ -374,8 +404,11 @@ __global__ void __launch_bounds__(kThreads)
       add(q, g);
     }
     Sums s = merge(Sums{ps.m, ps.z.x, ps.w.x}, Sums{ps.m, ps.z.y, ps.w.y});
-    if (lo + tid < span.head_end) add_logit(s, to_f32(x[lo + tid]));
-    if (tail + tid < hi) add_logit(s, to_f32(x[tail + tid]));
+    const bool has_head = lo + tid < span.head_end, has_tail = tail + tid < hi;
+    const float head_v = has_head ? to_f32(x[lo + tid]) : kNegInf, tail_v = has_tail ? to_f32(x[tail + tid]) : kNegInf;
+    const float target_v = target != ignore ? target_logit(x, vocab, target) : 0.0f;
+    if (has_head) add_logit(s, head_v);
+    if (has_tail) add_logit(s, tail_v);
     s = kRowThreads == 32 ? warp_merge(s) : block_merge(s, merge_buf);
     if constexpr (kTop) {
       // Threshold: a bound that at least `top` of the threads' best groups and
@@ -392,32 +425,51 @@ __global__ void __launch_bounds__(kThreads)
         count[0] = count[1] = 0;
         bound = 0;
       }
-      const unsigned long long thr = block_bound(best, top, kLowBit<T>, kth_buf);
-      if (best >= thr)
-        for (int i = tid; i < groups; i += kThreads)
-          if (make_key(group_max[i], i) >= thr) cand[atomicAdd(&count[0], 1)] = i;
-      __syncthreads();
-      // Of the candidates, the best `top` groups; the last of them bounds the
-      // elements that can be among the top from below.
-      const int n_cand = count[0];
-      for (int i = tid; i < n_cand; i += kThreads) {
-        const unsigned long long k = make_key(group_max[cand[i]], cand[i]);
-        int r = 0;
-        for (int j = 0; j < n_cand; ++j) r += make_key(group_max[cand[j]], cand[j]) > k;
-        if (r == top - 1) bound = k;
+      const int per = groups <= kMaxTop ? 1 : groups < kThreads || top > kWarps ? 4 : 32;
+      const unsigned long long thr = block_bound(best, top, per, kLowBit<T>, kth_buf);
+      if (best >= thr) {
+        // Maxima below the bound's value (not NaN, nor anything below NaN) are out; the rest by key.
+        const float thr_v = thr ? key_value(thr) : kNegInf;
+        for (int i = tid; i < groups; i += 4 * kThreads) {
+          float m[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) m[u] = group_max[min(i + u * kThreads, groups - 1)];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int c = i + u * kThreads;
+            if (c < groups && !(m[u] < thr_v) && make_key(m[u], c) >= thr)
+              cand[atomicAdd(&count[0], 1)] = static_cast<uint16_t>(c);
+          }
+        }
       }
       __syncthreads();
-      const uint32_t least = static_cast<uint32_t>(bound >> 32);
-      auto offer = [&](int64_t j) {
-        const float v = to_f32(x[j]);
+      const int n_cand = count[0];
+      unsigned long long least_group = thr;
+      if (n_cand * kGroup > kThreads) {
+        // Of many candidates the best `top` groups only; the last of them
+        // bounds the elements that can be among the top from below.
+        for (int i = tid; i < n_cand; i += kThreads) {
+          const unsigned long long k = make_key(group_max[cand[i]], cand[i]);
+          int r = 0;
+          for (int j = 0; j < n_cand; ++j) r += make_key(group_max[cand[j]], cand[j]) > k;
+          if (r == top - 1) bound = k;
+        }
+        __syncthreads();
+        least_group = bound;
+      }
+      const uint32_t least = static_cast<uint32_t>(least_group >> 32);
+      auto offer = [&](float v, int64_t j) {
         if (order_bits(v) >= least) elems[atomicAdd(&count[1], 1)] = make_key(v, static_cast<uint32_t>(j));
       };
       for (int i = tid; i < n_cand * kGroup; i += kThreads) {
         const uint32_t c = cand[i / kGroup];
-        if (make_key(group_max[c], c) >= bound) offer(span.head_end + static_cast<int64_t>(c) * kGroup + i % kGroup);
+        if (make_key(group_max[c], c) >= least_group) {
+          const int64_t j = span.head_end + static_cast<int64_t>(c) * kGroup + i % kGroup;
+          offer(to_f32(x[j]), j);
+        }
       }
-      if (lo + tid < span.head_end) offer(lo + tid);
-      if (tail + tid < hi) offer(tail + tid);
+      if (has_head) offer(head_v, lo + tid);
+      if (has_tail) offer(tail_v, tail + tid);
       __syncthreads();
       const int n = count[1];
       const float ln_z = logf(s.z);
@@ -439,7 +491,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (tid == 0) {
       if (slices == 1)
-        write_row<T>(out, row, x, vocab, targets[row], ignore, s);
+        write_row(out, row, target != ignore, target_v, s);
       else
         part_sums[row * slices + blockIdx.x] = s;
     }
@@ -461,6 +513,8 @@ __global__ void __launch_bounds__(kThreads)
   pdl_wait();
   const int tid = threadIdx.x;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int64_t target = tid == 0 ? targets[row] : ignore;
+    const float target_v = target != ignore ? target_logit(logits + row * ld, vocab, target) : 0.0f;
     Sums s{kNegInf, 0.0f, 0.0f};
     for (int i = tid; i < slices; i += kThreads) s = merge(s, part_sums[row * slices + i]);
     s = block_merge(s, merge_buf);
@@ -470,7 +524,7 @@ __global__ void __launch_bounds__(kThreads)
       const unsigned long long* keys = part_keys + (row * slices + tid) * top;
       if (tid == 0) count = 0;
       const unsigned long long first = tid < slices ? keys[0] : 0;
-      const unsigned long long thr = block_bound(first, top, kLowBit<T>, kth_buf);
+      const unsigned long long thr = block_bound(first, top, slices <= kMaxTop ? 1 : 4, kLowBit<T>, kth_buf);
       if (first != 0 && first >= thr)
         for (int i = 0; i < top; ++i) {
           const unsigned long long k = keys[i];
@@ -490,7 +544,7 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    if (tid == 0) write_row<T>(out, row, logits + row * ld, vocab, targets[row], ignore, s);
+    if (tid == 0) write_row(out, row, target != ignore, target_v, s);
     __syncthreads();
   }
 }
