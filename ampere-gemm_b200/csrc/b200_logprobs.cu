@@ -36,12 +36,14 @@ constexpr int kGroup = 8;
 // Longest slice of a row that one block takes when alternatives are wanted:
 // 8192 groups, 32 KB of maxima, 32 groups a thread.
 constexpr int kTopSlice = 65536;
-constexpr int kTopGroups = kTopSlice / kGroup;
-// Candidate groups after the threshold: those of the threads whose best group
-// reaches it, kMaxTop of them with kTopGroups / kThreads each at most.
-constexpr int kMaxCand = kMaxTop * (kTopGroups / kThreads);
-// Elements of the top groups, and those before the first and after the last.
-constexpr int kMaxElems = kMaxTop * kGroup + 4 * kGroup;
+// Rows this short go to a warp each when there are enough of them to give every
+// SM a block, with kWarpTop alternatives at most: no barriers, and eight rows'
+// loads side by side.  bf16, us, a block a row -> a warp a row: 100000 x 500
+// forward 270 -> 55, backward 214 -> 63, top 5 TOPA; 20000 x 5000 98 -> 54,
+// 98 -> 79, TOPB; 8192 x 8192 40 -> 32, 47.5 -> 50.5 (2000 x 8192: 11 -> 13
+// backward).
+constexpr int kWarpRow = 6144;
+constexpr int kWarpTop = 16;
 // Slices of a row at most when alternatives are wanted: one a thread of the join.
 constexpr int kMaxTopVocab = kTopSlice * kThreads;
 // Groups of a thread that are on their way at once.
@@ -210,20 +212,94 @@ __device__ __forceinline__ Sums block_merge(Sums s, MergeBuffer& buf) {
 // Lowest bit of fp32 that a value of the type can have (other than by its sign).
 template <typename T>
 constexpr int kLowBit = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+
+// Shared memory of the selection in a row (slice) of kRowThreads threads.
+template <int kRowThreads>
+struct Selection {
+  static constexpr int kMost = kRowThreads == 32 ? kWarpTop : kMaxTop;  // alternatives
+  static constexpr int kGroups = (kRowThreads == 32 ? kWarpRow : kTopSlice) / kGroup;
+  // Candidates whose elements are offered without ranking them: one a thread,
+  // about, and no more than `elems` holds.
+  static constexpr int kFewCand = kRowThreads == 32 ? kMost : kRowThreads / kGroup;
+  float group_max[kGroups];
+  // Elements of the top groups, and those before the first and after the last.
+  unsigned long long elems[kMost * kGroup + 4 * kGroup];
+  // Candidate groups after the threshold: all those of kMost threads at most.
+  uint16_t cand[kMost * (kGroups / kRowThreads)];
+  unsigned long long bound;
+  int count[2];
+};
+struct Nothing {};
+
+template <int kRowThreads>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (kRowThreads == 32)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+template <int kRowThreads>
+__device__ __forceinline__ int row_count(bool p) {
+  if constexpr (kRowThreads == 32)
+    return __popc(__ballot_sync(0xffffffffu, p));
+  else
+    return __syncthreads_count(p);
+}
+
+// A lower bound of the top k of the keys of a row's threads (one each; 0 for
+// none; all others differ), which at least k of them (or all) and at most `most`
+// reach.  Found bit by bit from the first in which the keys differ: the values'
+// bits, of which those below `low` are alike for values of one sign (16-bit
+// types), then, if too many values are equal, the indexes'.  `hi` and `lo`: the
+// largest and smallest value among the keys.
+template <int kRowThreads>
+__device__ __forceinline__ unsigned long long bound_by_bits(unsigned long long key, int k, int most, int low,
+                                                            uint32_t hi, uint32_t lo) {
+  const uint32_t v = static_cast<uint32_t>(key >> 32);
+  const int first = 31 - __clz((hi ^ lo) | 1u);
+  uint32_t t = first == 31 ? 0u : hi >> (first + 1) << (first + 1);
+  int reach = kRowThreads;  // keys that reach t
+  for (int bit = first; bit >= low; --bit) {
+    const uint32_t u = t | (1u << bit);
+    const int c = row_count<kRowThreads>(v >= u);
+    if (c >= k) {
+      t = u;
+      reach = c;
+    }
+    if (c == k) break;
+  }
+  if (reach <= most) return static_cast<unsigned long long>(t) << 32;
+  // Too many equal values at t (whose bits below `low` are all ones for a
+  // negative value, see order_bits): their indexes decide.
+  if ((t & 0x80000000u) == 0) t |= (1u << low) - 1;
+  const bool tied = key != 0 && v == t;
+  const int above = row_count<kRowThreads>(v > t);
+  uint32_t at = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t u = at | (1u << bit);
+    const int c = above + row_count<kRowThreads>(tied && static_cast<uint32_t>(key) >= u);
+    if (c >= k) at = u;
+    if (c == k) break;
+  }
+  return (static_cast<unsigned long long>(t) << 32) | at;
+}
+
+// The same for the keys of a warp.
+__device__ __forceinline__ unsigned long long warp_bound(unsigned long long key, int k, int low) {
+  const uint32_t v = static_cast<uint32_t>(key >> 32);
+  if (row_count<32>(key != 0) <= k) return 0;
+  return bound_by_bits<32>(key, k, kWarpTop, low, __reduce_max_sync(0xffffffffu, v), __reduce_min_sync(0xffffffffu, v));
+}
+
+// The same for the keys of a block, kMaxTop at most.  First try: the value of
+// the k-th best of the maxima of `per` neighbouring threads, 1 (keys in the
+// first kMaxTop threads only), 4 or 32 (k <= kWarps): three barriers, where one
+// a bit takes about fifteen.
 struct KthBuffer {
   __align__(16) uint32_t part[kMaxTop];
   uint32_t kth;
   uint32_t most[kWarps], least[kWarps];
 };
-
-// A lower bound of the top k of the block's keys (one a thread; 0 for none; all
-// others differ), which at least k of them (or all) and at most kMaxTop reach.
-// First try: the value of the k-th best of the maxima of `per` neighbouring
-// threads, 1 (keys in the first kMaxTop threads only), 4 or 32 (k <= kWarps).
-// If too many reach that, bit by bit from the first in which the keys differ:
-// the values' bits, of which those below `low` are alike for values of one sign
-// (16-bit types), then, if too many values are equal, the indexes'.  Bits alone,
-// a barrier each, took SLOW_NOTE us for 4096 x 50257 bf16, top 5, instead of FAST_NOTE.
 __device__ __forceinline__ unsigned long long block_bound(unsigned long long key, int k, int per, int low,
                                                           KthBuffer& buf) {
   const uint32_t v = static_cast<uint32_t>(key >> 32);
@@ -240,10 +316,10 @@ __device__ __forceinline__ unsigned long long block_bound(unsigned long long key
   __syncthreads();
   if (threadIdx.x < parts) {
     const uint32_t own = buf.part[threadIdx.x];
+    const int i = static_cast<int>(threadIdx.x);
     int before = 0;
     for (int j = 0; j < parts; j += 4) {
       const uint4 q = *reinterpret_cast<const uint4*>(&buf.part[j]);
-      const int i = static_cast<int>(threadIdx.x);
       before += (q.x > own || (q.x == own && j < i)) + (q.y > own || (q.y == own && j + 1 < i)) +
                 (q.z > own || (q.z == own && j + 2 < i)) + (q.w > own || (q.w == own && j + 3 < i));
     }
@@ -264,35 +340,10 @@ __device__ __forceinline__ unsigned long long block_bound(unsigned long long key
     hi = max(hi, buf.most[i]);
     lo = min(lo, buf.least[i]);
   }
-  const int first = 31 - __clz((hi ^ lo) | 1u);
-  uint32_t t = first == 31 ? 0u : hi >> (first + 1) << (first + 1);
-  int reach = kThreads;  // keys that reach t
-  for (int bit = first; bit >= low; --bit) {
-    const uint32_t u = t | (1u << bit);
-    const int c = __syncthreads_count(v >= u);
-    if (c >= k) {
-      t = u;
-      reach = c;
-    }
-    if (c == k) break;
-  }
-  if (reach <= kMaxTop) return static_cast<unsigned long long>(t) << 32;
-  // Too many equal values at t (whose bits below `low` are all ones for a
-  // negative value, see order_bits): their indexes decide.
-  if ((t & 0x80000000u) == 0) t |= (1u << low) - 1;
-  const bool tied = key != 0 && v == t;
-  const int above = __syncthreads_count(v > t);
-  uint32_t at = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t u = at | (1u << bit);
-    const int c = above + __syncthreads_count(tied && static_cast<uint32_t>(key) >= u);
-    if (c >= k) at = u;
-    if (c == k) break;
-  }
-  return (static_cast<unsigned long long>(t) << 32) | at;
+  return bound_by_bits<kThreads>(key, k, kMaxTop, low, hi, lo);
 }
 
-// The same within a warp.
+// A warp's sums, for every thread.
 __device__ __forceinline__ Sums warp_merge(Sums s) {
   float m = s.m;
 #pragma unroll
@@ -330,9 +381,8 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, bool 
   out.logprob[row] = lp;
 }
 
-// One slice (blockIdx.x) of a row, by a block or, for short rows without
-// alternatives, by each of its warps (kRowThreads = 32).  With one slice a row,
-// the row's outputs are written here; otherwise the slice's sums and its top
+// One slice (blockIdx.x) of a row, by a block or, for short rows, by each of its
+// warps (kRowThreads = 32).  With one slice a row, the row's outputs are written here; otherwise the slice's sums and its top
 // keys, largest first, go to `part_sums` / `part_keys` and logprobs_join_kernel
 // finishes the row.
 template <typename T, bool kTop, int kRowThreads>
@@ -340,22 +390,19 @@ __global__ void __launch_bounds__(kThreads)
     logprobs_fwd_kernel(const T* __restrict__ logits, const int64_t* __restrict__ targets, int64_t rows, int64_t vocab,
                         int64_t ld, int64_t slice, int top, int64_t ignore, Outputs out, Sums* __restrict__ part_sums,
                         unsigned long long* __restrict__ part_keys) {
-  static_assert(kRowThreads == kThreads || (kRowThreads == 32 && !kTop), "a block, or a warp without alternatives");
+  using Sel = Selection<kRowThreads>;
   constexpr int kV = kVec16<T>;
   constexpr int kPacks = kGroup / kV;  // packs of a group
   __shared__ MergeBuffer merge_buf;
   __shared__ KthBuffer kth_buf;
-  __shared__ float group_max[kTop ? kTopGroups : 1];
-  __shared__ uint16_t cand[kTop ? kMaxCand : 1];
-  __shared__ unsigned long long elems[kTop ? kMaxElems : 1];
-  __shared__ unsigned long long bound;
-  __shared__ int count[2];
+  __shared__ std::conditional_t<kTop, Sel, Nothing> sel_buf[kThreads / kRowThreads];
   pdl_wait();
   const int slices = gridDim.x;
   const int64_t lo = blockIdx.x * slice;
   const int64_t hi = min(lo + slice, vocab);
   constexpr int kRows = kThreads / kRowThreads;  // of a block
   const int tid = threadIdx.x % kRowThreads;
+  auto& sel = sel_buf[threadIdx.x / kRowThreads];
   for (int64_t row = static_cast<int64_t>(blockIdx.y) * kRows + threadIdx.x / kRowThreads; row < rows;
        row += static_cast<int64_t>(gridDim.y) * kRows) {
     const T* x = logits + row * ld;
@@ -380,8 +427,8 @@ __global__ void __launch_bounds__(kThreads)
       const float mx = max_nan(max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x),
                                max3_nan(v[2].y, v[3].x, v[3].y));
       const float mn = fminf(min3(min3(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x), min3(v[2].y, v[3].x, v[3].y));
-      if (kTop) {
-        group_max[g] = mx;
+      if constexpr (kTop) {
+        sel.group_max[g] = mx;
         // Strictly larger only: of equal groups the first stays.
         if (!(mx <= best_max)) {
           best_max = mx;
@@ -412,71 +459,77 @@ __global__ void __launch_bounds__(kThreads)
     s = kRowThreads == 32 ? warp_merge(s) : block_merge(s, merge_buf);
     if constexpr (kTop) {
       // Threshold: a bound that at least `top` of the threads' best groups and
-      // at most kMaxTop threads reach (or every group does).
+      // at most Sel::kMost threads reach (or every group does).
       unsigned long long best = best_group >= 0 ? make_key(best_max, best_group) : 0;
       if (s.m != s.m) {
         // A NaN in the row: comparisons above may have dropped it.
-        for (int i = tid; i < groups; i += kThreads) {
-          const unsigned long long k = make_key(group_max[i], i);
+        for (int i = tid; i < groups; i += kRowThreads) {
+          const unsigned long long k = make_key(sel.group_max[i], i);
           best = k > best ? k : best;
         }
       }
       if (tid == 0) {
-        count[0] = count[1] = 0;
-        bound = 0;
+        sel.count[0] = sel.count[1] = 0;
+        sel.bound = 0;
       }
-      const int per = groups <= kMaxTop ? 1 : groups < kThreads || top > kWarps ? 4 : 32;
-      const unsigned long long thr = block_bound(best, top, per, kLowBit<T>, kth_buf);
+      unsigned long long thr;
+      if constexpr (kRowThreads == 32) {
+        __syncwarp();
+        thr = warp_bound(best, top, kLowBit<T>);
+      } else {
+        const int per = groups <= kMaxTop ? 1 : groups < kRowThreads || top > kWarps ? 4 : 32;
+        thr = block_bound(best, top, per, kLowBit<T>, kth_buf);
+      }
       if (best >= thr) {
         // Maxima below the bound's value (not NaN, nor anything below NaN) are out; the rest by key.
         const float thr_v = thr ? key_value(thr) : kNegInf;
-        for (int i = tid; i < groups; i += 4 * kThreads) {
+        for (int i = tid; i < groups; i += 4 * kRowThreads) {
           float m[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) m[u] = group_max[min(i + u * kThreads, groups - 1)];
+          for (int u = 0; u < 4; ++u) m[u] = sel.group_max[min(i + u * kRowThreads, groups - 1)];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int c = i + u * kThreads;
+            const int c = i + u * kRowThreads;
             if (c < groups && !(m[u] < thr_v) && make_key(m[u], c) >= thr)
-              cand[atomicAdd(&count[0], 1)] = static_cast<uint16_t>(c);
+              sel.cand[atomicAdd(&sel.count[0], 1)] = static_cast<uint16_t>(c);
           }
         }
       }
-      __syncthreads();
-      const int n_cand = count[0];
+      row_sync<kRowThreads>();
+      const int n_cand = sel.count[0];
       unsigned long long least_group = thr;
-      if (n_cand * kGroup > kThreads) {
+      if (n_cand > Sel::kFewCand) {
         // Of many candidates the best `top` groups only; the last of them
         // bounds the elements that can be among the top from below.
-        for (int i = tid; i < n_cand; i += kThreads) {
-          const unsigned long long k = make_key(group_max[cand[i]], cand[i]);
+        for (int i = tid; i < n_cand; i += kRowThreads) {
+          const unsigned long long k = make_key(sel.group_max[sel.cand[i]], sel.cand[i]);
           int r = 0;
-          for (int j = 0; j < n_cand; ++j) r += make_key(group_max[cand[j]], cand[j]) > k;
-          if (r == top - 1) bound = k;
+          for (int j = 0; j < n_cand; ++j) r += make_key(sel.group_max[sel.cand[j]], sel.cand[j]) > k;
+          if (r == top - 1) sel.bound = k;
         }
-        __syncthreads();
-        least_group = bound;
+        row_sync<kRowThreads>();
+        least_group = sel.bound;
       }
       const uint32_t least = static_cast<uint32_t>(least_group >> 32);
       auto offer = [&](float v, int64_t j) {
-        if (order_bits(v) >= least) elems[atomicAdd(&count[1], 1)] = make_key(v, static_cast<uint32_t>(j));
+        if (order_bits(v) >= least) sel.elems[atomicAdd(&sel.count[1], 1)] = make_key(v, static_cast<uint32_t>(j));
       };
-      for (int i = tid; i < n_cand * kGroup; i += kThreads) {
-        const uint32_t c = cand[i / kGroup];
-        if (make_key(group_max[c], c) >= least_group) {
+      for (int i = tid; i < n_cand * kGroup; i += kRowThreads) {
+        const uint32_t c = sel.cand[i / kGroup];
+        if (make_key(sel.group_max[c], c) >= least_group) {
           const int64_t j = span.head_end + static_cast<int64_t>(c) * kGroup + i % kGroup;
           offer(to_f32(x[j]), j);
         }
       }
       if (has_head) offer(head_v, lo + tid);
       if (has_tail) offer(tail_v, tail + tid);
-      __syncthreads();
-      const int n = count[1];
+      row_sync<kRowThreads>();
+      const int n = sel.count[1];
       const float ln_z = logf(s.z);
-      for (int i = tid; i < n; i += kThreads) {
-        const unsigned long long k = elems[i];
+      for (int i = tid; i < n; i += kRowThreads) {
+        const unsigned long long k = sel.elems[i];
         int r = 0;
-        for (int j = 0; j < n; ++j) r += elems[j] > k;
+        for (int j = 0; j < n; ++j) r += sel.elems[j] > k;
         if (r < top) {
           if (slices == 1) {
             out.top_index[row * top + r] = key_index(k);
@@ -495,7 +548,7 @@ __global__ void __launch_bounds__(kThreads)
       else
         part_sums[row * slices + blockIdx.x] = s;
     }
-    if (kRowThreads != 32) __syncthreads();  // the next row reuses the shared arrays
+    row_sync<kRowThreads>();  // the next row reuses the shared arrays
   }
 }
 
@@ -642,13 +695,6 @@ int with_dtype(int dtype, Fn&& fn) {
   return fn(float{});
 }
 
-// Rows this short go to a warp each, without alternatives and when there are
-// enough of them to give every SM a block: no barriers, and eight rows' loads
-// side by side.  bf16, us, a block a row -> a warp a row, forward and backward:
-// 100000 x 500: 270 -> 55 and 214 -> 63; 20000 x 5000: 98 -> 54 and 98 -> 79;
-// 8192 x 8192: 40 -> 32 and 47.5 -> 50.5 (2000 x 8192: 11 -> 13 backward).
-constexpr int64_t kWarpRow = 6144;
-
 // Rows of a launch that are not taken by other blocks: gridDim.y.
 unsigned row_blocks(int64_t rows, int per_block) {
   return (unsigned)std::min<int64_t>((rows + per_block - 1) / per_block, 65535);
@@ -703,14 +749,13 @@ extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* target
   Sums* sums = static_cast<Sums*>(workspace);
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(
       static_cast<uint8_t*>(workspace) + round_up(rows * slices * (int64_t)sizeof(Sums), 256));
-  const bool warp_rows = top == 0 && slices == 1 && vocab <= kWarpRow && rows >= kWarps * dev.sm_count;
+  const bool warp_rows = slices == 1 && vocab <= kWarpRow && top <= kWarpTop && rows >= kWarps * dev.sm_count;
   const dim3 grid((unsigned)slices, row_blocks(rows, warp_rows ? kWarps : 1));
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const T* x = static_cast<const T*>(logits);
-    auto kern = top > 0     ? logprobs_fwd_kernel<T, true, kThreads>
-                : warp_rows ? logprobs_fwd_kernel<T, false, 32>
-                            : logprobs_fwd_kernel<T, false, kThreads>;
+    auto kern = warp_rows ? (top > 0 ? logprobs_fwd_kernel<T, true, 32> : logprobs_fwd_kernel<T, false, 32>)
+                          : (top > 0 ? logprobs_fwd_kernel<T, true, kThreads> : logprobs_fwd_kernel<T, false, kThreads>);
     int rc = cuda_code(launch_gemm(kern, grid, dim3(kThreads), 0, stream, x, targets, rows, vocab, ld, slice, top,
                                    ignore_index, out, sums, keys));
     if (rc || slices == 1) return rc;

@@ -138,8 +138,20 @@ def test_many_short_rows(cuda_device, native_lib, vocab, dtype):
     x, t = x[:, :vocab], t.clamp(max=vocab - 1)
     x[::50] = -math.inf
     t[7::40] = -100
+    x[5] = 1.0                                           # all alike
+    x[6] = torch.arange(vocab, device=cuda_device) % 2   # two values
     ex = Exact(x, t)
     ex.check(logprobs.token_logprobs(x, t))
+    for k in sorted({min(k, vocab) for k in (1, 5, 16, 17)}):
+        r = logprobs.token_logprobs(x, t, top_k=k)
+        ex.check(r)
+        ex.check_top(r, x, k)
+        bad = torch.empty_strided(x.shape, x.stride(), dtype=dtype, device=cuda_device).copy_(x)  # the same pitch
+        bad[::3, vocab // 2] = math.nan
+        q = logprobs.token_logprobs(bad, t, top_k=k)
+        assert q.entropy[::3].isnan().all() and (q.top_indices[::3, 0] == vocab // 2).all()
+        for a, b in ((q.logprobs, r.logprobs), (q.entropy, r.entropy), (q.top_indices, r.top_indices)):
+            assert torch.equal(a[1::3], b[1::3]) and torch.equal(a[2::3], b[2::3])
     leaf = x.clone().requires_grad_()
     r = logprobs.token_logprobs(leaf, t)
     gen = torch.Generator().manual_seed(vocab)
