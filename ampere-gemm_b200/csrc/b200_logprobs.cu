@@ -104,14 +104,67 @@ __device__ __forceinline__ void add_logit(Sums& s, float v) {
   s.w = fmaf(x, fmaxf(d, -1.0e4f), s.w);
 }
 
-// Adds a group of logits whose maximum is `mx` and smallest `mn` (NaN in mx if
-// one is).  The sums of a thread are pairs: one instruction adds to both.
+// max of two packed 16-bit elements; NaN where an operand is.
+template <typename T>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Three-input maximum (NaN if one is).
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Logits enter the sums no lower than this, which keeps 0 * -inf out of w.  It
+// makes no difference where the row's maximum is kClampFar<T> or more: what is
+// lifted still has probability 0.  Rows below that (all masked with a lowest
+// value) are summed again one by one.
+template <typename T>
+constexpr float kClamp = std::is_same<T, __half>::value ? -65504.0f : -1.0e30f;
+template <typename T>
+constexpr float kClampFar = std::is_same<T, __half>::value ? -65000.0f : -1.0e29f;
+
+// A group's maximum, and its logits clamped.
+template <typename T, int kPacks>
+__device__ __forceinline__ float group_most(const Pack<T, kVec16<T>> (&q)[kPacks]) {
+  if constexpr (sizeof(T) == 4) {
+    float2 v[kGroup / 2];
+    unpack<T, kVec16<T>, kPacks>(q, v);
+    return max_nan(max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x), max3_nan(v[2].y, v[3].x, v[3].y));
+  } else {
+    static_assert(kPacks == 1, "a group is one pack");
+    const uint32_t w = max_word<T>(max_word<T>(q[0].u[0], q[0].u[1]), max_word<T>(q[0].u[2], q[0].u[3]));
+    const float2 m = word_to_pair<T>(w);
+    return max_nan(m.x, m.y);
+  }
+}
+template <typename T, int kPacks>
+__device__ __forceinline__ void group_values(const Pack<T, kVec16<T>> (&q)[kPacks], float2 (&v)[kGroup / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    unpack<T, kVec16<T>, kPacks>(q, v);
+#pragma unroll
+    for (int i = 0; i < kGroup / 2; ++i) v[i] = make_float2(max_nan(v[i].x, kClamp<T>), max_nan(v[i].y, kClamp<T>));
+  } else {
+    const uint32_t clamp = pair_to_word<T>(pair_of(kClamp<T>));
+#pragma unroll
+    for (int i = 0; i < kGroup / 2; ++i) v[i] = word_to_pair<T>(max_word<T>(q[0].u[i], clamp));
+  }
+}
+
+// Adds a group of clamped logits with maximum `mx`.  The sums of a thread are
+// pairs: one instruction adds to both.
 struct PairSums {
   float m;
   float2 z, w;
 };
 
-__device__ __forceinline__ void add_group(PairSums& s, const float2 (&v)[kGroup / 2], float mx, float mn) {
+__device__ __forceinline__ void add_group(PairSums& s, const float2 (&v)[kGroup / 2], float mx) {
   if (!(mx <= s.m)) {
     Sums a{s.m, s.z.x, s.w.x}, b{s.m, s.z.y, s.w.y};
     const float m = max_nan(s.m, mx);
@@ -121,28 +174,14 @@ __device__ __forceinline__ void add_group(PairSums& s, const float2 (&v)[kGroup 
   }
   const float2 minus_m = pair_of(s.m == kNegInf ? 0.0f : -s.m);
   const float2 log2e = pair_of(kLog2e);
-  const bool far = mn < -1.0e30f;  // -inf, or a mask's lowest value: d is clamped, see add_logit
 #pragma unroll
   for (int i = 0; i < kGroup / 2; ++i) {
-    float2 d = add2(v[i], minus_m);
+    const float2 d = add2(v[i], minus_m);
     const float2 t = mul2(d, log2e);
     const float2 x = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-    if (far) d = make_float2(fmaxf(d.x, -1.0e4f), fmaxf(d.y, -1.0e4f));
     s.z = add2(s.z, x);
     s.w = fma2(x, d, s.w);
   }
-}
-
-// Three-input maximum (NaN if one is) and minimum.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float min3(float a, float b, float c) {
-  float r;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // Sorts after every key with a smaller value, or with the same value and a
@@ -423,10 +462,8 @@ __global__ void __launch_bounds__(kThreads)
     };
     auto add = [&](const Pack<T, kV> (&q)[kPacks], int g) {
       float2 v[kGroup / 2];
-      unpack<T, kV, kPacks>(q, v);
-      const float mx = max_nan(max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x),
-                               max3_nan(v[2].y, v[3].x, v[3].y));
-      const float mn = fminf(min3(min3(v[0].x, v[0].y, v[1].x), v[1].y, v[2].x), min3(v[2].y, v[3].x, v[3].y));
+      group_values<T, kPacks>(q, v);
+      const float mx = group_most<T, kPacks>(q);
       if constexpr (kTop) {
         sel.group_max[g] = mx;
         // Strictly larger only: of equal groups the first stays.
@@ -435,13 +472,26 @@ __global__ void __launch_bounds__(kThreads)
           best_group = g;
         }
       }
-      add_group(ps, v, mx, mn);
+      add_group(ps, v, mx);
     };
     int g = tid;
+    // A warp's threads begin with the maximum of their first groups together:
+    // few groups exceed it, where of a thread's own maximum some lane's group
+    // nearly always does, and all lanes wait for its rebase.
+    bool begin = (tid | 31) + (kUnroll - 1) * kRowThreads < groups;
     for (; g + (kUnroll - 1) * kRowThreads < groups; g += kUnroll * kRowThreads) {
       Pack<T, kV> q[kUnroll][kPacks];
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) load(q[i], g + i * kRowThreads);
+      if (begin) {
+        begin = false;
+        float m = group_most<T, kPacks>(q[0]);
+#pragma unroll
+        for (int i = 1; i < kUnroll; ++i) m = max_nan(m, group_most<T, kPacks>(q[i]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        ps.m = m;
+      }
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) add(q[i], g + i * kRowThreads);
     }
@@ -456,7 +506,14 @@ __global__ void __launch_bounds__(kThreads)
     const float target_v = target != ignore ? target_logit(x, vocab, target) : 0.0f;
     if (has_head) add_logit(s, head_v);
     if (has_tail) add_logit(s, tail_v);
-    s = kRowThreads == 32 ? warp_merge(s) : block_merge(s, merge_buf);
+    auto row_merge = [&](const Sums& a) { return kRowThreads == 32 ? warp_merge(a) : block_merge(a, merge_buf); };
+    s = row_merge(s);
+    if (s.m < kClampFar<T> && s.m != kNegInf) {
+      s = Sums{kNegInf, 0.0f, 0.0f};
+      for (int64_t j = lo + tid; j < hi; j += kRowThreads) add_logit(s, to_f32(x[j]));
+      row_sync<kRowThreads>();
+      s = row_merge(s);
+    }
     if constexpr (kTop) {
       // Threshold: a bound that at least `top` of the threads' best groups and
       // at most Sel::kMost threads reach (or every group does).
