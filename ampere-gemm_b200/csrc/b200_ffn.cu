@@ -167,11 +167,11 @@ constexpr int kRowsMaxSmem = 220 * 1024;
 template <typename Kern>
 int rows_clusters(Kern kern, int parts, int sm_count) {
   if (parts == 1) return sm_count;
-  static int cache[kMaxDevices][4];
+  static std::atomic<int> cache[kMaxDevices][4];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sm_count / parts;
-  int& n = cache[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3];
-  if (n > 0) return n;
+  std::atomic<int>& slot = cache[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3];
+  if (const int n = slot.load(std::memory_order_relaxed)) return n;
   (void)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsMaxSmem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count / parts * parts);
@@ -188,7 +188,9 @@ int rows_clusters(Kern kern, int parts, int sm_count) {
     (void)cudaGetLastError();
     got = sm_count / parts;
   }
-  return n = std::min(got, sm_count / parts);
+  got = std::min(got, sm_count / parts);
+  slot.store(got, std::memory_order_relaxed);
+  return got;
 }
 
 // How the rows kernel cuts a product up: CTAs of a cluster, rows of w per

@@ -47,10 +47,10 @@ constexpr int kTopSlice = 65536;
 // SM a block, with kWarpTop alternatives at most: no barriers, and eight rows'
 // loads side by side.  bf16, us, a block a row -> a warp a row: 100000 x 500
 // forward 270 -> 63, backward 214 -> 63, top 5 724 -> 130; 20000 x 5000 98 -> 53,
-// 98 -> 79, 179 -> 74; 8192 x 8192 40 -> 32, 47.5 -> 50.5 (2000 x 8192: 11 -> 13
+// 98 -> 79, 179 -> 73 (top 20 195 -> 108); 8192 x 8192 40 -> 32, 47.5 -> 50.5 (2000 x 8192: 11 -> 13
 // backward).
 constexpr int kWarpRow = 6144;
-constexpr int kWarpTop = 16;
+constexpr int kWarpTop = 24;
 // Slices of a row at most when alternatives are wanted: one a thread of the join.
 constexpr int kMaxTopVocab = kTopSlice * kThreads;
 // Groups of a thread that are on their way at once.

