@@ -7,11 +7,12 @@
 //
 // Bound by memory: forward reads x and writes y once, backward reads x and dy
 // and writes dx once.  Measured, of the measured copy bandwidth: 20011 x 5120
-// bf16 forward 75 us (0.84); 16384 x 4096 bf16 with fp32 weights 58 us forward
-// (0.71), 76 + 4 backward (0.77); 8 x 4096 fp16 3 us.  What remains is the issue
-// of instructions (half the slots) and the wait for a row's sums.  A row stays in registers, in its own type, between the
-// passes over it; all sums are in fp32 and y, dx, dw and db are rounded once.
-// Every sum has a fixed order, so results do not change from run to run.
+// bf16 forward 75 us (0.84); 16384 x 4096 bf16 with fp32 weights 52 us forward
+// (0.79), 76 + 5 backward (0.76); 8 x 4096 fp16 3 us.  What remains is the issue
+// of instructions (half the slots) and the wait for a row's sums.  A row stays
+// in registers, in its own type, between the passes over it; all sums are in
+// fp32 and y, dx, dw and db are rounded once.  Every sum has a fixed order, so
+// results do not change from run to run.
 #include <algorithm>
 #include <cstdint>
 
@@ -67,6 +68,24 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   return sum_of(red, tpr >> 5);
+}
+
+// The same for N rows at once.
+template <int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float (*red)[32]) {
+  if (tpr <= 32) {
+#pragma unroll
+    for (int r = 0; r < N; ++r) v[r] = lanes_sum(v[r], tpr);
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    v[r] = warp_sum(v[r]);
+    if ((threadIdx.x & 31) == 0) red[r][threadIdx.x >> 5] = v[r];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < N; ++r) v[r] = sum_of(red[r], tpr >> 5);
 }
 
 // Where a thread's packs of a row lie: pack j at (j * threads of the row +
@@ -131,6 +150,16 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Rows that a thread of the forward takes at once: two for 16-bit rows with fp32
+// weights, which are most of what the L1 cache delivers, where the row fills its
+// threads exactly (16384 x 4096: 59 -> 54 us, 8192 x 8192: 70 -> 64, 20000 x 768:
+// 15.4 -> 13.5).  With weights of the row's type one, for twice the blocks (30000
+// x 2560: 65 us against 75, 20011 x 5120: 80 against 82).
+template <typename T, typename W>
+__host__ __device__ constexpr int fwd_rows_at_once(int tpr) {
+  return tpr != 0 && sizeof(W) > sizeof(T) ? 2 : 1;
+}
+
 // Forward.  blockDim = (threads of a row, rows of a block).  The blocks are
 // resident and loop over rows.
 template <typename T, typename W, int VEC, int NV, int TPR>
@@ -138,71 +167,92 @@ __global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads
     layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
                           T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows,
                           int cols, int64_t ldx, int64_t ldy, float eps) {
-  __shared__ __align__(16) float red[2][32];
+  constexpr int kRows = fwd_rows_at_once<T, W>(TPR);
+  __shared__ __align__(16) float red[2][kRows][32];
   pdl_wait();
   const Columns<VEC, TPR> col{cols};
   const int tpr = TPR ? TPR : static_cast<int>(blockDim.x);
   const float inv_n = 1.0f / static_cast<float>(cols);
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+  const int64_t x_step = step * ldx, y_step = step * ldy;
   int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const T* xr = x + row * ldx;
   T* yr = y + row * ldy;
   // The rows of a block take their turns together: row - threadIdx.y is the same for all.
-  for (; row - threadIdx.y < rows; row += step, xr += step * ldx, yr += step * ldy) {
-    const bool active = row < rows;
-    Pack<T, VEC> v[NV];
-    load_row<T, VEC, NV>(v, xr, col, active);
-    float2 s2 = make_float2(0.0f, 0.0f);
+  for (; row - threadIdx.y < rows; row += kRows * step, xr += kRows * x_step, yr += kRows * y_step) {
+    bool active[kRows];
+    Pack<T, VEC> v[kRows][NV];
+    float mu[kRows], rstd[kRows];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      for_pairs<T, VEC>(v[j], [&](float2 f) { s2 = add2(s2, f); });
-    const float mu = row_sum(s2.x + s2.y, tpr, red[0]) * inv_n;
+    for (int r = 0; r < kRows; ++r) {
+      active[r] = row + r * step < rows;
+      load_row<T, VEC, NV>(v[r], xr + r * x_step, col, active[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float2 s2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        for_pairs<T, VEC>(v[r][j], [&](float2 f) { s2 = add2(s2, f); });
+      mu[r] = s2.x + s2.y;
+    }
+    row_sums(mu, tpr, red[0]);
     // The centred squares are summed in a second pass over the registers:
     // sum(x^2) - n mu^2 would lose the variance of a row with a large mean.
-    const float2 minus_mu = pair_of(-mu);
-    float2 q2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (col.has(j))
-        for_pairs<T, VEC>(v[j], [&](float2 f) {
-          f = add2(f, minus_mu);
-          if (VEC == 1) f.y = 0.0f;
-          q2 = fma2(f, f, q2);
-        });
+    for (int r = 0; r < kRows; ++r) {
+      mu[r] *= inv_n;
+      const float2 minus_mu = pair_of(-mu[r]);
+      float2 q2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (col.has(j))
+          for_pairs<T, VEC>(v[r][j], [&](float2 f) {
+            f = add2(f, minus_mu);
+            if (VEC == 1) f.y = 0.0f;
+            q2 = fma2(f, f, q2);
+          });
+      }
+      rstd[r] = q2.x + q2.y;
     }
-    const float rstd = inverse_sqrt(row_sum(q2.x + q2.y, tpr, red[1]) * inv_n + eps);
-    const float2 r2 = pair_of(rstd);
+    row_sums(rstd, tpr, red[1]);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) rstd[r] = inverse_sqrt(rstd[r] * inv_n + eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (active && col.has(j)) {
-        const int c = col.at(j);
-        if constexpr (VEC == 1) {
-          const float h = (to_f32(v[j].v) - mu) * rstd;
-          yr[c] = from_f32<T>(fmaf(h, w ? to_f32(w[c]) : 1.0f, b ? to_f32(b[c]) : 0.0f));
-        } else {
-          float2 f[VEC / 2];
+      if (!col.has(j)) continue;
+      const int c = col.at(j);
+      if constexpr (VEC == 1) {
+        const float wc = w ? to_f32(w[c]) : 1.0f, bc = b ? to_f32(b[c]) : 0.0f;
 #pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) f[i] = mul2(add2(v[j].pair(i), minus_mu), r2);
-          if (w) {
-            const Pack<W, VEC> p = load_pack<W, VEC>(w + c);
+        for (int r = 0; r < kRows; ++r)
+          if (active[r]) yr[r * y_step + c] = from_f32<T>(fmaf((to_f32(v[r][j].v) - mu[r]) * rstd[r], wc, bc));
+      } else {
+        Pack<W, VEC> pw, pb;
+        if (w) pw = load_pack<W, VEC>(w + c);
+        if (b) pb = load_pack<W, VEC>(b + c);
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) f[i] = mul2(f[i], p.pair(i));
-          }
-          if (b) {
-            const Pack<W, VEC> p = load_pack<W, VEC>(b + c);
-#pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) f[i] = add2(f[i], p.pair(i));
-          }
+        for (int r = 0; r < kRows; ++r) {
+          const float2 minus_mu = pair_of(-mu[r]), r2 = pair_of(rstd[r]);
           Pack<T, VEC> o;
 #pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) o.set_pair(i, f[i]);
-          store_pack<T, VEC>(yr + c, o);
+          for (int i = 0; i < VEC / 2; ++i) {
+            float2 f = mul2(add2(v[r][j].pair(i), minus_mu), r2);
+            if (w) f = mul2(f, pw.pair(i));
+            if (b) f = add2(f, pb.pair(i));
+            o.set_pair(i, f);
+          }
+          if (active[r]) store_pack<T, VEC>(yr + r * y_step + c, o);
         }
       }
     }
-    if (active && threadIdx.x == 0) {
-      if (mean_out) mean_out[row] = mu;
-      if (rstd_out) rstd_out[row] = rstd;
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (active[r]) {
+          if (mean_out) mean_out[row + r * step] = mu[r];
+          if (rstd_out) rstd_out[row + r * step] = rstd[r];
+        }
     }
   }
 }
@@ -256,8 +306,10 @@ constexpr int kAhead = NV <= 2 ? 3 : 1;
 // layer_norm_bwd_reduce_kernel adds those rows up.  With 16-byte packs, rows
 // arrive through a ring in shared memory in which every thread reads only what
 // it requested itself: no barrier, and no registers for rows on their way.
+// 128 registers a thread also where only 320 threads make a block (8192 x 5120
+// fp32: 86 us, against 109 for two blocks an SM, which spill).
 template <typename T, typename W, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR == 320 ? TPR : kBwdThreads, TPR == 320 ? 2 : 1)
+__global__ void __launch_bounds__(kBwdThreads)
     layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
                           const float* __restrict__ mean, const float* __restrict__ rstd_in, T* __restrict__ dx,
                           float* __restrict__ part, int64_t rows, int cols, int64_t lddy, int64_t ldx, int64_t lddx) {

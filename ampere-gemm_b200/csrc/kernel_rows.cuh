@@ -17,7 +17,7 @@
 //               ten share once the MMAs are over.
 //
 // Measured: w of 24576 x 4096 (gate and up) in 42 us, of 4096 x 12288 in 22 us
-// for one row of fp16 x: 0.74 and 0.70 of the measured copy bandwidth with the
+// for one row of fp16 x: 0.74 and 0.69 of the measured copy bandwidth with the
 // launch's start and end, which a short stream cannot hide.
 //
 // Launched with programmatic stream serialisation.  With `w_early`, w was not
