@@ -7,8 +7,8 @@
 //
 // Bound by memory: forward reads x and writes y once, backward reads x and dy
 // and writes dx once.  Measured, of the measured copy bandwidth: 20011 x 5120
-// bf16 forward 75 us (0.84); 16384 x 4096 bf16 with fp32 weights 52 us forward
-// (0.79), 76 + 5 backward (0.76); 8 x 4096 fp16 3 us.  What remains is the issue
+// bf16 forward 69 us (0.91); 16384 x 4096 bf16 with fp32 weights 47 us forward
+// (0.88), 76 + 5 backward (0.76); 8 x 4096 fp16 3 us.  What remains is the issue
 // of instructions (half the slots) and the wait for a row's sums.  A row stays
 // in registers, in its own type, between the passes over it; all sums are in
 // fp32 and y, dx, dw and db are rounded once.  Every sum has a fixed order, so
@@ -160,14 +160,31 @@ __host__ __device__ constexpr int fwd_rows_at_once(int tpr) {
   return tpr != 0 && sizeof(W) > sizeof(T) ? 2 : 1;
 }
 
+// Ring slots of the forward, each of the rows that are taken at once, and their
+// bytes of a thread; none where a slot would be more than 128 bytes.  For 16-bit
+// rows of two warps or more (us with and without: 20011 x 5120 69, 75; 16384 x
+// 4096 with fp32 weights 47, 52; 8192 x 8192 with them 48.5, 58; 4096 x 16384 51,
+// 56); rows of a warp and fp32 rows have enough on their way in registers (65536
+// x 1024 fp16 46, 43; 8192 x 5120 fp32 56.5, 54).
+template <typename T, typename W, int VEC, int NV, int TPR>
+struct FwdRing {
+  static constexpr int kSlot = fwd_rows_at_once<T, W>(TPR) * NV * 16;
+  static constexpr bool kUsed = TPR > 32 && sizeof(T) == 2 && VEC == 8 && kSlot <= 128;
+  static constexpr int kSlots = kUsed ? (kSlot > 64 ? 2 : 3) : 0;
+  static constexpr size_t kBytes = static_cast<size_t>(kSlots) * kSlot;
+};
+
 // Forward.  blockDim = (threads of a row, rows of a block).  The blocks are
-// resident and loop over rows.
+// resident and loop over rows.  With FwdRing, rows arrive through a ring in
+// shared memory in which every thread reads only what it requested itself.
 template <typename T, typename W, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads)
     layer_norm_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b,
                           T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows,
                           int cols, int64_t ldx, int64_t ldy, float eps) {
   constexpr int kRows = fwd_rows_at_once<T, W>(TPR);
+  constexpr int kSlots = FwdRing<T, W, VEC, NV, TPR>::kSlots;
+  extern __shared__ __align__(16) uint8_t dyn[];  // the ring
   __shared__ __align__(16) float red[2][kRows][32];
   pdl_wait();
   const Columns<VEC, TPR> col{cols};
@@ -178,6 +195,28 @@ __global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads
   int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const T* xr = x + row * ldx;
   T* yr = y + row * ldy;
+  const int threads = tpr * blockDim.y;
+  Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(dyn) + threadIdx.y * tpr + threadIdx.x;
+  int64_t next = row;  // the row requested next
+  const T* xn = xr;
+  auto request = [&](int slot) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (next + r * step < rows) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          copy_async_16(ring + ((slot * kRows + r) * NV + j) * threads, xn + r * x_step + col.at(j));
+      }
+    }
+    copy_async_commit();
+    next += kRows * step;
+    xn += kRows * x_step;
+  };
+  int slot = 0;
+  if constexpr (kSlots > 0) {
+#pragma unroll
+    for (int i = 0; i < kSlots - 1; ++i) request(i);
+  }
   // The rows of a block take their turns together: row - threadIdx.y is the same for all.
   for (; row - threadIdx.y < rows; row += kRows * step, xr += kRows * x_step, yr += kRows * y_step) {
     bool active[kRows];
@@ -186,7 +225,20 @@ __global__ void __launch_bounds__(TPR ? (TPR > 128 ? TPR : 128) : kMaxRowThreads
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       active[r] = row + r * step < rows;
-      load_row<T, VEC, NV>(v[r], xr + r * x_step, col, active[r]);
+      if constexpr (kSlots == 0) load_row<T, VEC, NV>(v[r], xr + r * x_step, col, active[r]);
+    }
+    if constexpr (kSlots > 0) {
+      request(slot == 0 ? kSlots - 1 : slot - 1);
+      copy_async_wait<kSlots - 1>();
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          v[r][j] = Pack<T, VEC>{};
+          if (active[r]) v[r][j] = ring[((slot * kRows + r) * NV + j) * threads];
+        }
+      }
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -770,8 +822,13 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
             constexpr int kT = fwd_exact<kV>(kNv, decltype(tc)::value) ? decltype(tc)::value : 0;
             constexpr auto kern = layer_norm_fwd_kernel<T, W, kV, kNv, kT>;
             const int64_t blocks = (rows + p.rows - 1) / p.rows;
-            const int grid = (int)std::min<int64_t>(blocks, resident_blocks<kern>(p.threads * p.rows, 0, dev.sm_count));
-            return cuda_code(launch_gemm(kern, dim3(grid), dim3(p.threads, p.rows), 0, stream,
+            const size_t smem = FwdRing<T, W, kV, kNv, kT>::kBytes * p.threads * p.rows;
+            static std::atomic<uint8_t> attr_done[kMaxDevices];
+            if (smem > 0)
+              if (int e = ensure_smem_attr(kern, (int)smem, attr_done)) return e;
+            const int fit = resident_blocks<kern>(p.threads * p.rows, smem, dev.sm_count);
+            const int grid = (int)std::min<int64_t>(blocks, fit);
+            return cuda_code(launch_gemm(kern, dim3(grid), dim3(p.threads, p.rows), smem, stream,
                                          static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b),
                                          static_cast<T*>(y), mean, rstd, rows, n, ldx, ldy, eps));
           });
