@@ -630,7 +630,9 @@ constexpr bool exact_threads(int t) {
 }
 template <int VEC>
 constexpr bool fwd_exact(int nv, int t) {
-  return VEC >= 4 && exact_threads(t) && t <= 256 && (nv * VEC == 24 || nv * VEC == 32 || nv * VEC == 64);
+  // 16 columns a thread for 2560, which 24, 32 and 64 do not divide into whole warps.
+  return VEC >= 4 && exact_threads(t) && t <= 256 &&
+         (nv * VEC == 24 || nv * VEC == 32 || nv * VEC == 64 || (nv * VEC == 16 && t == 160));
 }
 template <int VEC>
 constexpr bool bwd_exact(int nv, int t) {

@@ -69,7 +69,9 @@ def check_backward(dx, dw, db, x, w, dy, eps=EPS):
 
 
 SIZES = [(1, 1), (1, 8), (5, 7), (3, 64), (33, 257), (600, 256), (2000, 1000), (7, 2048), (1300, 4096), (2, 8192),
-         (9, 16384), (700, 520), (3, 9001), (2, 40000), (300, 20008)]
+         (9, 16384), (700, 520), (3, 9001), (2, 40000), (300, 20008),
+         # Several rounds of every block: 16, 32 and 64 columns a thread, one and two rows at once.
+         (6001, 2560), (5003, 4096), (4501, 5120), (4003, 1536), (1801, 16384)]
 TYPES = [(F16, F16), (F16, F32), (BF16, BF16), (BF16, F32), (F32, F32)]
 
 
