@@ -98,7 +98,7 @@ __global__ void copy_jobs_kernel(const __grid_constant__ CopyJobs jobs) {
     uint16_t* dst = j.dst + r * j.dst_ld;
     const int64_t cols = r < j.rows ? j.cols : 0;
     for (int64_t c = threadIdx.x * 8; c < j.dst_cols; c += blockDim.x * 8) {
-      uint16_t v[8] = {};
+      alignas(16) uint16_t v[8] = {};
       if (src16 && c + 8 <= cols) {
         *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + c);
       } else {

@@ -179,6 +179,17 @@ def test_strided_operands(cuda_device, native_lib, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pitch", [2 ** 31 + 8, 2 ** 31 + 1])
+def test_offsets_past_32_bits(cuda_device, native_lib, pitch):
+    """Rows of x that start beyond 2^32 elements, aligned or not."""
+    x0, w_in, w_out, _ = make(3, 72, 40, 24, F16, cuda_device)
+    base = torch.empty(2 * pitch + 72, dtype=F16, device=cuda_device)
+    x = base.as_strided((3, 72), (pitch, 1))
+    x.copy_(x0)
+    Exact(x0, w_in, w_out, "silu").y.check(ffn.gated_ffn(x, w_in, w_out))
+
+
+@pytest.mark.gpu
 def test_only_some_gradients(cuda_device, native_lib):
     x, w_in, w_out, dy = make(70, 64, 96, 80, BF16, cuda_device)
     full = run(x, w_in, w_out, "silu", dy)[1:]

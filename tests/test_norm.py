@@ -126,6 +126,21 @@ def test_strided_and_misaligned_rows(cuda_device, native_lib, dtype, offset, pit
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [257, 4096])
+def test_offsets_past_32_bits(cuda_device, native_lib, cols):
+    """Rows that start beyond 2^32 elements."""
+    rows, pitch = 3, 2 ** 31 + 8
+    x0, w, b, dy = make(rows, cols, F16, F32, cuda_device)
+    base = torch.empty((rows - 1) * pitch + cols, dtype=F16, device=cuda_device)
+    x = base.as_strided((rows, cols), (pitch, 1))
+    x.copy_(x0)
+    y, stats = norm._forward(x, w, b, EPS, True)
+    check_forward(y, x0, w, b)
+    dx, dw, db = norm._backward(dy, x, w, stats, F32, True, True)
+    check_backward(dx, dw, db, x0, w, dy)
+
+
+@pytest.mark.gpu
 def test_other_layouts(cuda_device, native_lib):
     x, w, b, dy = make(24, 40, F32, F32, cuda_device)
     t = x.t().contiguous().t()                                     # columns contiguous
