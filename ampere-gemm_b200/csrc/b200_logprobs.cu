@@ -84,12 +84,13 @@ struct Sums {
 };
 
 // Moves sums to a maximum `m` >= s.m.  x - m = (x - s.m) + (s.m - m); a sum
-// over nothing (s.m = -inf, z = 0) stays empty.
+// over nothing (s.m = -inf, z = 0) stays empty.  Where f is 0 the clamp of d
+// keeps z d finite, and so 0 * -inf out of w.
 __device__ __forceinline__ void rebase(Sums& s, float m) {
   if (s.m == m) return;
   const float d = s.m - m;
   const float f = exp2_approx(d * kLog2e);
-  s.w = s.z > 0.0f ? f * fmaf(s.z, d, s.w) : (s.z == 0.0f ? 0.0f : s.z);
+  s.w = s.z > 0.0f ? f * fmaf(s.z, fmaxf(d, -1.0e4f), s.w) : (s.z == 0.0f ? 0.0f : s.z);
   s.z = s.z * f;
   s.m = m;
 }

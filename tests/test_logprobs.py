@@ -384,3 +384,25 @@ def test_c_argument_checks_without_gpu(native_lib):
     assert fwd(*big) == 8                                   # misaligned workspace
     assert bwd(p, p, p, p, p, p, None, 4, 100, 100, 100, -100, 0, None) == 1
     assert bwd(p, p, p, p, p, p, p, 4, 100, 99, 100, -100, 0, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(4, 300), (1187, 300), (4, 50257), (4, 200003)])
+def test_forced_token(cuda_device, native_lib, rows, vocab, dtype):
+    """One logit at the type's highest value: it has all the probability, wherever it stands."""
+    x, t = make(rows, vocab, dtype, cuda_device)
+    at = torch.arange(rows, device=cuda_device) * 97 % vocab
+    at[:4] = torch.tensor([0, vocab - 1, vocab // 2, 9], device=cuda_device)
+    x[torch.arange(rows, device=cuda_device), at] = torch.finfo(dtype).max
+    t[::2] = at[::2]
+    ex = Exact(x, t)
+    r = logprobs.token_logprobs(x, t, top_k=3)
+    ex.check(r)
+    ex.check_top(r, x, 3)
+    ex.check(logprobs.token_logprobs(x, t))
+    leaf = x.clone().requires_grad_()
+    q = logprobs.token_logprobs(leaf, t)
+    gl, gh = (torch.randn(rows, device=cuda_device) for _ in range(2))
+    dx, = torch.autograd.grad((q.logprobs, q.entropy), (leaf,), (gl, gh))
+    ex.check_grad(dx, gl, gh)
