@@ -129,14 +129,22 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// Logits enter the sums no lower than this, which keeps 0 * -inf out of w.  It
-// makes no difference where the row's maximum is kClampFar<T> or more: what is
-// lifted still has probability 0.  Rows below that (all masked with a lowest
-// value) are summed again one by one.
+// Logits enter the sums no lower than this, which keeps 0 * -inf out of w, and
+// so does the maximum they are summed under: a group that is masked altogether
+// has differences of 0, not kClamp<T> minus the lowest value.  It makes no
+// difference where the row's maximum is kClampFar<T> or more: what is lifted
+// still has probability 0.  Rows below that (all masked with a lowest value)
+// are summed again one by one.
 template <typename T>
 constexpr float kClamp = std::is_same<T, __half>::value ? -65504.0f : -1.0e30f;
 template <typename T>
 constexpr float kClampFar = std::is_same<T, __half>::value ? -65000.0f : -1.0e29f;
+
+// The maximum that clamped logits with maximum `m` are summed under; -inf stays (nothing to sum).
+template <typename T>
+__device__ __forceinline__ float sum_base(float m) {
+  return m < kClamp<T> && m != kNegInf ? kClamp<T> : m;
+}
 
 // A group's maximum, and its logits clamped.
 template <typename T, int kPacks>
@@ -165,17 +173,18 @@ __device__ __forceinline__ void group_values(const Pack<T, kVec16<T>> (&q)[kPack
   }
 }
 
-// Adds a group of clamped logits with maximum `mx`.  The sums of a thread are
-// pairs: one instruction adds to both.
+// Adds a group of clamped logits whose maximum before was `mx`.  The sums of a
+// thread are pairs: one instruction adds to both.
 struct PairSums {
   float m;
   float2 z, w;
 };
 
+template <typename T>
 __device__ __forceinline__ void add_group(PairSums& s, const float2 (&v)[kGroup / 2], float mx) {
   if (!(mx <= s.m)) {
     Sums a{s.m, s.z.x, s.w.x}, b{s.m, s.z.y, s.w.y};
-    const float m = max_nan(s.m, mx);
+    const float m = sum_base<T>(max_nan(s.m, mx));
     rebase(a, m);
     rebase(b, m);
     s = PairSums{m, make_float2(a.z, b.z), make_float2(a.w, b.w)};
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kThreads)
           best_group = g;
         }
       }
-      add_group(ps, v, mx);
+      add_group<T>(ps, v, mx);
     };
     int g = tid;
     // A warp's threads begin with the maximum of their first groups together:
@@ -498,7 +507,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int i = 1; i < kUnroll; ++i) m = max_nan(m, group_most<T, kPacks>(q[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        ps.m = m;
+        ps.m = sum_base<T>(m);
       }
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) add(q[i], g + i * kRowThreads);

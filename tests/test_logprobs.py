@@ -386,6 +386,44 @@ def test_c_argument_checks_without_gpu(native_lib):
     assert bwd(p, p, p, p, p, p, p, 4, 100, 99, 100, -100, 0, None) == 1
 
 
+# Stretches of a row that are masked, as (first, last) of the vocabulary's length.
+STRETCHES = [(0.0, 0.05), (0.95, 1.0), (0.4, 0.6), (0.0, 0.5), (0.5, 1.0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(7, 300), (1187, 300), (7, 5000), (1187, 5000), (7, 50257), (7, 200003)])
+def test_masked_stretches(cuda_device, native_lib, rows, vocab, dtype):
+    """Contiguous masks of finite lowest values: padded vocabularies, constrained decoding."""
+    masks = [torch.finfo(dtype).min] if dtype == F16 else [torch.finfo(dtype).min, -1e38, -1e31, -2e30]
+    for mask in masks:
+        x, t = make(rows, vocab, dtype, cuda_device)
+        for i in range(rows):
+            if i % 7 < 5:
+                lo, hi = STRETCHES[i % 7]
+                x[i, round(lo * vocab):round(hi * vocab)] = mask
+            elif i % 7 == 5:                             # all but three logits
+                keep = x[i, [1, vocab // 2, vocab - 2]].clone()
+                x[i] = mask
+                x[i, [1, vocab // 2, vocab - 2]] = keep
+                t[i] = vocab // 2
+            else:                                        # a mixture of masks, one stretch each
+                x[i, :vocab // 3] = mask
+                x[i, vocab // 3:2 * vocab // 3] = -math.inf
+                t[i] = vocab - 1
+        ex = Exact(x, t)
+        ex.check(logprobs.token_logprobs(x, t))
+        for k in (1, 20, 40):
+            r = logprobs.token_logprobs(x, t, top_k=k)
+            ex.check(r)
+            ex.check_top(r, x, k)
+        leaf = x.clone().requires_grad_()
+        r = logprobs.token_logprobs(leaf, t)
+        gl, gh = (torch.randn(rows, device=cuda_device) for _ in range(2))
+        dx, = torch.autograd.grad((r.logprobs, r.entropy), (leaf,), (gl, gh))
+        ex.check_grad(dx, gl, gh)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("rows,vocab", [(4, 300), (1187, 300), (4, 50257), (4, 200003)])
