@@ -160,7 +160,9 @@ void* writable(void* p, int64_t& ld, int64_t rows, int64_t cols, Carver& ws, Cop
 
 // ---- few rows of x (kernel_rows.cuh) ----
 
-constexpr int kRowsMaxSmem = 220 * 1024;
+constexpr int kRowsMaxSmem = 227 * 1024;
+// An SM's shared memory, what the system takes of it for each CTA, and its TMEM columns.
+constexpr int kSmSmem = 228 * 1024, kCtaSmem = 1024, kSmTmemCols = 512;
 
 // Largest number of S-CTA clusters of the rows kernel resident at once, one
 // CTA an SM.
@@ -251,6 +253,48 @@ double pair_cycles(int tokens, int n, int k, int out_n, int sm_count) {
   return (double)waves * (std::max(512.0, 800.0 / row_tiles) * ((k + kBK - 1) / kBK) + 2000.0) + 9000.0;
 }
 
+// Shape and shared memory of a launch of the rows kernel.
+struct RowsLaunch {
+  RowsShape sh;
+  int smem = 0, tmem_cols = 0;
+};
+
+RowsLaunch rows_launch(int tokens, int n, int n_pad, int k, bool gate, const RowsPlan& plan) {
+  RowsLaunch l;
+  RowsShape& sh = l.sh;
+  const int accs = gate ? 2 : 1;
+  sh.tokens = tokens;
+  sh.tile = plan.tile;
+  sh.tokens_pad = (plan.tile + 15) / 16 * 16;
+  sh.n = n;
+  sh.n_pad = n_pad;
+  sh.n_blocks = (n + plan.block - 1) / plan.block;
+  sh.k_blocks = (k + kBK - 1) / kBK;
+  sh.block = plan.block;
+  sh.block_pad = (sh.block + 7) / 8 * 8;
+  const int sub = rows_sub_bytes(sh, gate);
+  const int share = (sh.k_blocks + plan.parts - 1) / plan.parts;
+  // 48 KB a stage (16 KB: 10-30 % slower, each stage costs its commit) in a
+  // ring of 200 KB (94 KB, beside the next launch's: 4-8 % slower).
+  constexpr int kStageTarget = 48 * 1024, kRing = 200 * 1024;
+  sh.k_sub = std::min(share, std::max(1, kStageTarget / sub));
+  const int stage = sub * sh.k_sub;
+  sh.stages = std::min({kRing / stage, kRowsMaxStages, (share + sh.k_sub - 1) / sh.k_sub});
+  sh.tail = (int)round_up(std::max(0, (128 - sh.block_pad - sh.tokens_pad) * 128), 1024);
+  // Tokens of a reduction round: what the stages hold in fp32.
+  const int token_bytes = accs * 128 * 4;
+  if (sh.stages * stage + sh.tail < 16 * token_bytes) sh.tail = 16 * token_bytes;
+  sh.chunk = std::min(sh.tokens_pad, (sh.stages * stage + sh.tail) / token_bytes / 16 * 16);
+  l.smem = sh.stages * stage + sh.tail + kRowsBarBytes + 1024;
+  l.tmem_cols = rows_tmem_columns(accs, sh.tokens_pad);
+  // At least the share of an SM's shared memory that the CTA takes of its
+  // TMEM: CTAs that share an SM then find TMEM for all of them.  One that
+  // waited for TMEM would hold up its cluster, and clusters that each hold what
+  // another one's CTA waits for would never end.
+  l.smem = std::max(l.smem, (int)((int64_t)l.tmem_cols * kSmSmem / kSmTmemCols) - kCtaSmem);
+  return l;
+}
+
 // One product on the rows kernel; `w` has `n` rows (2 n with kRowsGateUp) of k
 // elements, or is stored k x n (kWMajorN).
 template <bool kBf16, int kMode, bool kWMajorN>
@@ -261,33 +305,11 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ro
   if (int e = ensure_smem_attr(kern, kRowsMaxSmem, attr_done)) return e;
   constexpr bool kGate = kMode == kRowsGateUp;
   constexpr int kAccs = kGate ? 2 : 1;
-  RowsShape sh;
-  sh.tokens = tokens;
-  sh.tile = plan.tile;
-  sh.tokens_pad = (plan.tile + 15) / 16 * 16;
-  sh.n = n;
-  sh.n_pad = n_pad;
-  sh.n_blocks = (n + plan.block - 1) / plan.block;
-  sh.k_blocks = (k + kBK - 1) / kBK;
-  sh.block = plan.block;
-  sh.block_pad = (sh.block + 7) / 8 * 8;
+  RowsLaunch l = rows_launch(tokens, n, n_pad, k, kGate, plan);
+  RowsShape& sh = l.sh;
   sh.activation = act;
   sh.w_early = w_early ? 1 : 0;
-  const int sub = rows_sub_bytes(sh, kGate);
-  const int share = (sh.k_blocks + plan.parts - 1) / plan.parts;
-  // 48 KB a stage (16 KB: 10-30 % slower, each stage costs its commit) in a
-  // ring of 200 KB (94 KB, beside the next launch's: 4-8 % slower).
-  constexpr int kStageTarget = 48 * 1024, kRing = 200 * 1024;
-  sh.k_sub = std::min(share, std::max(1, kStageTarget / sub));
-  const int stage = sub * sh.k_sub;
-  sh.stages = std::min({kRing / stage, kRowsMaxStages, (share + sh.k_sub - 1) / sh.k_sub});
-  sh.tail = (int)round_up(std::max(0, (128 - sh.block_pad - sh.tokens_pad) * 128), 1024);
-  // Tokens of a reduction round: what the stages hold in fp32.
-  constexpr int kTokenBytes = kAccs * 128 * 4;
-  if (sh.stages * stage + sh.tail < 16 * kTokenBytes) sh.tail = 16 * kTokenBytes;
-  sh.chunk = std::min(sh.tokens_pad, (sh.stages * stage + sh.tail) / kTokenBytes / 16 * 16);
-  const int smem = sh.stages * stage + sh.tail + kRowsBarBytes + 1024;
-  if (smem > kRowsMaxSmem) return B200_ERR_CUDA;
+  if (l.smem > kRowsMaxSmem) return B200_ERR_CUDA;
   CUtensorMap tw, tx;
   int rc = kWMajorN ? make_tmap_2d(&tw, w, k, n, ldw, 64, kBK, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)
                     : make_tmap_2d(&tw, w, (uint64_t)kAccs * n, k, ldw, kBK, sh.block,
@@ -298,7 +320,7 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ro
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(sh.n_blocks * ((tokens + sh.tile - 1) / sh.tile) * plan.parts));
   cfg.blockDim = dim3(kRowsThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = l.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -313,20 +335,24 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ro
   return e == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
 
-// Whether a product goes to the rows kernel, and how.  Both ways were measured
-// over 64 to 3000 rows: at 4096 x 12288 the block takes 54 us for 1 row and 64
-// for 128 (pair kernel 287 and 131: its loads of a mostly empty tile of x
-// collide), from 300 rows on the pair kernel is as fast; at 1000 x 2731 a
-// training step takes 102 us for 300 rows (152) and 169 for 1111 (191).
+// Whether a product goes to the rows kernel, and how, with `slots_of[i]`
+// clusters of 2^i CTAs resident.  Both ways were measured over 64 to 3000 rows:
+// at 4096 x 12288 the block takes 54 us for 1 row and 64 for 128 (pair kernel
+// 287 and 131: its loads of a mostly empty tile of x collide), from 300 rows on
+// the pair kernel is as fast; at 1000 x 2731 a training step takes 102 us for
+// 300 rows (152) and 169 for 1111 (191).
+bool rows_wins_on(int tokens, int n, int k, bool gate, bool w_major_n, const int (&slots_of)[4], int sm_count,
+                  RowsPlan& plan) {
+  if (tokens > 16 * kRowsMaxTokens) return false;
+  plan = plan_rows(tokens, n, k, gate ? 2 : 1, w_major_n, slots_of);
+  return plan.cycles < pair_cycles(tokens, n, k, gate ? 128 : 256, sm_count);
+}
 template <bool kBf16, int kMode, bool kWMajorN>
 bool rows_wins(int tokens, int n, int k, int sm_count, RowsPlan& plan) {
-  constexpr bool kGate = kMode == kRowsGateUp;
-  if (tokens > 16 * kRowsMaxTokens) return false;
   auto kern = gemm_rows_kernel<kBf16, kMode, kWMajorN>;
   int slots[4];
   for (int i = 0; i < 4; ++i) slots[i] = rows_clusters(kern, 1 << i, sm_count);
-  plan = plan_rows(tokens, n, k, kGate ? 2 : 1, kWMajorN, slots);
-  return plan.cycles < pair_cycles(tokens, n, k, kGate ? 128 : 256, sm_count);
+  return rows_wins_on(tokens, n, k, kMode == kRowsGateUp, kWMajorN, slots, sm_count, plan);
 }
 
 // Columns [hidden, hidden_pad) of a, g and u hold whatever the tile computed
@@ -445,6 +471,26 @@ extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t dim, int6
     n += in + w_in + w_out + out + (backward ? in + w_in + w_out : 0);
   }
   return n;
+}
+
+extern "C" int b200_gated_ffn_plan(int64_t rows, int64_t n, int64_t k, int product, int sm_count, int* ctas,
+                                   int* smem_bytes, int* tmem_columns) {
+  using namespace b200;
+  if (rows <= 0 || n <= 0 || k <= 0 || sm_count < 8 || !ctas || !smem_bytes || !tmem_columns)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (product < B200_FFN_GATE_UP || product > B200_FFN_IN_GRAD) return B200_ERR_INVALID_ARGUMENT;
+  if (rows > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  const bool gate = product == B200_FFN_GATE_UP, w_major_n = product == B200_FFN_GATE_GRAD || product == B200_FFN_IN_GRAD;
+  int slots[4];
+  for (int i = 0; i < 4; ++i) slots[i] = sm_count >> i;
+  RowsPlan plan;
+  *ctas = *smem_bytes = *tmem_columns = 0;
+  if (!rows_wins_on((int)rows, (int)n, (int)k, gate, w_major_n, slots, sm_count, plan)) return B200_OK;
+  const RowsLaunch l = rows_launch((int)rows, (int)n, (int)n, (int)k, gate, plan);
+  *ctas = plan.parts;
+  *smem_bytes = l.smem;
+  *tmem_columns = l.tmem_cols;
+  return B200_OK;
 }
 
 extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w_out, void* y, void* gate_up,

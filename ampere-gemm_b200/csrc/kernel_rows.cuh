@@ -78,6 +78,12 @@ struct RowsOut {
 __host__ __device__ inline int rows_sub_bytes(const RowsShape& s, bool gate) {
   return ((gate ? 2 : 1) * s.block_pad + s.tokens_pad) * 128;
 }
+// TMEM columns of a CTA: a power of two, 32 at least.
+__host__ __device__ inline int rows_tmem_columns(int accs, int tokens_pad) {
+  int cols = 32;
+  while (cols < accs * tokens_pad) cols *= 2;
+  return cols;
+}
 constexpr int kRowsBarBytes = (2 * kRowsMaxStages + 2) * 8 + 16;
 
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -253,8 +259,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   const int start = static_cast<int>(static_cast<int64_t>(cluster) * num_stages / (gridDim.x / parts));
   auto k_stage = [&](int it) { return it + start < num_stages ? it + start : it + start - num_stages; };
   auto subs = [&](int it) { return min(sh.k_sub, kb1 - kb0 - k_stage(it) * sh.k_sub); };
-  uint32_t tmem_cols = 32;
-  while (tmem_cols < static_cast<uint32_t>(kAccs * sh.tokens_pad)) tmem_cols *= 2;
+  const uint32_t tmem_cols = static_cast<uint32_t>(rows_tmem_columns(kAccs, sh.tokens_pad));
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmap_w);

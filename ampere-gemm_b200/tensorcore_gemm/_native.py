@@ -121,6 +121,8 @@ _SIGNATURES = {
         [ctypes.c_void_p] * 7 + [ctypes.c_int64] * 5 + [ctypes.c_int, ctypes.c_void_p],
     ),
     "b200_gated_ffn_workspace_size": (ctypes.c_int64, [ctypes.c_int64] * 4 + [ctypes.c_int] * 2),
+    "b200_gated_ffn_plan": (ctypes.c_int, [ctypes.c_int64] * 3 + [ctypes.c_int] * 2 +
+                            [ctypes.POINTER(ctypes.c_int)] * 3),
     "b200_gated_ffn_fwd": (
         ctypes.c_int,
         [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 8 +
@@ -296,6 +298,18 @@ def ipc_close(ptr: int) -> None:
 
 def ipc_free(ptr: int) -> None:
     check(load().b200_ipc_free(ctypes.c_void_p(int(ptr))), "b200_ipc_free")
+
+
+FFN_PRODUCTS = {"gate_up": 0, "out": 1, "gate_grad": 2, "in_grad": 3}
+
+
+def gated_ffn_plan(rows: int, n: int, k: int, product: str, sm_count: int = 148) -> tuple[int, int, int]:
+    """(CTAs of a cluster, shared memory, TMEM columns) of one of the block's products on the kernel for few
+    rows, (0, 0, 0) where it runs on the GEMM's tiles (b200_gated_ffn_plan); no GPU needed."""
+    out = [ctypes.c_int() for _ in range(3)]
+    check(load().b200_gated_ffn_plan(int(rows), int(n), int(k), FFN_PRODUCTS[product], int(sm_count),
+                                     *(ctypes.byref(v) for v in out)), "b200_gated_ffn_plan")
+    return tuple(v.value for v in out)
 
 
 VARIANT_NAMES = {v: k for k, v in VARIANTS.items()}

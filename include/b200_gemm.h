@@ -279,6 +279,20 @@ B200_API int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_in,
                                 int64_t ldw_out, int64_t lddx, int64_t lddw_in, int64_t lddw_out, int activation,
                                 int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * How one of the block's products over `rows` rows is launched, as
+ * b200_gemm_plan: host-only, for `sm_count` SMs (8 at least) that hold as many
+ * clusters as fit.  *ctas: CTAs of a cluster of the kernel for few rows, with
+ * the dynamic shared memory and the TMEM columns of each; all 0 when the
+ * product runs on the GEMM's tiles.
+ */
+#define B200_FFN_GATE_UP 0   /* x w_in^T with the activation; n = hidden, k = dim */
+#define B200_FFN_OUT 1       /* a w_out^T; n = out_dim, k = hidden */
+#define B200_FFN_GATE_GRAD 2 /* dy w_out with the activation's gradient; n = hidden, k = out_dim */
+#define B200_FFN_IN_GRAD 3   /* [dg du] w_in; n = dim, k = 2 hidden, each half rounded up to 8 */
+B200_API int b200_gated_ffn_plan(int64_t rows, int64_t n, int64_t k, int product, int sm_count, int* ctas,
+                                 int* smem_bytes, int* tmem_columns);
+
 /* Human-readable text of a return code (static storage). Counterpart of the
  * TORCH_CHECK messages of the reference launcher (gemm.py:33-47, 150-152). */
 B200_API const char* b200_gemm_strerror(int code);

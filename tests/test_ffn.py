@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from tensorcore_gemm import ffn
+from tensorcore_gemm import _native, ffn
 
 F16, BF16 = torch.float16, torch.bfloat16
 UNIT = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
@@ -342,3 +342,32 @@ def test_c_argument_checks_without_gpu(native_lib):
     for i, v, code in [(0, None, 1), (4, None, 1), (4, p + 2, 2), (16, 63, 1), (18, 60, 1),
                        (21, p + 8, 8), (22, 1535, 8)]:
         assert bwd(*with_(args, i, v)) == code, (i, v)
+
+
+# The products of a pass of (rows, dim, hidden, out_dim) as b200_gated_ffn_plan takes them.
+def products(rows, dim, hidden, out_dim):
+    pad = -(-hidden // 8) * 8
+    return {"gate_up": (rows, hidden, dim), "out": (rows, out_dim, hidden), "gate_grad": (rows, hidden, out_dim),
+            "in_grad": (rows, dim, 2 * pad)}
+
+
+SM_SHARED, CTA_RESERVED, TMEM_COLUMNS = 228 * 1024, 1024, 512   # of an SM; of each CTA; of an SM
+
+
+def test_few_rows_ctas_never_wait_for_tensor_memory(native_lib):
+    """CTAs of the few-rows kernel that share an SM find tensor memory for all of them.
+
+    A CTA whose allocation waited would hold up its cluster, and clusters that each hold what another one's CTA
+    waits for would never end.  With its share of the SM's shared memory at least its share of the tensor memory,
+    CTAs that fit the one fit the other, whichever launches they come from."""
+    seen = set()
+    for rows in (1, 8, 16, 17, 33, 64, 65, 100, 128, 129, 200, 256, 257, 400, 512, 700, 1500, 4000):
+        for n in (8, 64, 72, 128, 200, 384, 512, 1000, 2048, 2731, 4096, 12288):
+            for k in (8, 64, 128, 192, 256, 320, 512, 520, 1024, 2048, 4096, 12288):
+                for product in _native.FFN_PRODUCTS:
+                    ctas, smem, columns = _native.gated_ffn_plan(rows, n, k, product)
+                    if ctas:
+                        seen.add((ctas, columns))
+                        assert (smem + CTA_RESERVED) * TMEM_COLUMNS >= columns * SM_SHARED, (rows, n, k, product)
+                        assert smem <= SM_SHARED - CTA_RESERVED
+    assert {c for c, _ in seen} == {1, 2, 4, 8} and {t for _, t in seen} == {32, 64, 128, 256, 512}
