@@ -24,6 +24,16 @@ def check_cuda(name: str, t, dtypes=tuple(DTYPE_CODES)) -> None:
         raise RuntimeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
 
 
+def check_operand(name: str, t, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """`t`, contiguous, or an error where it is not what the kernels will read it as."""
+    check_cuda(name, t, (dtype,))
+    if t.shape != torch.Size(shape):
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}")
+    return t.contiguous()
+
+
 def as_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """`t` as a matrix of its last dimension's rows, and its row pitch.
 

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
                     workspace)
 
 ACTIVATIONS = {"silu": _native.B200_ACT_SILU, "gelu": _native.B200_ACT_GELU, "gelu_tanh": _native.B200_ACT_GELU_TANH}
@@ -146,6 +146,10 @@ def _(x, w_in, w_out, activation):
 def _gated_ffn_backward_op(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
                            gate_up: torch.Tensor,
                            activation: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check(x, w_in, w_out, activation)
+    out_dim, hidden = w_out.shape
+    dy = check_operand("dy", dy, (*x.shape[:-1], out_dim), x.dtype, x.device)
+    gate_up = check_operand("gate_up", gate_up, (x.shape[:-1].numel(), 2 * _pad8(hidden)), x.dtype, x.device)
     return _backward(dy, x, w_in, w_out, gate_up, activation, True, True, True)
 
 

@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
                     workspace)
 
 #: Most alternatives a call can ask for.
@@ -157,6 +157,12 @@ def _(logits, targets, top_k, ignore_index):
 def _token_logprobs_backward_op(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor,
                                 entropy: torch.Tensor, g_logprob: Optional[torch.Tensor],
                                 g_entropy: Optional[torch.Tensor], ignore_index: int) -> torch.Tensor:
+    _check(logits, targets, 0)
+    f32, dev = torch.float32, logits.device
+    stats = check_operand("stats", stats, (*targets.shape, 2), f32, dev)
+    entropy = check_operand("entropy", entropy, targets.shape, f32, dev)
+    g_logprob, g_entropy = (None if g is None else check_operand(name, g, targets.shape, f32, dev)
+                            for name, g in (("g_logprob", g_logprob), ("g_entropy", g_entropy)))
     return _backward(logits, targets, stats, entropy, g_logprob, g_entropy, ignore_index)
 
 

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, launch, once_differentiable, plain_eager, ptr, wants_grad,
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
                     workspace)
 
 
@@ -135,6 +135,12 @@ def _(x, weight, bias, eps):
 @torch.library.custom_op("tensorcore_gemm::layer_norm_backward", mutates_args=())
 def _layer_norm_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
                             wdtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check(x, weight, None)
+    if wdtype not in (x.dtype, torch.float32) or (weight is not None and weight.dtype != wdtype):
+        raise RuntimeError("wdtype must be weight's dtype, and x's or float32")
+    dy = check_operand("dy", dy, x.shape, x.dtype, x.device)
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    stats = check_operand("stats", stats, (2, rows), torch.float32, x.device)
     return _backward(dy, x, weight, stats, wdtype, True, True)
 
 

@@ -371,3 +371,23 @@ def test_few_rows_ctas_never_wait_for_tensor_memory(native_lib):
                         assert (smem + CTA_RESERVED) * TMEM_COLUMNS >= columns * SM_SHARED, (rows, n, k, product)
                         assert smem <= SM_SHARED - CTA_RESERVED
     assert {c for c, _ in seen} == {1, 2, 4, 8} and {t for _, t in seen} == {32, 64, 128, 256, 512}
+
+
+@pytest.mark.gpu
+def test_backward_operator_refusals(cuda_device, native_lib):
+    """The backward operator refuses what its kernels would read out of range."""
+    op = torch.ops.tensorcore_gemm.gated_ffn_backward
+    x, w_in, w_out, dy = make(40, 64, 70, 56, F16, cuda_device)
+    _, gu = torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, "silu")
+    for p, q in zip(op(dy, x, w_in, w_out, gu, "silu"), run(x, w_in, w_out, "silu", dy)[1:]):
+        assert torch.equal(p, q)
+    assert torch.equal(op(dy, x, w_in, w_out, gu.t().contiguous().t(), "silu")[0], op(dy, x, w_in, w_out, gu, "silu")[0])
+    for args, match in [((dy[:, :40], x, w_in, w_out, gu), "dy must have shape"), ((dy[:8], x, w_in, w_out, gu), "dy must have"),
+                        ((dy.float(), x, w_in, w_out, gu), "dy must be"), ((dy.cpu(), x, w_in, w_out, gu), "CUDA"),
+                        ((dy, x, w_in, w_out, gu[:8]), "gate_up must have"), ((dy, x, w_in, w_out, gu[:, :140]), "gate_up must"),
+                        ((dy, x, w_in, w_out, gu.bfloat16()), "gate_up must be"), ((dy, x, w_in[:, :32], w_out, gu), "Inner"),
+                        ((dy, x[:8], w_in, w_out, gu), "dy must have")]:
+        with pytest.raises(RuntimeError, match=match):
+            op(*args, "silu")
+    with pytest.raises(ValueError, match="Unsupported activation"):
+        op(dy, x, w_in, w_out, gu, "relu")

@@ -444,3 +444,21 @@ def test_forced_token(cuda_device, native_lib, rows, vocab, dtype):
     gl, gh = (torch.randn(rows, device=cuda_device) for _ in range(2))
     dx, = torch.autograd.grad((q.logprobs, q.entropy), (leaf,), (gl, gh))
     ex.check_grad(dx, gl, gh)
+
+
+@pytest.mark.gpu
+def test_backward_operator_refusals(cuda_device, native_lib):
+    """The backward operator refuses what its kernels would read out of range."""
+    op = torch.ops.tensorcore_gemm.token_logprobs_backward
+    x, t = make(6, 90, BF16, cuda_device)
+    _, ent, stats, *_ = torch.ops.tensorcore_gemm.token_logprobs(x, t, 0, -100)
+    g = torch.randn(6, device=cuda_device)
+    Exact(x, t).check_grad(op(x, t, stats, ent, g, g, -100), g, g)
+    Exact(x, t).check_grad(op(x, t, stats.t().contiguous().t(), ent, g, None, -100), g, 0 * g)
+    for args, match in [((x, t, stats[:3], ent, g, g), "stats must have shape"), ((x, t, stats.double(), ent, g, g), "stats must be"),
+                        ((x, t, stats, ent[:3], g, g), "entropy must"), ((x, t, stats, ent, g[:3], g), "g_logprob must"),
+                        ((x, t, stats, ent, g, g.half()), "g_entropy must"), ((x, t, stats, ent, None, g[:1]), "g_entropy must"),
+                        ((x, t[:3], stats, ent, g, g), "shape"), ((x, t, stats.cpu(), ent, g, g), "CUDA"),
+                        ((x.double(), t, stats, ent, g, g), "logits must")]:
+        with pytest.raises(RuntimeError, match=match):
+            op(*args, -100)

@@ -292,3 +292,20 @@ def test_c_argument_checks_without_gpu(native_lib):
     assert size(-1, 8) == -1 and size(10, 8) == 10 * 2 * 8 * 4
     assert bwd(p, p, None, p, p, p, p, p, 10, 8, 8, 8, 8, 0, 0, p, 639, None) == 8      # workspace one byte short
     assert bwd(p, p, None, p, p, p, p, p, 10, 8, 8, 8, 8, 0, 0, p + 4, 640, None) == 8  # and misaligned
+
+
+@pytest.mark.gpu
+def test_backward_operator_refusals(cuda_device, native_lib):
+    """The backward operator refuses what its kernels would read out of range."""
+    op = torch.ops.tensorcore_gemm.layer_norm_backward
+    x, w, b, dy = make(6, 64, BF16, BF16, cuda_device)
+    _, stats = torch.ops.tensorcore_gemm.layer_norm(x, w, b, EPS)
+    check_backward(*op(dy, x, w, stats, BF16), x, w, dy)
+    check_backward(*op(dy, x, w, stats.t().contiguous().t(), BF16), x, w, dy)
+    for args, match in [((dy[:, :32], x, w, stats, BF16), "dy must have shape"), ((dy[:3], x, w, stats, BF16), "dy must have"),
+                        ((dy.half(), x, w, stats, BF16), "dy must be"), ((dy.cpu(), x, w, stats, BF16), "CUDA"),
+                        ((dy, x, w, stats[:, :3], BF16), "stats must have"), ((dy, x, w, stats.double(), BF16), "stats must be"),
+                        ((dy, x, w, stats[:1], BF16), "stats must have"), ((dy, x, w[:8], stats, BF16), "weight must be"),
+                        ((dy, x, w, stats, F32), "wdtype"), ((dy, x, None, stats, F16), "wdtype")]:
+        with pytest.raises(RuntimeError, match=match):
+            op(*args)
