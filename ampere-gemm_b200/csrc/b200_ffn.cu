@@ -426,12 +426,19 @@ int product(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int
                     kWMajorN ? B200_B_ROW_MAJOR : B200_B_COL_MAJOR, stream);
 }
 
+// Dimensions, 2 hidden rounded up among them, are rounded up to tiles and dealt
+// out in even shares with 32 bits.
+constexpr int64_t kMaxDim = 0x7f000000;
+bool too_large(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim) {
+  return rows > kMaxDim || dim > kMaxDim || hidden > kMaxDim / 2 || out_dim > kMaxDim;
+}
+
 // Checks shared by the two directions; *empty: some dimension is 0.
 int check_ffn(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, int activation, int dtype, bool* empty) {
   if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return B200_ERR_INVALID_ARGUMENT;
   if (activation < B200_ACT_SILU || activation > B200_ACT_GELU_TANH) return B200_ERR_INVALID_ARGUMENT;
   if (dtype != B200_DTYPE_F16 && dtype != B200_DTYPE_BF16) return B200_ERR_INVALID_ARGUMENT;
-  if (rows > 0x7fffffff || dim > 0x7fffffff || hidden > 0x3fffffff || out_dim > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (too_large(rows, dim, hidden, out_dim)) return B200_ERR_TOO_LARGE;
   *empty = rows == 0 || dim == 0 || hidden == 0 || out_dim == 0;
   return B200_OK;
 }
@@ -461,8 +468,7 @@ extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t dim, int6
                                                  int backward, int unaligned) {
   using namespace b200;
   if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return -B200_ERR_INVALID_ARGUMENT;
-  if (rows > 0x7fffffff || dim > 0x7fffffff || hidden > 0x3fffffff || out_dim > 0x7fffffff)
-    return -B200_ERR_TOO_LARGE;
+  if (too_large(rows, dim, hidden, out_dim)) return -B200_ERR_TOO_LARGE;
   const int64_t hp = pad8(hidden);
   int64_t n = part_bytes(rows, hp) + (backward ? part_bytes(rows, 2 * hp) : 0);
   if (unaligned || hidden % 8 != 0 || dim % 8 != 0 || out_dim % 8 != 0) {
@@ -479,7 +485,7 @@ extern "C" int b200_gated_ffn_plan(int64_t rows, int64_t n, int64_t k, int produ
   if (rows <= 0 || n <= 0 || k <= 0 || sm_count < 8 || !ctas || !smem_bytes || !tmem_columns)
     return B200_ERR_INVALID_ARGUMENT;
   if (product < B200_FFN_GATE_UP || product > B200_FFN_IN_GRAD) return B200_ERR_INVALID_ARGUMENT;
-  if (rows > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (rows > kMaxDim || n > kMaxDim || k > kMaxDim) return B200_ERR_TOO_LARGE;
   const bool gate = product == B200_FFN_GATE_UP, w_major_n = product == B200_FFN_GATE_GRAD || product == B200_FFN_IN_GRAD;
   int slots[4];
   for (int i = 0; i < 4; ++i) slots[i] = sm_count >> i;

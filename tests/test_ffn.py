@@ -391,3 +391,21 @@ def test_backward_operator_refusals(cuda_device, native_lib):
             op(*args, "silu")
     with pytest.raises(ValueError, match="Unsupported activation"):
         op(dy, x, w_in, w_out, gu, "relu")
+
+
+def test_dimension_limits_without_gpu(native_lib):
+    """Sizes whose rounding up would pass 32 bits are refused, not wrapped (2 hidden as a depth, above all)."""
+    size, fwd, bwd = (native_lib.b200_gated_ffn_workspace_size, native_lib.b200_gated_ffn_fwd,
+                      native_lib.b200_gated_ffn_bwd)
+    p, most = 4096, 0x7f000000
+    for dims in [(1, 8, 0x3fffffff, 8), (1, 8, most // 2 + 1, 8), (most + 1, 8, 8, 8), (0x7fffffff, 1, 1, 1),
+                 (1, most + 1, 8, 8), (1, 8, 8, 0x7fffffff)]:
+        rows, dim, hidden, out_dim = dims
+        assert size(*dims, 0, 0) == size(*dims, 1, 0) == -3
+        assert fwd(*[p] * 5, *dims, dim, dim, hidden, out_dim, 0, 1, p, 1 << 62, None) == 3
+        assert bwd(*[p] * 8, *dims, out_dim, dim, dim, hidden, dim, dim, hidden, 0, 1, p, 1 << 62, None) == 3
+    assert size(1, 8, most // 2, 8, 1, 0) > 0 and size(1, most, 8, 8, 1, 0) > 0 and size(most, 8, 8, 8, 1, 0) > 0
+    for product in _native.FFN_PRODUCTS:                    # the plan's own arithmetic at the limits
+        for rows, n, k in [(1, most, 8), (300, most, 64), (1, 8, most), (most, 8, 8)]:
+            ctas, smem, columns = _native.gated_ffn_plan(rows, n, k, product)
+            assert ctas in (0, 1, 2, 4, 8) and 0 <= smem <= 227 * 1024 and columns <= 512
