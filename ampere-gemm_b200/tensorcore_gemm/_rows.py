@@ -86,9 +86,13 @@ def launch(name: str, dev: int, *args) -> None:
         _native.check(code, name)
 
 
+_DISPATCH_MODES, _JIT_TRACE = torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+
+
 def plain_eager(*tensors) -> bool:
-    """True when the call can go straight to the kernels: real tensors, not being traced."""
-    if torch.compiler.is_compiling():
+    """True when the call can go straight to the kernels: real tensors, and nobody who listens at the dispatcher
+    (a compiler, a dispatch mode such as make_fx's, torch.jit.trace)."""
+    if torch.compiler.is_compiling() or _DISPATCH_MODES() or _JIT_TRACE() is not None:
         return False
     for t in tensors:
         if isinstance(t, torch.Tensor) and type(t) not in (torch.Tensor, torch.nn.Parameter):

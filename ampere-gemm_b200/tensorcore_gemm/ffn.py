@@ -104,7 +104,10 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return *_backward(dy, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:3]), None
+        if plain_eager(dy):
+            return *_backward(dy, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:3]), None
+        grads = torch.ops.tensorcore_gemm.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation)
+        return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None
 
 
 def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:

@@ -101,7 +101,9 @@ class _TokenLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logprob, g_entropy, _g_top, _g_index):
         logits, targets, stats, entropy = ctx.saved_tensors
-        return _backward(logits, targets, stats, entropy, g_logprob, g_entropy, ctx.ignore_index), None, None, None
+        eager = plain_eager(g_logprob, g_entropy)
+        backward = _backward if eager else torch.ops.tensorcore_gemm.token_logprobs_backward
+        return backward(logits, targets, stats, entropy, g_logprob, g_entropy, ctx.ignore_index), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,

@@ -93,8 +93,11 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = _backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
-        return dx if need_x else None, dw, db, None
+        if plain_eager(dy):
+            dx, dw, db = _backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
+        else:
+            dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype)
+        return dx if need_x else None, dw if need_w else None, db if need_b else None, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
