@@ -6,6 +6,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .gemm import _GET_DEVICE, _current_stream
@@ -101,7 +102,19 @@ def plain_eager(*tensors) -> bool:
 
 
 def wants_grad(*tensors) -> bool:
+    """True when the call has to be an autograd.Function's: gradients are wanted, or, within a dual level, may be
+    (the Function raises for an operand with a tangent, as it has no forward-mode derivative)."""
+    if forward_ad._current_level >= 0:
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def refuse_tangents(*tensors) -> None:
+    """For the dispatcher operators, which torch.library would otherwise let drop a tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this operator has no forward-mode derivative (jvp)")
 
 
 class _Refuse(torch.autograd.Function):

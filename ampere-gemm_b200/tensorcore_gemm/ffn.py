@@ -16,8 +16,8 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
-                    workspace)
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr,
+                    refuse_tangents, wants_grad, workspace)
 
 ACTIVATIONS = {"silu": _native.B200_ACT_SILU, "gelu": _native.B200_ACT_GELU, "gelu_tanh": _native.B200_ACT_GELU_TANH}
 
@@ -134,6 +134,7 @@ def _gated_ffn_op(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
                   activation: str) -> tuple[torch.Tensor, torch.Tensor]:
     """y and [g u] of `gated_ffn` (the latter is not differentiable)."""
     _check(x, w_in, w_out, activation)
+    refuse_tangents(x, w_in, w_out)
     return _forward(x, w_in, w_out, activation, True)
 
 

@@ -19,8 +19,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
-                    workspace)
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr,
+                    refuse_tangents, wants_grad, workspace)
 
 #: Most alternatives a call can ask for.
 MAX_TOP = _native.B200_LOGPROBS_MAX_TOP
@@ -139,6 +139,7 @@ def _token_logprobs_op(
         ignore_index: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """logprobs, entropy, stats, top_logprobs, top_indices (the last three are not differentiable)."""
     _check(logits, targets, top_k)
+    refuse_tangents(logits)
     lp, ent, stats, tv, ti = _forward(logits, targets, top_k, ignore_index)
     if not top_k:
         tv, ti = (torch.empty((*targets.shape, 0), dtype=d, device=logits.device) for d in (torch.float32, torch.int64))

@@ -17,8 +17,8 @@ from typing import Optional
 import torch
 
 from . import _native
-from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr, wants_grad,
-                    workspace)
+from ._rows import (DTYPE_CODES, as_rows, check_cuda, check_operand, launch, once_differentiable, plain_eager, ptr,
+                    refuse_tangents, wants_grad, workspace)
 
 
 def _check(x, weight, bias) -> None:
@@ -124,6 +124,7 @@ def _layer_norm_op(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Option
                    eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """y of `layer_norm`, and the rows' mean and 1 / standard deviation (not differentiable)."""
     _check(x, weight, bias)
+    refuse_tangents(x, weight, bias)
     return _forward(x, weight, bias, eps, True)
 
 

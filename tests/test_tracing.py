@@ -1,8 +1,9 @@
-"""The row operators under tracers and dispatch modes: traced in full, never silently wrong."""
+"""The row operators under tracers, dispatch modes and forward mode: traced in full, or refused, never silently wrong."""
 from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
@@ -91,3 +92,27 @@ def test_jit_trace(cuda_device, native_lib, name):
     traced = torch.jit.trace(call, first, check_trace=False)
     assert f"tensorcore_gemm::{name}" in str(traced.graph)
     assert same(traced(*other), call(*other))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(OPERATORS))
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(cuda_device, native_lib, name, grad):
+    """No forward-mode derivative: an operand with a tangent raises, at the entry point and at the dispatcher."""
+    call, args, _ = OPERATORS[name]
+    operands = args(cuda_device, 1)[0]
+    want = call(*operands)
+    with forward_ad.dual_level():
+        assert same(call(*operands), want)                   # no tangent among them
+        for i in range(len(operands)):
+            dual = list(operands)
+            dual[i] = forward_ad.make_dual(operands[i].clone().requires_grad_(grad), torch.ones_like(operands[i]))
+            with pytest.raises(RuntimeError, match="jvp"):
+                call(*dual)
+        x = forward_ad.make_dual(operands[0].clone().requires_grad_(grad), torch.ones_like(operands[0]))
+        rest = {"layer_norm": (*operands[1:], 1e-5), "gated_ffn": (*operands[1:], "silu"),
+                "token_logprobs": (torch.arange(9, device=cuda_device), 0, -100)}[name]
+        with pytest.raises(RuntimeError, match="jvp"):
+            getattr(torch.ops.tensorcore_gemm, name)(x, *rest)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: call(t, *operands[1:])[0], (operands[0],), (torch.ones_like(operands[0]),))
