@@ -92,11 +92,11 @@ _DISPATCH_MODES, _JIT_TRACE = torch._C._len_torch_dispatch_stack, torch._C._get_
 
 def plain_eager(*tensors) -> bool:
     """True when the call can go straight to the kernels: real tensors, and nobody who listens at the dispatcher
-    (a compiler, a dispatch mode such as make_fx's, torch.jit.trace)."""
+    (a compiler, a dispatch mode such as make_fx's, torch.jit.trace) or works through it (negated views)."""
     if torch.compiler.is_compiling() or _DISPATCH_MODES() or _JIT_TRACE() is not None:
         return False
     for t in tensors:
-        if isinstance(t, torch.Tensor) and type(t) not in (torch.Tensor, torch.nn.Parameter):
+        if isinstance(t, torch.Tensor) and (type(t) not in (torch.Tensor, torch.nn.Parameter) or t.is_neg()):
             return False
     return True
 

@@ -116,3 +116,12 @@ def test_tangents_are_refused(cuda_device, native_lib, name, grad):
             getattr(torch.ops.tensorcore_gemm, name)(x, *rest)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: call(t, *operands[1:])[0], (operands[0],), (torch.ones_like(operands[0]),))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(OPERATORS))
+def test_negated_views(cuda_device, native_lib, name):
+    """The imaginary part of a conjugate is a view whose memory holds the negated values."""
+    call, args, _ = OPERATORS[name]
+    operands = args(cuda_device, 1)[0]
+    assert same(call(*(torch._neg_view(t) for t in operands)), call(*(-t for t in operands)))
