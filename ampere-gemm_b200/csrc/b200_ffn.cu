@@ -409,21 +409,44 @@ int gate_bwd(const void* dy, int64_t lddy, const void* w_out, int64_t ldw, const
   return launch_gate<kBf16, kEpiGateBwd>(dy, lddy, w_out, ldw, a, s, fx, stream);
 }
 
+// Whether the GEMM may split the last wave of an M x N x K product along K: all
+// those that it would on a device of 64 pairs of SMs or more, by a rule on sizes
+// alone, so that a workspace's size does not depend on the device.
+bool may_split(int64_t M, int64_t N, int64_t K) {
+  return K > 2048 && ((M + 255) / 256) * ((N + 255) / 256) > 64;
+}
+// Bytes of the workspace that the block's products share for it.
+int64_t split_bytes(int64_t rows, int64_t dim, int64_t hidden, int64_t out_dim, bool backward) {
+  const bool any = backward ? may_split(rows, dim, 2 * pad8(hidden)) || may_split(2 * hidden, dim, rows) ||
+                                  may_split(out_dim, hidden, rows)
+                            : may_split(rows, out_dim, hidden);
+  return any ? round_up(kSplitBytes, 256) : 0;
+}
+// Takes it out of the call's workspace, its counters set to zero on `stream`; NULL for none.
+int take_split(Carver& ws, int64_t bytes, void** split_ws, cudaStream_t stream) {
+  *split_ws = bytes > 0 ? ws.at : nullptr;
+  if (bytes == 0) return B200_OK;
+  constexpr int64_t kParts = kSplitParts * kSplitPartBytes;
+  uint8_t* counters = ws.at + kParts;
+  ws.at += bytes;
+  return cudaMemsetAsync(counters, 0, kSplitBytes - kParts, stream) == cudaSuccess ? B200_OK : B200_ERR_CUDA;
+}
+
 int plain_gemm(bool bf16, const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
-               int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* stream) {
-  return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, stream);
+               int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* split_ws, void* stream) {
+  return (bf16 ? gemm_bf16_run : gemm_f16_run)(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, split_ws, stream);
 }
 
 // C = A B with A rows x k, B stored n x k or k x n (kWMajorN), on the kernel that is faster.
 template <bool kBf16, bool kWMajorN>
 int product(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int rows, int n, int k,
-            bool b_early, const DeviceInfo& dev, cudaStream_t stream) {
+            bool b_early, const DeviceInfo& dev, void* split_ws, cudaStream_t stream) {
   RowsPlan plan;
   if (rows_wins<kBf16, kRowsPlain, kWMajorN>(rows, n, k, dev.sm_count, plan))
     return launch_rows<kBf16, kRowsPlain, kWMajorN>(A, lda, B, ldb, RowsOut{static_cast<uint16_t*>(C), ldc}, rows, n, n,
                                                     k, 0, b_early, plan, stream);
   return plain_gemm(kBf16, A, B, C, rows, n, k, lda, ldb, ldc, B200_A_ROW_MAJOR,
-                    kWMajorN ? B200_B_ROW_MAJOR : B200_B_COL_MAJOR, stream);
+                    kWMajorN ? B200_B_ROW_MAJOR : B200_B_COL_MAJOR, split_ws, stream);
 }
 
 // Dimensions, 2 hidden rounded up among them, are rounded up to tiles and dealt
@@ -470,7 +493,8 @@ extern "C" int64_t b200_gated_ffn_workspace_size(int64_t rows, int64_t dim, int6
   if (rows < 0 || dim < 0 || hidden < 0 || out_dim < 0) return -B200_ERR_INVALID_ARGUMENT;
   if (too_large(rows, dim, hidden, out_dim)) return -B200_ERR_TOO_LARGE;
   const int64_t hp = pad8(hidden);
-  int64_t n = part_bytes(rows, hp) + (backward ? part_bytes(rows, 2 * hp) : 0);
+  int64_t n = part_bytes(rows, hp) + (backward ? part_bytes(rows, 2 * hp) : 0) +
+              split_bytes(rows, dim, hidden, out_dim, backward != 0);
   if (unaligned || hidden % 8 != 0 || dim % 8 != 0 || out_dim % 8 != 0) {
     const int64_t in = part_bytes(rows, dim), w_in = part_bytes(2 * hp, dim), w_out = part_bytes(out_dim, hp),
                   out = part_bytes(rows, out_dim);
@@ -526,6 +550,8 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   Carver ws{static_cast<uint8_t*>(workspace)};
   CopyJobs before, after;
   uint16_t* a = ws.take(rows, hp);
+  void* split_ws = nullptr;
+  if (int rc = take_split(ws, split_bytes(rows, dim, hidden, out_dim, false), &split_ws, stream)) return rc;
   x = readable(x, ldx, rows, dim, ws, before);
   w_in = readable(w_in, ldw_in, 2 * hidden, dim, ws, before);
   w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
@@ -537,7 +563,7 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   y = writable(y, ldy, rows, out_dim, ws, after);
   // w_out was written two kernels ago at the latest: its loads may start early.
   rc = (bf16 ? product<true, false> : product<false, false>)(a, hp, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim,
-                                                             (int)hidden, true, dev, stream);
+                                                             (int)hidden, true, dev, split_ws, stream);
   return rc ? rc : run_copies(after, stream);
 }
 
@@ -573,6 +599,8 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
   CopyJobs before, after;
   uint16_t* a = ws.take(rows, hp);
   uint16_t* dgu = ws.take(rows, 2 * hp);
+  void* split_ws = nullptr;
+  if (int rc = take_split(ws, split_bytes(rows, dim, hidden, out_dim, true), &split_ws, stream)) return rc;
   dy = readable(dy, lddy, rows, out_dim, ws, before);
   w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
   if (dw_in) x = readable(x, ldx, rows, dim, ws, before);
@@ -598,7 +626,7 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
   if (dx) {
     dx = writable(dx, lddx, rows, dim, ws, after);
     rc = (bf16 ? product<true, true> : product<false, true>)(dgu, 2 * hp, w_in, ldw_in, dx, lddx, (int)rows, (int)dim,
-                                                             (int)(2 * hp), true, dev, stream);
+                                                             (int)(2 * hp), true, dev, split_ws, stream);
     if (rc) return rc;
   }
   if (dw_in) {
@@ -607,14 +635,14 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
     const int parts = hidden == hp ? 1 : 2;
     for (int half = 0; half < parts; ++half) {
       rc = plain_gemm(bf16, dgu + half * hp, x, out + half * hidden * lddw_in, 2 * hidden / parts, dim, rows, 2 * hp,
-                      ldx, lddw_in, B200_A_COL_MAJOR, B200_B_ROW_MAJOR, stream_ptr);
+                      ldx, lddw_in, B200_A_COL_MAJOR, B200_B_ROW_MAJOR, split_ws, stream_ptr);
       if (rc) return rc;
     }
   }
   if (dw_out) {
     dw_out = writable(dw_out, lddw_out, out_dim, hidden, ws, after);
     rc = plain_gemm(bf16, dy, a, dw_out, out_dim, hidden, rows, lddy, hp, lddw_out, B200_A_COL_MAJOR,
-                    B200_B_ROW_MAJOR, stream_ptr);
+                    B200_B_ROW_MAJOR, split_ws, stream_ptr);
     if (rc) return rc;
   }
   return run_copies(after, stream);

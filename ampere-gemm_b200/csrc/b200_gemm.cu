@@ -179,11 +179,8 @@ int gemm_repacked(const void* A, const void* B, void* C, int64_t M, int64_t N, i
 }  // namespace b200
 
 int b200::gemm_f16_run(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
-                       int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* stream) {
-  DeviceInfo dev;
-  if (int rc = current_device_info(dev)) return rc;
-  return gemm_aligned<false>(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, EpiParams{}, dev,
-                             static_cast<cudaStream_t>(stream));
+                       int64_t ldb, int64_t ldc, int a_layout, int b_layout, void* split_ws, void* stream) {
+  return gemm_run<false>(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, split_ws, stream);
 }
 
 extern "C" int b200_gemm_f16(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,

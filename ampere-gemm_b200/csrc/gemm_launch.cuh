@@ -14,6 +14,7 @@
 #include <utility>
 
 #include "gemm_common.cuh"
+#include "gemm_internal.h"
 #include "kernel_cta1.cuh"
 #include "kernel_cta2.cuh"
 #include "kernel_skinny.cuh"
@@ -199,6 +200,7 @@ struct CallOptions {
   bool no_split = false;           // run every tile whole: no split workspace (allocation-free entry)
   uint64_t withhold_fixup_ns = 0;  // fixup-wait self-test (see SplitTail)
   int force_variant = -1;          // >= 0: this variant instead of b200_gemm_set_variant's / auto
+  void* split_ws = nullptr;        // kSplitBytes of the caller's memory instead of the stream's own workspace
 };
 thread_local CallOptions t_call;
 
@@ -255,7 +257,15 @@ int launch_tcgen05_pair(const GemmArgs& g, int group_m) {
     s2.dp_tiles = (int)(tiles - r);
     s2.S = S;
     s2.withhold_fixup_ns = t_call.withhold_fixup_ns;
-    if (split_workspace(stream, sm_count, s2)) st = s2;
+    if (t_call.split_ws) {
+      if (2 * r * S <= kSplitParts) {
+        s2.ws = static_cast<float*>(t_call.split_ws);
+        s2.counters = reinterpret_cast<uint32_t*>(s2.ws + (size_t)kSplitParts * kPartFloats);
+        st = s2;
+      }
+    } else if (split_workspace(stream, sm_count, s2)) {
+      st = s2;
+    }
     if (std::getenv("B200_GEMM_DEBUG"))
       std::fprintf(stderr, "b200_gemm: %lld tiles on %d pairs, last %lld tiles split %d ways%s\n", tiles, grid_pairs, r,
                    S, st.S > 1 ? "" : " (no workspace: unsplit)");
@@ -522,6 +532,21 @@ int gemm_aligned(const void* A, const void* B, void* C, int64_t M, int64_t N, in
   return with_layouts(row_b, col_a, [&](auto rb, auto ca) {
     return launch_tcgen05<kBf16, 256, 4, decltype(rb)::value, decltype(ca)::value>(g, group_m);
   });
+}
+
+// See gemm_f16_run() in gemm_internal.h.
+template <bool kBf16>
+int gemm_run(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
+             int64_t ldc, int a_layout, int b_layout, void* split_ws, void* stream) {
+  static_assert(kSplitPartBytes == kPartFloats * sizeof(float), "a part is one CTA's share of a pair tile");
+  DeviceInfo dev;
+  if (int rc = current_device_info(dev)) return rc;
+  CallOptions opts;
+  opts.no_split = split_ws == nullptr;
+  opts.split_ws = split_ws;
+  ScopedCallOptions scope(opts);
+  return gemm_aligned<kBf16>(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, EpiParams{}, dev,
+                             static_cast<cudaStream_t>(stream));
 }
 
 // Reads and clears this translation unit's error word (0: none, negative: a CUDA error).

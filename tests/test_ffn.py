@@ -409,3 +409,51 @@ def test_dimension_limits_without_gpu(native_lib):
         for rows, n, k in [(1, most, 8), (300, most, 64), (1, 8, most), (most, 8, 8)]:
             ctas, smem, columns = _native.gated_ffn_plan(rows, n, k, product)
             assert ctas in (0, 1, 2, 4, 8) and 0 <= smem <= 227 * 1024 and columns <= 512
+
+
+# A training step whose dw_out is a product that the GEMM splits along K in its last wave.
+SPLIT = (8192, 64, 2048, 2560)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_split_products_use_the_callers_workspace(cuda_device, native_lib, dtype):
+    """No device memory is allocated, whatever the stream, and a captured step computes what an eager one does."""
+    rows, dim, hidden, out_dim = SPLIT
+    assert _native.plan(out_dim, hidden, rows) == ("pair", 4)
+    x, w_in, w_out, dy = make(*SPLIT, dtype, cuda_device)
+    check_all(x, w_in, w_out, "silu", dy)
+    code = 0 if dtype == F16 else 1
+    gu = torch.empty((rows, 2 * hidden), dtype=dtype, device=cuda_device)
+    y, dx, dwi, dwo = (torch.empty_like(t) for t in (dy, x, w_in, w_out))
+    ws = torch.empty(native_lib.b200_gated_ffn_workspace_size(*SPLIT, 1, 0), dtype=torch.uint8, device=cuda_device)
+
+    def step(stream):
+        p = [t.data_ptr() for t in (x, w_in, w_out, y, gu)]
+        assert native_lib.b200_gated_ffn_fwd(*p, *SPLIT, dim, dim, hidden, out_dim, 0, code, ws.data_ptr(), ws.numel(),
+                                             stream.cuda_stream) == 0
+        p = [t.data_ptr() for t in (dy, x, w_in, w_out, gu, dx, dwi, dwo)]
+        assert native_lib.b200_gated_ffn_bwd(*p, *SPLIT, out_dim, dim, dim, hidden, dim, dim, hidden, 0, code,
+                                             ws.data_ptr(), ws.numel(), stream.cuda_stream) == 0
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    step(streams[0])
+    streams[0].synchronize()
+    want = [t.clone() for t in (y, dx, dwi, dwo)]
+    free = torch.cuda.mem_get_info()[0]
+    ws.fill_(255)                                            # leftovers of another use
+    torch.cuda.synchronize()
+    step(streams[1])
+    streams[1].synchronize()
+    assert torch.cuda.mem_get_info()[0] == free
+    assert all(torch.equal(p, q) for p, q in zip((y, dx, dwi, dwo), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream())
+    for t in (y, dx, dwi, dwo):
+        t.zero_()
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip((y, dx, dwi, dwo), want))
