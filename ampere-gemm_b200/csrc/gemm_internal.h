@@ -14,8 +14,8 @@ constexpr int64_t kSplitBytes = kSplitParts * kSplitPartBytes + 1024;
 // C = A * B (fp32 accumulate, rounded once to the operands' type) on operands
 // that satisfy TMA's alignment rules, M and N > 0, on the current device;
 // layouts as in b200_gemm_f16_ex.  `split_ws` is kSplitBytes of the caller's
-// memory (NULL: every tile runs whole); nothing is allocated.  `stream` is a
-// cudaStream_t.
+// memory (NULL: every tile runs whole); nothing is allocated, and
+// b200_gemm_set_variant does not apply.  `stream` is a cudaStream_t.
 int gemm_f16_run(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
                  int64_t ldc, int a_layout, int b_layout, void* split_ws, void* stream);
 int gemm_bf16_run(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,

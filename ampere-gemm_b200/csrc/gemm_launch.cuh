@@ -543,6 +543,7 @@ int gemm_run(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_
   if (int rc = current_device_info(dev)) return rc;
   CallOptions opts;
   opts.no_split = split_ws == nullptr;
+  opts.force_variant = B200_VARIANT_AUTO;
   opts.split_ws = split_ws;
   ScopedCallOptions scope(opts);
   return gemm_aligned<kBf16>(A, B, C, M, N, K, lda, ldb, ldc, a_layout, b_layout, EpiParams{}, dev,

@@ -256,8 +256,8 @@ B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets,
  * start on 16 bytes cost a copy.  The workspace (256-byte aligned) must not be
  * reused until the call's work on `stream` has finished; its size is
  * b200_gated_ffn_workspace_size(), with `unaligned` != 0 when the rows of any
- * operand do not start on 16 bytes; the call allocates no memory besides it.
- * Dimensions, 2 hidden among them, are at
+ * operand do not start on 16 bytes; the call allocates no memory besides it,
+ * and b200_gemm_set_variant does not apply to its products.  Dimensions, 2 hidden among them, are at
  * most 0x7f000000.  No counterpart in the reference.
  */
 #define B200_ACT_SILU 0      /* g / (1 + exp(-g)) */

@@ -457,3 +457,17 @@ def test_split_products_use_the_callers_workspace(cuda_device, native_lib, dtype
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip((y, dx, dwi, dwo), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_variant_override_leaves_the_block_alone(cuda_device, native_lib, dtype):
+    """b200_gemm_set_variant steers the GEMM's entry points; the block chooses for itself, in both types alike."""
+    x, w_in, w_out, dy = make(*SPLIT, dtype, cuda_device)
+    want = run(x, w_in, w_out, "silu", dy)
+    try:
+        for variant in ("cta1", "pair", "pair2m"):
+            _native.set_variant(variant)
+            assert all(torch.equal(p, q) for p, q in zip(run(x, w_in, w_out, "silu", dy), want))
+    finally:
+        _native.set_variant("auto")
