@@ -94,7 +94,8 @@ __device__ __forceinline__ ActValue activate(float g) {
     constexpr float kC = 0.79788456080286536f, kA = 0.044715f;
     const float s = sigmoid_approx(2.0f * kC * g * (1.0f + kA * g * g));
     r.f = g * s;
-    if (kSlope) r.slope = s + g * (2.0f * s * (1.0f - s)) * (kC * (1.0f + 3.0f * kA * g * g));
+    // Where g^2 is infinite, s (1 - s) is 0: the bound keeps 0 * infinity out.
+    if (kSlope) r.slope = s + g * (2.0f * s * (1.0f - s)) * fminf(kC * (1.0f + 3.0f * kA * g * g), 1.0e30f);
   }
   return r;
 }

@@ -471,3 +471,18 @@ def test_variant_override_leaves_the_block_alone(cuda_device, native_lib, dtype)
             assert all(torch.equal(p, q) for p, q in zip(run(x, w_in, w_out, "silu", dy), want))
     finally:
         _native.set_variant("auto")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 300, 4100])
+@pytest.mark.parametrize("kind", list(ffn.ACTIVATIONS))
+def test_gates_whose_square_overflows(cuda_device, native_lib, kind, rows):
+    """bf16 gates of +-1e20: the slope is 1 or 0, whatever g^2 is."""
+    x, w_in, w_out, dy = make(rows, 64, 72, 64, BF16, cuda_device)
+    x, w_in = x.clone(), w_in.clone()
+    x[:, 0] = 1.0
+    w_in[3, 0], w_in[70, 0] = 1e20, -1e20
+    ex = Exact(x, w_in, w_out, kind, dy)
+    for want, got in zip((ex.y, ex.dx, ex.dw_in, ex.dw_out), run(x, w_in, w_out, kind, dy)):
+        assert got.isfinite().all()
+        want.check(got)
