@@ -106,8 +106,7 @@ class _GatedFfn(torch.autograd.Function):
     def backward(ctx, dy):
         if plain_eager(dy):
             return *_backward(dy, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:3]), None
-        grads = torch.ops.tensorcore_gemm.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation)
-        return *(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None
+        return *_traced_backward(dy, ctx.saved_tensors, ctx.activation, ctx.needs_input_grad), None
 
 
 def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
@@ -119,7 +118,7 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
     (and, for the backward pass, g and u) are rounded to x's type.
     """
     if not plain_eager(x, w_in, w_out):
-        return torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, activation)[0]
+        return torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, activation, wants_grad(x, w_in, w_out))[0]
     _check(x, w_in, w_out, activation)
     if wants_grad(x, w_in, w_out):
         return _GatedFfn.apply(x, w_in, w_out, activation)
@@ -130,47 +129,59 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
 # The dispatcher operators
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("tensorcore_gemm::gated_ffn", mutates_args=())
-def _gated_ffn_op(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
-                  activation: str) -> tuple[torch.Tensor, torch.Tensor]:
-    """y and [g u] of `gated_ffn` (the latter is not differentiable)."""
+def _gated_ffn_op(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activation: str,
+                  save: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """y and [g u] of `gated_ffn` (the latter is not differentiable; without rows unless `save`d for the gradient)."""
     _check(x, w_in, w_out, activation)
     refuse_tangents(x, w_in, w_out)
-    return _forward(x, w_in, w_out, activation, True)
+    y, gate_up = _forward(x, w_in, w_out, activation, save)
+    return y, x.new_empty((0, 2 * _pad8(w_out.shape[1]))) if gate_up is None else gate_up
 
 
 @_gated_ffn_op.register_fake
-def _(x, w_in, w_out, activation):
+def _(x, w_in, w_out, activation, save=True):
     _check(x, w_in, w_out, activation)
-    rows = x.shape[:-1].numel()
+    rows = x.shape[:-1].numel() if save else 0
     return (torch.empty((*x.shape[:-1], w_out.shape[0]), dtype=x.dtype, device=x.device),
             torch.empty((rows, 2 * _pad8(w_out.shape[1])), dtype=x.dtype, device=x.device))
 
 
 @torch.library.custom_op("tensorcore_gemm::gated_ffn_backward", mutates_args=())
 def _gated_ffn_backward_op(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
-                           gate_up: torch.Tensor,
-                           activation: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                           gate_up: torch.Tensor, activation: str, need_x: bool = True, need_in: bool = True,
+                           need_out: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """dx, dw_in and dw_out (without elements where not needed)."""
     _check(x, w_in, w_out, activation)
     out_dim, hidden = w_out.shape
     dy = check_operand("dy", dy, (*x.shape[:-1], out_dim), x.dtype, x.device)
     gate_up = check_operand("gate_up", gate_up, (x.shape[:-1].numel(), 2 * _pad8(hidden)), x.dtype, x.device)
-    return _backward(dy, x, w_in, w_out, gate_up, activation, True, True, True)
+    grads = _backward(dy, x, w_in, w_out, gate_up, activation, need_x, need_in, need_out)
+    return tuple(x.new_empty(0) if g is None else g for g in grads)
 
 
 @_gated_ffn_backward_op.register_fake
-def _(dy, x, w_in, w_out, gate_up, activation):
-    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, w_in, w_out))
+def _(dy, x, w_in, w_out, gate_up, activation, need_x=True, need_in=True, need_out=True):
+    return tuple(torch.empty(t.shape if need else (0,), dtype=t.dtype, device=t.device)
+                 for t, need in ((x, need_x), (w_in, need_in), (w_out, need_out)))
+
+
+def _traced_backward(dy, saved, activation, needs):
+    """dx, dw_in and dw_out, those that `needs` names, through the dispatcher; None for the others."""
+    grads = torch.ops.tensorcore_gemm.gated_ffn_backward(dy, *saved, activation, *needs[:3])
+    return tuple(g if need else None for g, need in zip(grads, needs))
 
 
 def _setup_context(ctx, inputs, output) -> None:
-    x, w_in, w_out, activation = inputs
+    x, w_in, w_out, activation, save = inputs
     ctx.save_for_backward(x, w_in, w_out, output[1])
-    ctx.activation = activation
+    ctx.activation, ctx.saved = activation, save
     ctx.mark_non_differentiable(output[1])
 
 
 def _op_backward(ctx, dy, _dgate_up):
-    return *torch.ops.tensorcore_gemm.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation), None
+    if not ctx.saved:
+        raise RuntimeError("gated_ffn was called with save=False: it has no gradient")
+    return *_traced_backward(dy, ctx.saved_tensors, ctx.activation, ctx.needs_input_grad), None, None
 
 
 _gated_ffn_op.register_autograd(_op_backward, setup_context=_setup_context)

@@ -96,7 +96,7 @@ class _LayerNorm(torch.autograd.Function):
         if plain_eager(dy):
             dx, dw, db = _backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
         else:
-            dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype)
+            dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
         return dx if need_x else None, dw if need_w else None, db if need_b else None, None
 
 
@@ -138,19 +138,22 @@ def _(x, weight, bias, eps):
 
 @torch.library.custom_op("tensorcore_gemm::layer_norm_backward", mutates_args=())
 def _layer_norm_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
-                            wdtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                            wdtype: torch.dtype, need_weight: bool = True,
+                            need_bias: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """dx, dweight and dbias (the latter two without elements where not needed)."""
     _check(x, weight, None)
     if wdtype not in (x.dtype, torch.float32) or (weight is not None and weight.dtype != wdtype):
         raise RuntimeError("wdtype must be weight's dtype, and x's or float32")
     dy = check_operand("dy", dy, x.shape, x.dtype, x.device)
     rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
     stats = check_operand("stats", stats, (2, rows), torch.float32, x.device)
-    return _backward(dy, x, weight, stats, wdtype, True, True)
+    grads = _backward(dy, x, weight, stats, wdtype, need_weight, need_bias)
+    return tuple(x.new_empty(0, dtype=wdtype) if g is None else g for g in grads)
 
 
 @_layer_norm_backward_op.register_fake
-def _(dy, x, weight, stats, wdtype):
-    sums = [torch.empty(x.shape[-1], dtype=wdtype, device=x.device) for _ in range(2)]
+def _(dy, x, weight, stats, wdtype, need_weight=True, need_bias=True):
+    sums = [torch.empty(x.shape[-1] if need else 0, dtype=wdtype, device=x.device) for need in (need_weight, need_bias)]
     return torch.empty(x.shape, dtype=x.dtype, device=x.device), *sums
 
 
@@ -158,14 +161,14 @@ def _setup_context(ctx, inputs, output) -> None:
     x, weight, bias, _ = inputs
     ctx.save_for_backward(x, weight, output[1])
     ctx.wdtype = _wdtype(x, weight, bias)
-    ctx.has = (weight is not None, bias is not None)
     ctx.mark_non_differentiable(output[1])
 
 
 def _op_backward(ctx, dy, _dstats):
     x, weight, stats = ctx.saved_tensors
-    dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype)
-    return dx, dw if ctx.has[0] else None, db if ctx.has[1] else None, None
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dx, dw, db = torch.ops.tensorcore_gemm.layer_norm_backward(dy, x, weight, stats, ctx.wdtype, need_w, need_b)
+    return dx if need_x else None, dw if need_w else None, db if need_b else None, None
 
 
 _layer_norm_op.register_autograd(_op_backward, setup_context=_setup_context)

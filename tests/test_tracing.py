@@ -125,3 +125,65 @@ def test_negated_views(cuda_device, native_lib, name):
     call, args, _ = OPERATORS[name]
     operands = args(cuda_device, 1)[0]
     assert same(call(*(torch._neg_view(t) for t in operands)), call(*(-t for t in operands)))
+
+
+def _compiled(call):
+    return torch.compile(call, backend="aot_eager", fullgraph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(OPERATORS))
+def test_compiled(cuda_device, native_lib, name):
+    call, args, n = OPERATORS[name]
+    operands, grads = args(cuda_device, 4)
+    assert same(_compiled(call)(*operands), call(*operands))
+    results = []
+    for f in (_compiled(call), call):
+        leaves = [t.clone().requires_grad_() for t in operands]
+        results.append(torch.autograd.grad(f(*leaves)[:n], leaves, grads))
+    assert same(*results)
+
+
+class Record(TorchDispatchMode):
+    """Shapes of the outputs of the package's operators."""
+
+    def __init__(self):
+        super().__init__()
+        self.shapes = {}
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if "tensorcore_gemm" in str(func):
+            self.shapes[str(func).split(".")[1]] = [tuple(t.shape) for t in out]
+        return out
+
+
+@pytest.mark.gpu
+def test_only_what_is_needed_is_computed(cuda_device, native_lib):
+    """At the dispatcher, as in eager calls: nothing is kept without a gradient, no gradient of frozen weights."""
+    (x, wi, wo), (dy,) = _ffn_args(cuda_device, 5)
+    with Record() as seen:
+        y = ffn.gated_ffn(x, wi, wo)
+    assert seen.shapes == {"gated_ffn": [(9, 24), (0, 80)]}
+    for i in range(3):
+        operands = [x, wi, wo]
+        operands[i] = operands[i].clone().requires_grad_()
+        want, = torch.autograd.grad(ffn.gated_ffn(*operands), (operands[i],), dy)
+        with Record() as seen:
+            z = ffn.gated_ffn(*operands)
+            got, = torch.autograd.grad(z, (operands[i],), dy)
+        assert torch.equal(z, y) and torch.equal(got, want)
+        assert seen.shapes["gated_ffn"] == [(9, 24), (9, 80)]
+        assert seen.shapes["gated_ffn_backward"] == [tuple(t.shape) if j == i else (0,) for j, t in enumerate(operands)]
+    with pytest.raises(RuntimeError, match="save=False"):
+        leaf = x.clone().requires_grad_()
+        torch.ops.tensorcore_gemm.gated_ffn(leaf, wi, wo, "silu", False)[0].sum().backward()
+    (x, w, b), (dy,) = _norm_args(cuda_device, 5)
+    for i in range(3):
+        operands = [x, w, b]
+        operands[i] = operands[i].clone().requires_grad_()
+        want, = torch.autograd.grad(norm.layer_norm(*operands), (operands[i],), dy)
+        with Record() as seen:
+            got, = torch.autograd.grad(norm.layer_norm(*operands), (operands[i],), dy)
+        assert torch.equal(got, want)
+        assert seen.shapes["layer_norm_backward"] == [(9, 72), (72,) if i == 1 else (0,), (72,) if i == 2 else (0,)]
