@@ -709,7 +709,9 @@ __global__ void __launch_bounds__(kThreads)
     T* d = dlogits + row * ldd;
     const int64_t target = targets[row];
     const float2 st = stats[row];
-    const float gl = g_logprob && target != ignore ? g_logprob[row] : 0.0f;
+    float gl = g_logprob && target != ignore ? g_logprob[row] : 0.0f;
+    // A target outside the vocabulary: the log probability is NaN, and so is what follows from it.
+    if (gl != 0.0f && (target < 0 || target >= vocab)) gl = __uint_as_float(0x7fffffffu);
     const RowGrad r{-st.x, -st.y, entropy[row], gl, g_entropy ? g_entropy[row] : 0.0f};
     if (st.x == kNegInf) {
       // No probability anywhere: nothing depends on the logits.

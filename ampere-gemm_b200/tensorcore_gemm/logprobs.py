@@ -114,8 +114,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0,
     int64 or int32.  Also gives each row's entropy and, for top_k > 0 (at most
     MAX_TOP), the top_k largest log probabilities with their indices, equal
     logits by lower index.  A target equal to ignore_index has log probability
-    0 and no gradient through it; another one outside [0, V) gives NaN.  A row
-    of -inf throughout has log probability -inf, entropy 0 and gradient 0.
+    0 and no gradient through it; another one outside [0, V) gives NaN, and a
+    NaN gradient to its row unless the log probability's is 0.  A row of -inf
+    throughout has log probability -inf, entropy 0 and gradient 0.
     Differentiable in the logits through logprobs and entropy (once); the
     alternatives are not differentiable.
     """

@@ -237,7 +237,9 @@ B200_API int b200_token_logprobs_fwd(const void* logits, const int64_t* targets,
 /*
  * The gradient of the logits (pitch ldd, of `dtype`) from those of the log
  * probabilities and of the entropies (rows floats each, either may be NULL).
- * Rows whose target is ignore_index get the entropy's part only.
+ * Rows whose target is ignore_index get the entropy's part only; rows whose
+ * target is outside [0, vocab) otherwise are NaN unless their log probability's
+ * gradient is 0.
  */
 B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
                                      const float* entropy, const float* g_logprob, const float* g_entropy,

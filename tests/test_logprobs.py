@@ -462,3 +462,24 @@ def test_backward_operator_refusals(cuda_device, native_lib):
                         ((x.double(), t, stats, ent, g, g), "logits must")]:
         with pytest.raises(RuntimeError, match=match):
             op(*args, -100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(6, 600), (6, 40000), (1300, 600)])
+def test_invalid_targets_have_no_finite_gradient(cuda_device, native_lib, rows, vocab):
+    """The gradient of a NaN log probability is NaN, not that of -lse; rows that do not use it are as they were."""
+    x, t = make(rows, vocab, F32, cuda_device)
+    t[1], t[2], t[3], t[4] = vocab, -1, 2 ** 40, -1
+    gl, gh = (torch.randn(rows, device=cuda_device) for _ in range(2))
+    gl[4] = 0.0
+    leaf = x.clone().requires_grad_()
+    r = logprobs.token_logprobs(leaf, t)
+    dx, = torch.autograd.grad((r.logprobs, r.entropy), (leaf,), (gl, gh), retain_graph=True)
+    assert r.logprobs[1:5].isnan().all() and dx[1:4].isnan().all()
+    t2 = t.clone()
+    t2[4] = -100
+    good = [i for i in range(rows) if i not in (1, 2, 3)]
+    Exact(x[good], t2[good]).check_grad(dx[good], gl[good], gh[good])
+    dx, = torch.autograd.grad(r.entropy, (leaf,), gh)
+    t2[1:5] = -100
+    Exact(x, t2).check_grad(dx, 0 * gl, gh)
