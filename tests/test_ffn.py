@@ -486,3 +486,67 @@ def test_gates_whose_square_overflows(cuda_device, native_lib, kind, rows):
     for want, got in zip((ex.y, ex.dx, ex.dw_in, ex.dw_out), run(x, w_in, w_out, kind, dy)):
         assert got.isfinite().all()
         want.check(got)
+
+
+# Every product on the GEMM's tiles (256 rows; 128 columns of gate and up, 256 of da; 128 deep): less than a tile and
+# several in each direction, hidden widths off 8, one stage of depth and several, more tiles than pairs of SMs.
+MANY_ROWS = [(4097, 8, 8, 8), (4100, 64, 267, 72), (4353, 200, 1000, 136), (4609, 520, 2731, 264), (5000, 136, 135, 640)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(ffn.ACTIVATIONS))
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size", MANY_ROWS)
+def test_many_rows(cuda_device, native_lib, size, dtype, kind):
+    """The epilogues of the pair kernel, forward and backward, and the GEMMs beside them."""
+    for product, args in products(*size).items():
+        assert _native.gated_ffn_plan(*args, product) == (0, 0, 0), product
+    x, w_in, w_out, dy = make(*size, dtype, cuda_device)
+    check_all(x, w_in, w_out, kind, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(ffn.ACTIVATIONS))
+def test_many_rows_strided_and_repeated(cuda_device, native_lib, kind):
+    """Operands with pitches and off 16 bytes, a NaN row, the same bits from run to run."""
+    rows, dim, hidden, out_dim = 4201, 136, 530, 200
+    x, w_in, w_out, dy = make(rows, dim + 8, hidden, out_dim + 8, BF16, cuda_device)
+    for a, b in ((8, 8), (3, 1)):
+        xs, wi, wo, dys = x[:, a:a + dim], w_in[:, b:b + dim], w_out[b:b + out_dim], dy[:, a:a + out_dim]
+        ex = Exact(xs, wi, wo, kind, dys)
+        leaves = [t.detach().requires_grad_() for t in (xs, wi, wo)]
+        y = ffn.gated_ffn(*leaves, activation=kind)
+        first = (y, *torch.autograd.grad(y, leaves, dys))
+        for want, got in zip((ex.y, ex.dx, ex.dw_in, ex.dw_out), first):
+            want.check(got)
+        y = ffn.gated_ffn(*leaves, activation=kind)
+        assert all(torch.equal(p, q) for p, q in zip(first, (y, *torch.autograd.grad(y, leaves, dys))))
+    bad = xs.clone()
+    bad[7, 5] = float("nan")
+    y = ffn.gated_ffn(bad, wi, wo, activation=kind)
+    assert y[7].isnan().all() and torch.equal(torch.cat([y[:7], y[8:]]), torch.cat([first[0][:7], first[0][8:]]))
+
+
+# Sizes whose products run on each kernel of the GEMM, with the product and the kernel that it is there for.
+KERNELS = [((4100, 2008, 520, 2008), {"out": "pair2m", "in_grad": "pair2m"}),
+           ((5000, 1000, 520, 1000), {"out": "pair2m_192", "in_grad": "pair2m_192"}),
+           ((5000, 1500, 520, 1500), {"out": "pair2m_224", "in_grad": "pair2m_224"}),
+           ((4100, 520, 520, 2600), {"out": "pair", "in_grad": "cta1", "dw_in": "pair", "dw_out": "pair"}),
+           ((5000, 2008, 520, 520), {"out": "cta1", "in_grad": "pair"}),
+           ((4100, 1500, 2600, 520), {"dw_in": "pair2m"}), ((4100, 2600, 1500, 520), {"dw_in": "pair2m_224"}),
+           ((4100, 520, 2600, 2600), {"dw_out": "pair2m_224"}), ((4100, 520, 3500, 2600), {"dw_out": "cta1"})]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size,kernels", KERNELS)
+def test_every_gemm_kernel(cuda_device, native_lib, size, kernels, dtype):
+    """The wide pair in its three widths, the pair and the one-CTA kernel behind the block, in both types."""
+    rows, dim, hidden, out_dim = size
+    args = dict(products(*size), dw_in=(2 * hidden, dim, rows), dw_out=(out_dim, hidden, rows))
+    for product, kernel in kernels.items():
+        assert _native.plan(*args[product])[0] == kernel
+        if product in _native.FFN_PRODUCTS:
+            assert _native.gated_ffn_plan(*args[product], product) == (0, 0, 0)
+    x, w_in, w_out, dy = make(*size, dtype, cuda_device)
+    check_all(x, w_in, w_out, "silu", dy)
