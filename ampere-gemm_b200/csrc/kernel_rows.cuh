@@ -332,10 +332,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       ++issued;
       if (++stage == sh.stages) { stage = 0; phase ^= 1u; }
     }
-    if (!ok && lane == 0) {
-      // Let every load still in flight land before the CTA leaves.
-      for (int it = max(0, issued - sh.stages); it < issued; ++it)
-        mbar_wait_drain(&full_bar[it % sh.stages], static_cast<uint32_t>(it / sh.stages) & 1u);
+    if (lane == 0) {
+      // Every load lands before the CTA leaves, also where the issuer has given
+      // up and nothing else waits for them.
+      for (int it = max(0, issued - sh.stages); it < issued; ++it) {
+        uint64_t* bar = &full_bar[it % sh.stages];
+        const uint32_t parity = static_cast<uint32_t>(it / sh.stages) & 1u;
+        if (!mbar_wait(bar, parity, kDevTimeoutProducer)) mbar_wait_drain(bar, parity);
+      }
     }
   } else if (warp == 1) {
     const uint32_t el = elect_lane();
