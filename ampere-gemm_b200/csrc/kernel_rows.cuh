@@ -280,6 +280,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
+  // The bounded waits below do not run while the kernel before this one does.
+  if (warp != 0) griddep_wait();
 
   if (warp == 0) {
     const uint32_t el = elect_lane();
