@@ -539,7 +539,7 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   }
   if (!x || !w_in || !w_out || !y || ldx < dim || ldw_in < dim || ldw_out < hidden || ldy < out_dim)
     return B200_ERR_INVALID_ARGUMENT;
-  if (gate_up && !aligned16(gate_up)) return B200_ERR_MISALIGNED;
+  if ((gate_up && !aligned16(gate_up)) || !aligned_to(2, x, w_in, w_out, y)) return B200_ERR_MISALIGNED;
   const bool copies = !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) || !pitch_ok(w_out, ldw_out) || !pitch_ok(y, ldy);
   if (!workspace_ok(workspace, workspace_bytes, b200_gated_ffn_workspace_size(rows, dim, hidden, out_dim, 0, copies)))
     return B200_ERR_WORKSPACE;
@@ -584,7 +584,7 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
   }
   if (!dy || !x || !w_in || !w_out || !gate_up || lddy < out_dim || ldx < dim || ldw_in < dim || ldw_out < hidden)
     return B200_ERR_INVALID_ARGUMENT;
-  if (!aligned16(gate_up)) return B200_ERR_MISALIGNED;
+  if (!aligned16(gate_up) || !aligned_to(2, dy, x, w_in, w_out, dx, dw_in, dw_out)) return B200_ERR_MISALIGNED;
   const bool copies = !pitch_ok(dy, lddy) || !pitch_ok(x, ldx) || !pitch_ok(w_in, ldw_in) ||
                       !pitch_ok(w_out, ldw_out) || (dx && !pitch_ok(dx, lddx)) ||
                       (dw_in && !pitch_ok(dw_in, lddw_in)) || (dw_out && !pitch_ok(dw_out, lddw_out));

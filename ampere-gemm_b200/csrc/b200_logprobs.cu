@@ -762,6 +762,7 @@ __global__ void __launch_bounds__(kThreads)
 
 int cuda_code(cudaError_t e) { return e == cudaSuccess ? B200_OK : B200_ERR_CUDA; }
 
+int dtype_size(int d) { return d == B200_DTYPE_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == B200_DTYPE_F16 || d == B200_DTYPE_BF16 || d == B200_DTYPE_F32; }
 
 template <typename Fn>
@@ -812,6 +813,9 @@ extern "C" int b200_token_logprobs_fwd(const void* logits, const int64_t* target
   if (vocab == 0 || !logits || !targets || !logprob || !entropy || ld < vocab ||
       (top > 0 && (!top_logprob || !top_index)))
     return B200_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(dtype_size(dtype), logits) || !aligned_to(8, targets, stats, top_index) ||
+      !aligned_to(4, logprob, entropy, top_logprob))
+    return B200_ERR_MISALIGNED;
   const int64_t need = b200_token_logprobs_workspace_size(rows, vocab, top);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
     return B200_ERR_WORKSPACE;
@@ -853,6 +857,9 @@ extern "C" int b200_token_logprobs_bwd(const void* logits, const int64_t* target
   if (rows == 0 || vocab == 0) return B200_OK;
   if (!logits || !targets || !stats || !entropy || !dlogits || ld < vocab || ldd < vocab)
     return B200_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(dtype_size(dtype), logits, dlogits) || !aligned_to(8, targets, stats) ||
+      !aligned_to(4, entropy, g_logprob, g_entropy))
+    return B200_ERR_MISALIGNED;
   DeviceInfo dev;
   if (int rc = current_device_info(dev)) return rc;
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;

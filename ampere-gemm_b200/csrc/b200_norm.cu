@@ -796,6 +796,8 @@ extern "C" int b200_layer_norm_fwd(const void* x, const void* w, const void* b, 
   if (int rc = check_norm_args(rows, cols, dtype, wdtype)) return rc;
   if (rows == 0 || cols == 0) return B200_OK;
   if (!x || !y || ldx < cols || ldy < cols) return B200_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(dtype_size(dtype), x, y) || !aligned_to(dtype_size(wdtype), w, b) || !aligned_to(4, mean, rstd))
+    return B200_ERR_MISALIGNED;
   DeviceInfo dev;
   if (int rc = current_device_info(dev)) return rc;
   if (!dev.sm100) return B200_ERR_UNSUPPORTED_DEVICE;
@@ -855,6 +857,9 @@ extern "C" int b200_layer_norm_bwd(const void* dy, const void* x, const void* w,
   if (int rc = check_norm_args(rows, cols, dtype, wdtype)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   if (cols == 0) return B200_OK;
+  if (!aligned_to(dtype_size(dtype), dy, x, dx) || !aligned_to(dtype_size(wdtype), w, dw, db) ||
+      !aligned_to(4, mean, rstd))
+    return B200_ERR_MISALIGNED;
   if (rows == 0) {
     const size_t bytes = (size_t)cols * dtype_size(wdtype);
     if (dw && cudaMemsetAsync(dw, 0, bytes, stream) != cudaSuccess) return B200_ERR_CUDA;

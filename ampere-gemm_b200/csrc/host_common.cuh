@@ -95,6 +95,12 @@ cudaError_t launch_gemm(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sm
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Every pointer on a multiple of `bytes` (NULL: fine).
+template <typename... P>
+bool aligned_to(uintptr_t bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ... | 0) & (bytes - 1)) == 0;
+}
+
 bool pitch_ok(const void* p, int64_t ld) { return aligned16(p) && (ld % 8) == 0; }
 
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }

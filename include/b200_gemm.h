@@ -182,7 +182,9 @@ B200_API int b200_ipc_free(void* ptr);
 B200_API int b200_ipc_open(const void* handle, void** ptr);
 B200_API int b200_ipc_close(void* ptr);
 
-/* Element types of the operators below. */
+/* Element types of the operators below.  Each of their pointers is aligned to
+ * its elements at least, stats of b200_token_logprobs_* to 8 bytes;
+ * B200_ERR_MISALIGNED otherwise. */
 #define B200_DTYPE_F16 0
 #define B200_DTYPE_BF16 1
 #define B200_DTYPE_F32 2

@@ -158,3 +158,24 @@ def test_launch_plan_forced_variant_and_errors(native_lib):
         _native.set_variant("auto")
     with pytest.raises(RuntimeError):
         _native.plan(0, 8, 8)
+
+
+def test_operators_refuse_misaligned_pointers_without_gpu(native_lib):
+    """Pointers that are not aligned to their elements come back as an error, before any launch."""
+    p, odd = 4096, {}
+    norm = [p] * 6 + [4, 64, 64, 64, 1, 2, 1e-5, None]                      # x, w, b, y, mean, rstd; bf16, fp32 weights
+    odd["b200_layer_norm_fwd"] = norm, {0: 1, 1: 2, 2: 2, 3: 1, 4: 2, 5: 2}
+    grad = [p] * 8 + [4, 64, 64, 64, 64, 1, 2, p, 1 << 30, None]            # dy, x, w, mean, rstd, dx, dw, db
+    odd["b200_layer_norm_bwd"] = grad, {0: 1, 1: 1, 2: 2, 3: 2, 4: 2, 5: 1, 6: 2, 7: 2}
+    lp = [p] * 7 + [4, 100, 100, 2, -100, 2, None, 0, None]                 # logits, targets, logprob, entropy, stats, top
+    odd["b200_token_logprobs_fwd"] = lp, {0: 2, 1: 4, 2: 2, 3: 2, 4: 4, 5: 2, 6: 4}
+    lpg = [p] * 7 + [4, 100, 100, 100, -100, 0, None]                       # logits, targets, stats, entropy, gl, gh, dx
+    odd["b200_token_logprobs_bwd"] = lpg, {0: 1, 1: 4, 2: 4, 3: 2, 4: 2, 5: 2, 6: 1}
+    ffn = [p] * 5 + [4, 64, 64, 64, 64, 64, 64, 64, 0, 1, p, 1 << 30, None]
+    odd["b200_gated_ffn_fwd"] = ffn, {0: 1, 1: 1, 2: 1, 3: 1, 4: 8}
+    fgr = [p] * 8 + [4, 64, 64, 64] + [64] * 7 + [0, 1, p, 1 << 30, None]
+    odd["b200_gated_ffn_bwd"] = fgr, {0: 1, 1: 1, 2: 1, 3: 1, 4: 8, 5: 1, 6: 1, 7: 1}
+    for name, (args, offsets) in odd.items():
+        for i, off in offsets.items():
+            bad = [a + off if j == i else a for j, a in enumerate(args)]
+            assert getattr(native_lib, name)(*bad) == 2, (name, i)
