@@ -17,6 +17,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100) GPU")
 
 
+def pytest_collection_modifyitems(items):
+    """Tests against the reference's own kernels and package fail where its sources were not there to build them from.
+    They come last, so that a run that stops at its first failure has run all the others."""
+    needs_reference = {"ref_lib", "reference_cublas"}
+    items.sort(key=lambda item: not needs_reference.isdisjoint(getattr(item, "fixturenames", ())))
+
+
 @pytest.fixture(scope="session")
 def native_lib():
     """Build (if stale and nvcc is present) and load libb200gemm.so."""
