@@ -117,11 +117,11 @@ __global__ void copy_jobs_kernel(const __grid_constant__ CopyJobs jobs) {
   }
 }
 
-int run_copies(const CopyJobs& jobs, cudaStream_t stream) {
+int run_copies(const CopyJobs& jobs, int sm_count, cudaStream_t stream) {
   if (jobs.n == 0) return B200_OK;
   int64_t rows = 1;
   for (int i = 0; i < jobs.n; ++i) rows = std::max(rows, jobs.job[i].rows + jobs.job[i].zero_rows);
-  const cudaError_t e = launch_gemm(copy_jobs_kernel, dim3((unsigned)std::min<int64_t>(rows, 8 * 148), jobs.n),
+  const cudaError_t e = launch_gemm(copy_jobs_kernel, dim3((unsigned)std::min<int64_t>(rows, 8 * sm_count), jobs.n),
                                     dim3(128), 0, stream, jobs);
   return e == cudaSuccess ? B200_OK : B200_ERR_CUDA;
 }
@@ -555,7 +555,7 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   x = readable(x, ldx, rows, dim, ws, before);
   w_in = readable(w_in, ldw_in, 2 * hidden, dim, ws, before);
   w_out = readable(w_out, ldw_out, out_dim, hidden, ws, before);
-  if (int rc = run_copies(before, stream)) return rc;
+  if (int rc = run_copies(before, dev.sm_count, stream)) return rc;
   const GateShape s{(int)rows, (int)hidden, (int)dim, (int)hp};
   int rc = (bf16 ? b200::gate_up<true> : b200::gate_up<false>)(
       x, ldx, w_in, ldw_in, a, static_cast<uint16_t*>(gate_up), activation, s, dev, stream);
@@ -564,7 +564,7 @@ extern "C" int b200_gated_ffn_fwd(const void* x, const void* w_in, const void* w
   // w_out was written two kernels ago at the latest: its loads may start early.
   rc = (bf16 ? product<true, false> : product<false, false>)(a, hp, w_out, ldw_out, y, ldy, (int)rows, (int)out_dim,
                                                              (int)hidden, true, dev, split_ws, stream);
-  return rc ? rc : run_copies(after, stream);
+  return rc ? rc : run_copies(after, dev.sm_count, stream);
 }
 
 extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_in, const void* w_out,
@@ -618,7 +618,7 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
       ldw_in = pad8(dim);
     }
   }
-  if (int rc = run_copies(before, stream)) return rc;
+  if (int rc = run_copies(before, dev.sm_count, stream)) return rc;
   const GateShape s{(int)rows, (int)hidden, (int)out_dim, (int)hp};
   int rc = (bf16 ? gate_bwd<true> : gate_bwd<false>)(dy, lddy, w_out, ldw_out, static_cast<const uint16_t*>(gate_up),
                                                      dgu, a, activation, s, dev, stream);
@@ -645,5 +645,5 @@ extern "C" int b200_gated_ffn_bwd(const void* dy, const void* x, const void* w_i
                     B200_B_ROW_MAJOR, split_ws, stream_ptr);
     if (rc) return rc;
   }
-  return run_copies(after, stream);
+  return run_copies(after, dev.sm_count, stream);
 }

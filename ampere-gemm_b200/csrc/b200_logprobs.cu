@@ -779,6 +779,8 @@ unsigned row_blocks(int64_t rows, int per_block) {
 
 // Slices a row is cut into: enough blocks for the device when rows are few
 // (4096 logits each at least), and none longer than the selection can hold.
+// The blocks are a constant, four for each SM of a B200, because the workspace's
+// size, which is asked for without a device, follows from them.
 int64_t row_slices(int64_t rows, int64_t vocab, int top) {
   constexpr int64_t kBlocks = 4 * 148, kLeast = 4096;
   int64_t s = std::max<int64_t>(1, std::min(kBlocks / std::max<int64_t>(rows, 1), vocab / kLeast));
