@@ -114,8 +114,13 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
 
     All float16 or all bfloat16.  activation: "silu", "gelu" or "gelu_tanh".
     Any sizes and strides; operands whose rows do not start on 16 bytes are
-    copied first.  Differentiable in x, w_in and w_out (once).  a = act(g) u
-    (and, for the backward pass, g and u) are rounded to x's type.
+    copied first.  Differentiable in x, w_in and w_out (once).
+
+    Between the launches a = act(g) u, and for the gradients g, u, dg and du,
+    are rounded to x's type.  In float16 such a value past 65504 is infinite and
+    one below 6e-5 loses bits, where 32 bits would have held it: the range of
+    any float16 network, which losses are scaled for; bfloat16 has that of 32
+    bits.
     """
     if not plain_eager(x, w_in, w_out):
         return torch.ops.tensorcore_gemm.gated_ffn(x, w_in, w_out, activation, wants_grad(x, w_in, w_out))[0]

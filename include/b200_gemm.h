@@ -254,7 +254,7 @@ B200_API int b200_token_logprobs_bwd(const void* logits, const int64_t* targets,
  *   g = x Wg^T, u = x Wu^T, a = act(g) u, y = a w_out^T
  * for `rows` rows of x, all of `dtype` (B200_DTYPE_F16 or B200_DTYPE_BF16) with
  * fp32 accumulation and activation; a is rounded to `dtype` between the two
- * launches.  gate_up (may be NULL) receives g and u for the backward call: rows
+ * launches (in fp16 to infinity past 65504, as g, u, dg and du are).  gate_up (may be NULL) receives g and u for the backward call: rows
  * of 2 P elements, P = hidden rounded up to a multiple of 8, 16-byte aligned.
  * Other operands are taken at any alignment and pitch; those whose rows do not
  * start on 16 bytes cost a copy.  The workspace (256-byte aligned) must not be

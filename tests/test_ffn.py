@@ -550,3 +550,29 @@ def test_every_gemm_kernel(cuda_device, native_lib, size, kernels, dtype):
             assert _native.gated_ffn_plan(*args[product], product) == (0, 0, 0)
     x, w_in, w_out, dy = make(*size, dtype, cuda_device)
     check_all(x, w_in, w_out, "silu", dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 300, 4100])
+def test_range_between_the_launches(cuda_device, native_lib, rows):
+    """a, dg and du past fp16's range are infinite in fp16, in their rows only; bf16 holds them."""
+    for dtype in (F16, BF16):
+        x, w_in, w_out, dy = make(rows, 64, 72, 64, dtype, cuda_device)
+        x, w_in, dy = x.clone(), w_in.clone(), dy.clone()
+        w_in[5] = w_in[77] = 0.0
+        w_in[5, 0] = w_in[77, 0] = 1.0                       # g and u of unit 5
+        x[1, 0] = 400.0                                      # a = 160000
+        x[2, 0], dy[2] = 200.0, 4000.0 * w_out[:, 5].sign()  # a = 40000, dg = da u far past the range
+        y, dx, dwi, dwo = run(x, w_in, w_out, "silu", dy)
+        rest = [i for i in range(rows) if i not in (1, 2)]
+        if rest:
+            ex = Exact(x[rest], w_in, w_out, "silu", dy[rest])
+            ex.y.check(y[rest])
+            ex.dx.check(dx[rest])
+        if dtype == F16:
+            assert not y[1].isfinite().any() and not dx[2].isfinite().all() and not dwo.isfinite().all()
+        else:
+            ex = Exact(x, w_in, w_out, "silu", dy)
+            for want, got in ((ex.y, y), (ex.dx, dx), (ex.dw_in, dwi), (ex.dw_out, dwo)):
+                assert got.isfinite().all()
+                want.check(got)
