@@ -290,7 +290,9 @@ RowsLaunch rows_launch(int tokens, int n, int n_pad, int k, bool gate, const Row
   // At least the share of an SM's shared memory that the CTA takes of its
   // TMEM: CTAs that share an SM then find TMEM for all of them.  One that
   // waited for TMEM would hold up its cluster, and clusters that each hold what
-  // another one's CTA waits for would never end.
+  // another one's CTA waits for would never end.  (The whole SM for every CTA of
+  // a cluster would do too, but successive launches no longer overlap: 24 x 512
+  // x 1408 10.4 -> 12.6 us.)
   l.smem = std::max(l.smem, (int)((int64_t)l.tmem_cols * kSmSmem / kSmTmemCols) - kCtaSmem);
   return l;
 }
