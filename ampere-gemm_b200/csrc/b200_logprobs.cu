@@ -16,10 +16,11 @@
 // sums), the backward reads them and writes their gradient once.  In the way of
 // that stand one exponential a logit (16-bit logits: the units that compute them
 // are 62 % busy, fp32 ones half of that) and, with alternatives, the selection at
-// a row's end.  Measured, of the measured copy bandwidth: 4096 x 50257 bf16
-// forward 78 us (0.81), top 5 107 us (0.59), top 64 165 us; 2048 x 50257 fp32
-// 66 us (0.95); 8192 x 65536 bf16 forward and backward 545 us (0.90).  Sums are in
-// fp32 in a fixed order.  More loads on their way (eight groups a thread, 64
+// a row's end.  Measured back to back over inputs that L2 does not hold, of the
+// measured copy bandwidth: 4096 x 50257 bf16 forward 79 us (0.79), top 5 109 us
+// (0.57), top 64 168 us; 2048 x 50257 fp32 69 us (0.91); 8192 x 65536 bf16 forward
+// 182 us (0.90), backward 316 us (1.04).  Sums are in fp32 in a fixed order.
+// More loads on their way (eight groups a thread, 64
 // registers) took 91 us instead of 78, all loads of a row's end at once with 48
 // registers 83: both spill.
 #include <algorithm>
@@ -46,9 +47,9 @@ constexpr int kTopSlice = 65536;
 // Rows this short go to a warp each when there are enough of them to give every
 // SM a block, with kWarpTop alternatives at most: no barriers, and eight rows'
 // loads side by side.  bf16, us, a block a row -> a warp a row: 100000 x 500
-// forward 270 -> 63, backward 214 -> 63, top 5 724 -> 130; 20000 x 5000 98 -> 53,
-// 98 -> 79, 179 -> 73 (top 20 195 -> 108); 8192 x 8192 40 -> 32, 47.5 -> 50.5 (2000 x 8192: 11 -> 13
-// backward).
+// forward 270 -> 65, backward 214 -> 74, top 5 724 -> 131; 20000 x 5000 98 -> 54,
+// 98 -> 83, 179 -> 75 (top 20 195 -> 110); 8192 x 8192 40 -> 32, 47.5 -> 50.5
+// (2000 x 8192: 11 -> 13 backward).
 constexpr int kWarpRow = 6144;
 constexpr int kWarpTop = 24;
 // Slices of a row at most when alternatives are wanted: one a thread of the join.

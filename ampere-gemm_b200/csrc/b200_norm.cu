@@ -7,8 +7,8 @@
 //
 // Bound by memory: forward reads x and writes y once, backward reads x and dy
 // and writes dx once.  Measured, of the measured copy bandwidth: 20011 x 5120
-// bf16 forward 69 us (0.91); 16384 x 4096 bf16 with fp32 weights 47 us forward
-// (0.88), 76 + 5 backward (0.76); 8 x 4096 fp16 3 us.  What remains is the issue
+// bf16 forward 71 us (0.88); 16384 x 4096 bf16 with fp32 weights 49 us forward
+// (0.84), 77 + 5 backward (0.75); 8 x 4096 fp16 3.5 us (L2 cold).  What remains is the issue
 // of instructions (half the slots) and the wait for a row's sums.  A row stays
 // in registers, in its own type, between the passes over it; all sums are in
 // fp32 and y, dx, dw and db are rounded once.  Every sum has a fixed order, so

@@ -5,9 +5,9 @@
 //
 // Activations are computed in fp32 from the fp32 accumulators (forward) or
 // from the saved 16-bit g and u (backward).  Both hide behind the MMAs of the
-// next tile where the product is deep: 4001 x 4096 x 12288 fp16 forward 547 us
-// (0.90 of the measured peak), 8192 x 4096 x 11008 bf16 forward with g and u
-// stored 985 us (0.91), backward 627 us (0.72).
+// next tile where the product is deep: 4001 x 4096 x 12288 fp16 forward 538 us
+// (0.91 of the measured peak), 8192 x 4096 x 11008 bf16 forward with g and u
+// stored 978 us (0.92), backward 607 us (0.74).
 #pragma once
 
 #include "gemm_common.cuh"

@@ -7,7 +7,8 @@
 Both input projections, the activation and the product are one launch, the
 output projection a second one; so is da with dg, du and a in the backward
 pass.  `gated_ffn` is the entry point; `torch.ops.tensorcore_gemm.gated_ffn`
-is the same operator for tracers (it also returns [g u]).  fp16 or bf16
+is the same operator for tracers (it also returns [g u], without rows where
+its `save` is false).  fp16 or bf16
 operands, fp32 accumulation and activation; CUDA tensors only, nothing falls
 back to another implementation.
 """
